@@ -10,3 +10,5 @@ from .models import (  # noqa: F401
 )
 from .conditioner import GraphConditioner  # noqa: F401
 from .collate import CollatedBatch, MinibatchStream, segment_ids  # noqa: F401
+from .losses import balance_loss, linear_cross_entropy  # noqa: F401
+from .optim import AdamW, adamw_step_  # noqa: F401

@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(_HERE, "libceeg.so")
 
 CEEG_F32, CEEG_BF16 = 0, 1
 
-_c_i64, _c_int, _c_f32, _c_u64, _c_sz, _vp = C.c_int64, C.c_int, C.c_float, C.c_uint64, C.c_size_t, C.c_void_p
+_c_i64, _c_int, _c_f32, _c_f64, _c_u64, _c_sz, _vp = C.c_int64, C.c_int, C.c_float, C.c_double, C.c_uint64, C.c_size_t, C.c_void_p
 
 # name -> (restype, argtypes); mirrors include/ceeg.h one to one
 SIGNATURES = {
@@ -111,6 +111,16 @@ SIGNATURES = {
     "ceeg_neg_filter_bits": (_c_int, [_c_i64]),
     "ceeg_neg_filter_build": (_c_int, [_vp, _vp, _c_i64, _c_int, _vp, _vp]),
     "ceeg_neg_sample_uniform_filtered": (_c_int, [_vp, _vp, _c_i64, _c_i64, _c_u64, _vp, _c_int, _vp, _vp, _vp]),
+    "ceeg_linear_ce_fwd_ws_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_int]),
+    "ceeg_linear_ce_bwd_ws_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_int]),
+    "ceeg_linear_ce_fwd": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _vp, _vp, _vp, _vp, _c_sz, _vp]),
+    "ceeg_linear_ce_bwd": (_c_int, [_vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _c_sz, _vp]),
+    "ceeg_balance_ws_bytes": (_c_sz, [_c_i64, _c_int]),
+    "ceeg_balance_fwd": (_c_int, [_vp, _c_i64, _c_int, _vp, _c_int, _c_i64, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _c_sz, _vp]),
+    "ceeg_balance_bwd": (_c_int, [_vp, _c_i64, _c_int, _c_i64, _c_int, _vp, _vp, _vp, _vp, _vp]),
+    "ceeg_adamw_block": (_c_int, []),
+    "ceeg_adamw_step": (_c_int, [_c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_f64, _c_f64, _c_f64, _c_f64, _c_f64, _c_i64, _vp, _vp,
+                                 _c_u64, _vp]),
 }
 
 _lib = None

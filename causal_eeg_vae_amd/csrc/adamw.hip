@@ -1,0 +1,294 @@
+// AdamW over a list of tensors in one launch, first and second moment in 32 bits or in 8:
+//   m = b1 m + (1 - b1) g;   v = b2 v + (1 - b2) g^2;   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+// 8 bits: m and sqrt(v) (the root halves the range of exponents that has to fit) are e4m3 numbers times one fp32 scale per 256 consecutive elements, the
+// block's largest magnitude / 448.  A step changes v by 1 - b2 of itself, far less than half a step of an 8-bit number, so rounding to
+// nearest would hold v where it is for ever; a magnitude is therefore rounded UP with the probability that keeps the expectation - of m, and
+// of v itself: keeping that of the root would add the rounding's variance to v, up to 2^-8 of it a step, which outgrows the decay 1 - b2.
+// 16 random bits of Philox per value.  sqrt(v) > 0 never becomes 0: a denominator that vanishes while m does not would blow the next step up.
+// Bound: HBM bytes (fp32 28 per element; 8 bits 16 with fp32 parameters, 10 with bf16).  A wave takes one block of 256 elements, 4 per lane - 16-byte loads, the
+// block's maximum by one butterfly, one Philox call per lane for its four elements - so the 8-bit form needs no LDS and no barrier.
+// The tensors' pointers travel in the kernel arguments: no table in device memory, nothing to copy or to keep alive.
+#include <math.h>
+#include "ceeg_internal.h"
+
+namespace {
+constexpr int AW_THREADS = 256;
+constexpr int AW_BLOCK = 256;   // elements per wave step and per 8-bit scale
+constexpr int AW_LIST = 56;     // tensors per launch: 56 * 60 + 80 bytes stay below the 4096 bytes of kernel arguments
+constexpr float AW_TOP = 448.f; // largest e4m3 number
+constexpr float AW_PER_TOP = 1.f / 448.f;
+constexpr float AW_TINY = 0x1p-100f;
+
+struct AwList {
+  void* p[AW_LIST];
+  const void* g[AW_LIST];
+  void* m[AW_LIST];
+  void* v[AW_LIST];
+  float* ms[AW_LIST];
+  float* vs[AW_LIST];
+  int64_t n[AW_LIST];
+  uint32_t first[AW_LIST];  // first workgroup of the tensor
+  int32_t count;
+};
+struct AwHyper {
+  float b1, b2, omb1, omb2, eps, decay, step_size, inv_sqrt_c2;
+  double b1d, b2d, lrd, wdd;
+  const float* step_dev;  // NULL: step_size and inv_sqrt_c2 above hold
+  const float* lr_dev;    // NULL: lrd
+  uint64_t seed;
+  uint32_t ordinal;       // place of the launch's first tensor in the caller's list
+  uint32_t per_wg;        // elements per workgroup
+};
+
+template <bool BF16>
+__device__ __forceinline__ void aw_load4(const void* p, int64_t i, int64_t n, bool vec, float (&x)[4]) {
+  if (BF16) {
+    const unsigned short* q = static_cast<const unsigned short*>(p) + i;
+    if (vec && i + 4 <= n) {
+      const ushort4 u = *reinterpret_cast<const ushort4*>(q);
+      x[0] = ceeg_bf16_to_f32(u.x); x[1] = ceeg_bf16_to_f32(u.y); x[2] = ceeg_bf16_to_f32(u.z); x[3] = ceeg_bf16_to_f32(u.w);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = i + k < n ? ceeg_bf16_to_f32(q[k]) : 0.f;
+    }
+  } else {
+    const float* q = static_cast<const float*>(p) + i;
+    if (vec && i + 4 <= n) {
+      const float4 u = *reinterpret_cast<const float4*>(q);
+      x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = i + k < n ? q[k] : 0.f;
+    }
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ void aw_store4(void* p, int64_t i, int64_t n, bool vec, const float (&x)[4]) {
+  if (BF16) {  // a bf16 parameter is rounded to nearest, as every bf16 result of this library
+    unsigned short* q = static_cast<unsigned short*>(p) + i;
+    if (vec && i + 4 <= n) {
+      *reinterpret_cast<ushort4*>(q) = make_ushort4(ceeg_f32_to_bf16(x[0]), ceeg_f32_to_bf16(x[1]), ceeg_f32_to_bf16(x[2]), ceeg_f32_to_bf16(x[3]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + k < n) q[k] = ceeg_f32_to_bf16(x[k]);
+    }
+  } else {
+    float* q = static_cast<float*>(p) + i;
+    if (vec && i + 4 <= n) {
+      *reinterpret_cast<float4*>(q) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + k < n) q[k] = x[k];
+    }
+  }
+}
+__device__ __forceinline__ uint32_t aw_codes4(const uint8_t* p, int64_t i, int64_t n, bool vec) {
+  if (vec && i + 4 <= n) return *reinterpret_cast<const uint32_t*>(p + i);
+  uint32_t w = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (i + k < n) w |= (uint32_t)p[i + k] << (8 * k);
+  return w;
+}
+__device__ __forceinline__ void aw_put_codes4(uint8_t* p, int64_t i, int64_t n, bool vec, uint32_t w) {
+  if (vec && i + 4 <= n) {
+    *reinterpret_cast<uint32_t*>(p + i) = w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k < n) p[i + k] = (uint8_t)(w >> (8 * k));
+  }
+}
+// e4m3 (1 sign, 4 exponent bits with bias 7, 3 mantissa bits, no infinities, 0x7f NaN) -> fp32, exact
+__device__ __forceinline__ float aw_e4m3(uint32_t c) {
+  const uint32_t a = c & 0x7fu;
+  float x = a < 8u ? (float)a * 0x1p-9f : __uint_as_float((a << 20) + (120u << 23));
+  if (a == 0x7fu) x = __uint_as_float(0x7fc00000u);
+  return (c & 0x80u) ? -x : x;
+}
+__device__ __forceinline__ float aw_finite_abs(float x) {
+  const float a = fabsf(x);
+  return a <= 3.402823466e38f ? a : 0.f;  // infinities and NaN do not set a block's scale
+}
+__device__ __forceinline__ float aw_wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+// x / scale as an e4m3 number, rounded by the 16 random bits r so that the expectation of its magnitude (SECOND: of its square) is kept
+template <bool SECOND>
+__device__ __forceinline__ uint32_t aw_round(float x, float scale, uint32_t r) {
+  const uint32_t sign = (__float_as_uint(x) >> 24) & 0x80u;
+  if (!(fabsf(x) <= 3.402823466e38f)) return sign | 0x7fu;  // stays a NaN
+  if (scale == 0.f) return sign;
+  const float y = fminf(fabsf(x) / scale, AW_TOP);
+  const uint32_t u = __float_as_uint(y);
+  const bool small = y < 0x1p-6f;  // there the numbers are 2^-9 apart
+  uint32_t c = small ? (uint32_t)(y * 512.f) : (u >> 20) - (120u << 3);  // the number below
+  const float low = small ? (float)c * 0x1p-9f : __uint_as_float(u & 0xfff00000u);
+  const float step = small ? 0x1p-9f : __uint_as_float((u & 0x7f800000u) - (3u << 23));
+  float share = (y - low) * (small ? 512.f : __uint_as_float((257u << 23) - (u & 0x7f800000u)));  // (y - low) / step, exact
+  if (SECOND) share = share * (y + low) / (low + low + step);
+  if (share * 65536.f + (float)r >= 65536.f) ++c;
+  if (SECOND && c == 0u && y > 0.f) c = 1u;
+  return sign | c;
+}
+
+template <bool BF16, int BITS>
+__global__ __launch_bounds__(AW_THREADS) void adamw_kernel(AwList L, AwHyper h) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int lo = 0, hi = L.count - 1;  // the tensor whose workgroups hold this one
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (L.first[mid] <= blockIdx.x) lo = mid; else hi = mid - 1;
+  }
+  const int64_t n = L.n[lo];
+  const int64_t begin = (int64_t)(blockIdx.x - L.first[lo]) * h.per_wg;
+  const int64_t end = begin + h.per_wg < n ? begin + h.per_wg : n;
+  float step_size = h.step_size, inv_sqrt_c2 = h.inv_sqrt_c2, decay = h.decay;
+  uint64_t seed = h.seed;
+  if (h.step_dev || h.lr_dev) {
+    const double lr = h.lr_dev ? (double)h.lr_dev[0] : h.lrd;
+    decay = (float)(1.0 - lr * h.wdd);
+    if (h.step_dev) {
+      const double t = (double)h.step_dev[0];
+      step_size = (float)(lr / (1.0 - pow(h.b1d, t)));
+      inv_sqrt_c2 = (float)(1.0 / sqrt(1.0 - pow(h.b2d, t)));
+      seed += (uint64_t)(int64_t)t * 0x9E3779B97F4A7C15ull;  // a replayed launch draws other numbers every step
+    } else {
+      step_size = (float)(lr * h.b1d);  // the host put 1 / (1 - b1^t) there
+    }
+  }
+  void* const p = L.p[lo];
+  const void* const g = L.g[lo];
+  void* const m = L.m[lo];
+  void* const v = L.v[lo];
+  const uintptr_t pg = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g);
+  const uintptr_t mv = reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v);
+  const bool vec = (pg & (BF16 ? 7 : 15)) == 0, svec = (mv & (BITS == 8 ? 3 : 15)) == 0;
+
+  for (int64_t b0 = begin + (int64_t)wave * AW_BLOCK; b0 < end; b0 += AW_THREADS / 64 * AW_BLOCK) {
+    const int64_t i = b0 + 4 * lane;
+    float pv[4], gv[4], mo[4], vo[4];
+    aw_load4<BF16>(p, i, n, vec, pv);
+    aw_load4<BF16>(g, i, n, vec, gv);
+    if (BITS == 8) {
+      const float sm = L.ms[lo][b0 / AW_BLOCK], sv = L.vs[lo][b0 / AW_BLOCK];
+      const uint32_t cm = aw_codes4(static_cast<const uint8_t*>(m), i, n, svec), cv = aw_codes4(static_cast<const uint8_t*>(v), i, n, svec);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        mo[k] = aw_e4m3(cm >> (8 * k) & 0xffu) * sm;
+        const float u = aw_e4m3(cv >> (8 * k) & 0xffu) * sv;
+        vo[k] = u * u;
+      }
+    } else {
+      aw_load4<false>(m, i, n, svec, mo);
+      aw_load4<false>(v, i, n, svec, vo);
+    }
+    float root[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      mo[k] = h.b1 * mo[k] + h.omb1 * gv[k];
+      vo[k] = h.b2 * vo[k] + h.omb2 * (gv[k] * gv[k]);
+      root[k] = sqrtf(vo[k]);
+      pv[k] = pv[k] * decay - step_size * (mo[k] / (root[k] * inv_sqrt_c2 + h.eps));
+    }
+    aw_store4<BF16>(p, i, n, vec, pv);
+    if (BITS == 8) {
+      float tm = 0.f, tv = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (i + k >= n) mo[k] = root[k] = 0.f;
+        tm = fmaxf(tm, aw_finite_abs(mo[k]));
+        tv = fmaxf(tv, aw_finite_abs(root[k]));
+      }
+      tm = aw_wave_max(tm);
+      tv = aw_wave_max(tv);
+      const float sm = tm < AW_TINY ? 0.f : tm * AW_PER_TOP, sv = tv < AW_TINY ? 0.f : tv * AW_PER_TOP;
+      const uint64_t quad = (uint64_t)i >> 2;
+      const uint4 r = ceeg_philox(seed, (uint32_t)quad, (uint32_t)(quad >> 32), CEEG_TAG_ADAMW, h.ordinal + lo);
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+      uint32_t cm = 0, cv = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        cm |= aw_round<false>(mo[k], sm, w[k] & 0xffffu) << (8 * k);
+        cv |= aw_round<true>(root[k], sv, w[k] >> 16) << (8 * k);
+      }
+      aw_put_codes4(static_cast<uint8_t*>(m), i, n, svec, cm);
+      aw_put_codes4(static_cast<uint8_t*>(v), i, n, svec, cv);
+      if (lane == 0) {
+        L.ms[lo][b0 / AW_BLOCK] = sm;
+        L.vs[lo][b0 / AW_BLOCK] = sv;
+      }
+    } else {
+      aw_store4<false>(m, i, n, svec, mo);
+      aw_store4<false>(v, i, n, svec, vo);
+    }
+  }
+}
+}  // namespace
+
+extern "C" int ceeg_adamw_block(void) { return AW_BLOCK; }
+
+extern "C" int ceeg_adamw_step(int tensors, const int64_t* numel, void* const* p, const void* const* g, void* const* m, void* const* v,
+                               float* const* m_scale, float* const* v_scale, int dtype, int state_bits, double lr, double beta1, double beta2,
+                               double eps, double weight_decay, int64_t step, const float* lr_dev, const float* step_dev, uint64_t seed,
+                               void* stream) {
+  if (tensors < 0 || (tensors > 0 && (!numel || !p || !g || !m || !v))) return CEEG_EINVAL;
+  if (dtype != CEEG_F32 && dtype != CEEG_BF16) return CEEG_EUNSUPPORTED;
+  if (state_bits != 8 && state_bits != 32) return CEEG_EUNSUPPORTED;
+  if (state_bits == 8 && tensors > 0 && (!m_scale || !v_scale)) return CEEG_EINVAL;
+  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0) || (!step_dev && step < 1)) return CEEG_EINVAL;
+  const uintptr_t palign = dtype == CEEG_F32 ? 3 : 1;
+  int64_t total = 0;
+  for (int t = 0; t < tensors; ++t) {
+    if (numel[t] < 0 || numel[t] > ((int64_t)1 << 40)) return CEEG_EINVAL;
+    if (numel[t] == 0) continue;
+    if (!p[t] || !g[t] || !m[t] || !v[t] || ((reinterpret_cast<uintptr_t>(p[t]) | reinterpret_cast<uintptr_t>(g[t])) & palign)) return CEEG_EINVAL;
+    if (state_bits == 8 ? (!m_scale[t] || !v_scale[t] || !ceeg_aligned(m_scale[t], 4) || !ceeg_aligned(v_scale[t], 4))
+                        : (!ceeg_aligned(m[t], 4) || !ceeg_aligned(v[t], 4))) return CEEG_EINVAL;
+    total += numel[t];
+  }
+  AwHyper h;
+  const double c1 = step_dev ? 1.0 : 1.0 - pow(beta1, (double)step), c2 = step_dev ? 1.0 : 1.0 - pow(beta2, (double)step);
+  h.b1 = (float)beta1; h.b2 = (float)beta2; h.omb1 = (float)(1.0 - beta1); h.omb2 = (float)(1.0 - beta2);
+  h.eps = (float)eps; h.decay = (float)(1.0 - lr * weight_decay); h.step_size = (float)(lr / c1); h.inv_sqrt_c2 = (float)(1.0 / sqrt(c2));
+  h.b1d = step_dev ? beta1 : 1.0 / c1; h.b2d = beta2; h.lrd = lr; h.wdd = weight_decay;
+  h.step_dev = step_dev; h.lr_dev = lr_dev;
+  h.seed = seed;
+  // 4096 elements per workgroup amortise its start where there are enough of them to fill 256 compute units several times over; below
+  // that one block per wave spreads a small list over as many of them as there are
+  h.per_wg = total >= (int64_t)4096 * 2048 ? 4096 : 1024;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  for (int t = 0; t < tensors;) {
+    AwList L;
+    int c = 0;
+    uint64_t wgs = 0;
+    h.ordinal = (uint32_t)t;
+    // a launch takes consecutive tensors (empty ones keep their place) while their workgroups fit a grid
+    for (; t < tensors && c < AW_LIST; ++t, ++c) {
+      const uint64_t more = (uint64_t)((numel[t] + h.per_wg - 1) / h.per_wg);
+      if (more > 0x7fffffffull) return CEEG_EUNSUPPORTED;
+      if (wgs + more > 0x7fffffffull) break;
+      L.p[c] = p[t]; L.g[c] = g[t]; L.m[c] = m[t]; L.v[c] = v[t]; L.n[c] = numel[t]; L.first[c] = (uint32_t)wgs;
+      L.ms[c] = state_bits == 8 ? m_scale[t] : nullptr;
+      L.vs[c] = state_bits == 8 ? v_scale[t] : nullptr;
+      wgs += more;
+    }
+    L.count = c;
+    for (int k = c; k < AW_LIST; ++k) { L.p[k] = L.m[k] = L.v[k] = nullptr; L.g[k] = nullptr; L.ms[k] = L.vs[k] = nullptr; L.n[k] = 0; L.first[k] = 0; }
+    if (wgs == 0) continue;
+    const dim3 grid((unsigned)wgs), block(AW_THREADS);
+    if (dtype == CEEG_F32) {
+      if (state_bits == 32) adamw_kernel<false, 32><<<grid, block, 0, st>>>(L, h);
+      else adamw_kernel<false, 8><<<grid, block, 0, st>>>(L, h);
+    } else {
+      if (state_bits == 32) adamw_kernel<true, 32><<<grid, block, 0, st>>>(L, h);
+      else adamw_kernel<true, 8><<<grid, block, 0, st>>>(L, h);
+    }
+    CEEG_CHECK_LAUNCH();
+  }
+  return CEEG_OK;
+}

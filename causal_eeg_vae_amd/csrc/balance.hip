@@ -1,0 +1,365 @@
+// Balance loss of an assignment of rows to codes (or experts), the per-code counts, and its gradient:
+//   p = softmax(scores);  n = rows that count;  counts_e = #{(t, j): row t counts, idx[t, j] = e};  f = counts / (n K);  P = sum_t p_t / n
+//   loss = E sum_e f_e P_e;     d loss / d scores[t, e] = E / n * p_te (f_e - sum_e' f_e' p_te')          (the counts carry no gradient)
+// Bound: HBM bytes - the scores are read once forward, once backward, the gradient written once.  A row lives in the registers of one lane group (1 to 64
+// lanes, 16-byte loads where the rows allow them), its softmax is two butterflies; the column sums of p stay in registers over all rows
+// of a wave, because a lane keeps its columns, and are joined over waves and workgroups in a fixed order: no float atomics.  The counts are
+// integer LDS atomics, whose order does not matter.
+#include "ceeg_internal.h"
+
+namespace {
+constexpr int BL_THREADS = 256;
+constexpr int BL_WAVES = BL_THREADS / 64;
+constexpr int BL_MAX_E = 4096;
+constexpr int BL_MAX_WG = 1024;
+
+struct BlRow {  // where the scores of a row and the columns of a lane are
+  const void* s;
+  int64_t ld, T;
+  int E, lanes;  // lanes: lane-group size of one row, a power of two
+  const uint8_t* mask;
+};
+
+// NV pieces of VEC consecutive columns per lane; piece j of lane l (of `lanes`) starts at column (j * lanes + l) * VEC
+template <bool BF16, int VEC, int NV>
+__device__ __forceinline__ void bl_load(const BlRow& a, int64_t t, int l, float (&x)[NV * VEC]) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * a.lanes + l) * VEC;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) x[j * VEC + k] = -INFINITY;
+    if (c >= a.E) continue;  // VEC > 1 only where E is a multiple of it
+    if (BF16) {
+      const unsigned short* q = static_cast<const unsigned short*>(a.s) + t * a.ld + c;
+      if (VEC == 8) {
+        const uint4 u = *reinterpret_cast<const uint4*>(q);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[j * VEC + (2 * k) % VEC] = __uint_as_float(w[k] << 16);
+          x[j * VEC + (2 * k + 1) % VEC] = __uint_as_float(w[k] & 0xffff0000u);
+        }
+      } else {
+        x[j * VEC] = ceeg_bf16_to_f32(q[0]);
+      }
+    } else {
+      const float* q = static_cast<const float*>(a.s) + t * a.ld + c;
+      if (VEC == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(q);
+        x[j * VEC] = u.x; x[j * VEC + 1 % VEC] = u.y; x[j * VEC + 2 % VEC] = u.z; x[j * VEC + 3 % VEC] = u.w;
+      } else {
+        x[j * VEC] = q[0];
+      }
+    }
+  }
+}
+
+// x -> softmax over the lane group; a row of nothing but -inf has no probability anywhere
+template <int N>
+__device__ __forceinline__ void bl_softmax(int lanes, float (&x)[N]) {
+  float top = x[0];
+#pragma unroll
+  for (int k = 1; k < N; ++k) top = fmaxf(top, x[k]);
+  for (int o = lanes >> 1; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    x[k] = __expf(x[k] - base);
+    sum += x[k];
+  }
+  for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int k = 0; k < N; ++k) x[k] *= inv;
+}
+
+// per workgroup: part_p[wg][E] (column sums of p), part_c[wg][E] (counts), part_n[wg] = {rows that count, a code out of range was seen}
+template <bool BF16, int VEC, int NV>
+__global__ __launch_bounds__(BL_THREADS) void balance_rows_kernel(BlRow a, const void* __restrict__ idx, int idx64, int K, float* __restrict__ part_p,
+                                                                  int32_t* __restrict__ part_c, int2* __restrict__ part_n) {
+  extern __shared__ int s_mem[];
+  int* s_c = s_mem;                                    // [E]
+  float* s_p = reinterpret_cast<float*>(s_mem + a.E);  // [E]
+  __shared__ int s_n[2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int e = threadIdx.x; e < a.E; e += BL_THREADS) s_c[e] = 0;
+  if (threadIdx.x < 2) s_n[threadIdx.x] = 0;
+  __syncthreads();
+  const int per = 64 / a.lanes, l = lane & (a.lanes - 1), sub = lane / a.lanes;
+  float acc[NV * VEC];
+#pragma unroll
+  for (int k = 0; k < NV * VEC; ++k) acc[k] = 0.f;
+  int rows = 0, bad = 0;
+  const int64_t stride = (int64_t)gridDim.x * BL_WAVES * per;
+  for (int64_t t0 = ((int64_t)blockIdx.x * BL_WAVES + wave) * per; t0 < a.T; t0 += stride) {  // the same number of turns for a wave's lanes
+    const int64_t t = t0 + sub;
+    const bool on = t < a.T && (!a.mask || a.mask[t]);
+    float x[NV * VEC];
+    if (on) {
+      bl_load<BF16, VEC, NV>(a, t, l, x);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV * VEC; ++k) x[k] = -INFINITY;
+    }
+    bl_softmax(a.lanes, x);
+#pragma unroll
+    for (int k = 0; k < NV * VEC; ++k) acc[k] += x[k];
+    if (on) {
+      for (int j = l; j < K; j += a.lanes) {
+        const int64_t e = idx64 ? static_cast<const int64_t*>(idx)[t * K + j] : (int64_t)static_cast<const int32_t*>(idx)[t * K + j];
+        if (e >= 0 && e < a.E) atomicAdd(&s_c[e], 1);
+        else if (e != -1) bad = 1;
+      }
+      rows += l == 0;
+    }
+  }
+  // the lane groups of a wave hold the same columns
+  for (int o = a.lanes; o < 64; o <<= 1) {
+#pragma unroll
+    for (int k = 0; k < NV * VEC; ++k) acc[k] += __shfl_xor(acc[k], o, 64);
+  }
+  for (int w = 0; w < BL_WAVES; ++w) {  // the waves add their sums in turn
+    if (wave == w && sub == 0) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const int c = (j * a.lanes + l) * VEC + k;
+          if (c < a.E) s_p[c] = w == 0 ? acc[j * VEC + k] : s_p[c] + acc[j * VEC + k];
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (rows) atomicAdd(&s_n[0], rows);
+  if (bad) atomicOr(&s_n[1], 1);
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.E; e += BL_THREADS) {
+    part_p[(int64_t)blockIdx.x * a.E + e] = s_p[e];
+    part_c[(int64_t)blockIdx.x * a.E + e] = s_c[e];
+  }
+  if (threadIdx.x == 0) part_n[blockIdx.x] = make_int2(s_n[0], s_n[1]);
+}
+
+// 64 columns per workgroup: P and counts over all workgroups of the row pass; f = counts / (n K); stats = [f (E), n]; dots[wg] = sum f P
+__global__ __launch_bounds__(1024) void balance_join_kernel(const float* __restrict__ part_p, const int32_t* __restrict__ part_c,
+                                                            const int2* __restrict__ part_n, int wgs, int E, int K, int64_t* __restrict__ counts,
+                                                            float* __restrict__ stats, double* __restrict__ dots) {
+  __shared__ double s_p[16][64];
+  __shared__ long long s_c[16][64];
+  __shared__ long long s_n[16];
+  __shared__ int s_bad;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int e = blockIdx.x * 64 + lane;
+  if (threadIdx.x == 0) s_bad = 0;
+  double p = 0.0;
+  long long c = 0, n = 0;
+  int bad = 0;
+  if (e < E) {
+    for (int b = w; b < wgs; b += 16) {
+      p += (double)part_p[(int64_t)b * E + e];
+      c += part_c[(int64_t)b * E + e];
+    }
+  }
+  for (int b = threadIdx.x; b < wgs; b += 1024) {
+    n += part_n[b].x;
+    bad |= part_n[b].y;
+  }
+  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+  s_p[w][lane] = p;
+  s_c[w][lane] = c;
+  if (lane == 0) s_n[w] = n;
+  __syncthreads();
+  if (bad) s_bad = 1;  // every writer writes the same
+  __syncthreads();
+  if (w == 0) {
+    p = 0.0; c = 0; n = 0;
+    for (int k = 0; k < 16; ++k) { p += s_p[k][lane]; c += s_c[k][lane]; n += s_n[k]; }
+    // no row that counts: loss and gradient are zero.  A code outside [-1, E) cannot raise an error from here: it makes the loss and the gradient NaN.
+    const double rows = n > 0 ? (double)n : 1.0;
+    double f = (double)c / (rows * K);
+    if (s_bad) f = __longlong_as_double(0x7ff8000000000000LL);
+    double d = 0.0;
+    if (e < E) {
+      counts[e] = c;
+      stats[e] = (float)f;
+      d = f * (p / rows);
+    }
+    if (blockIdx.x == 0 && lane == 0) stats[E] = (float)rows;
+    d = ceeg_wave_sum_d(d);
+    if (lane == 0) dots[blockIdx.x] = d;
+  }
+}
+
+__global__ void balance_loss_kernel(const double* __restrict__ dots, int n, int E, float* __restrict__ loss) {
+  const double d = ceeg_wave_sum_d((int)threadIdx.x < n ? dots[threadIdx.x] : 0.0);  // E <= 4096: at most 64 parts
+  if (threadIdx.x == 0) loss[0] = (float)(d * E);
+}
+
+template <bool BF16, int VEC, int NV>
+__global__ __launch_bounds__(BL_THREADS) void balance_grad_kernel(BlRow a, const float* __restrict__ stats, const float* __restrict__ g, void* __restrict__ ds) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int per = 64 / a.lanes, l = lane & (a.lanes - 1), sub = lane / a.lanes;
+  float f[NV * VEC];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const int c = (j * a.lanes + l) * VEC + k;
+      f[j * VEC + k] = c < a.E ? stats[c] : 0.f;
+    }
+  }
+  const float scale = (float)((double)g[0] * a.E / (double)stats[a.E]);
+  const int64_t stride = (int64_t)gridDim.x * BL_WAVES * per;
+  for (int64_t t0 = ((int64_t)blockIdx.x * BL_WAVES + wave) * per; t0 < a.T; t0 += stride) {
+    const int64_t t = t0 + sub;
+    if (t >= a.T) continue;  // whole lane groups leave together; the butterflies stay inside a group
+    const bool on = !a.mask || a.mask[t];
+    float x[NV * VEC];
+    if (on) {
+      bl_load<BF16, VEC, NV>(a, t, l, x);
+      bl_softmax(a.lanes, x);
+      float d = 0.f;
+#pragma unroll
+      for (int k = 0; k < NV * VEC; ++k) d = __fmaf_rn(f[k], x[k], d);
+      for (int o = a.lanes >> 1; o > 0; o >>= 1) d += __shfl_xor(d, o, 64);
+#pragma unroll
+      for (int k = 0; k < NV * VEC; ++k) x[k] = scale * x[k] * (f[k] - d);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV * VEC; ++k) x[k] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * a.lanes + l) * VEC;
+      if (c >= a.E) continue;
+      if (BF16) {
+        unsigned short* q = static_cast<unsigned short*>(ds) + t * a.E + c;
+        if (VEC == 8) {
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[k] = (uint32_t)ceeg_f32_to_bf16(x[j * VEC + (2 * k) % VEC]) | ((uint32_t)ceeg_f32_to_bf16(x[j * VEC + (2 * k + 1) % VEC]) << 16);
+          *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+          q[0] = ceeg_f32_to_bf16(x[j * VEC]);
+        }
+      } else {
+        float* q = static_cast<float*>(ds) + t * a.E + c;
+        if (VEC == 4) *reinterpret_cast<float4*>(q) = make_float4(x[j * VEC], x[j * VEC + 1 % VEC], x[j * VEC + 2 % VEC], x[j * VEC + 3 % VEC]);
+        else q[0] = x[j * VEC];
+      }
+    }
+  }
+}
+
+// lanes of a row and pieces per lane: the fewest lanes that hold a row in one piece each, 64 with as many pieces as it takes beyond that
+void bl_shape(int E, int vec, int* lanes, int* nv) {
+  const int pieces = (E + vec - 1) / vec;
+  int l = 1;
+  while (l < 64 && l < pieces) l <<= 1;
+  *lanes = l;
+  *nv = (pieces + l - 1) / l;
+}
+bool bl_vec(const void* s, int64_t ld, int E, int dtype) {
+  const int per = dtype == CEEG_BF16 ? 8 : 4;
+  return E % per == 0 && ld % per == 0 && ceeg_aligned(s, 16);
+}
+int bl_wgs(int64_t T, int E, int lanes) {
+  // as many workgroups as there are rows for, 1024 at most (four per compute unit), fewer where their partial sums would weigh more than the rows
+  int64_t wgs = (T + BL_WAVES * (64 / lanes) - 1) / (BL_WAVES * (64 / lanes));
+  const int64_t cap = E > 1024 ? BL_MAX_WG / 4 : BL_MAX_WG;
+  return (int)(wgs < cap ? wgs : cap);
+}
+int bl_check(const void* s, int64_t ld, int64_t T, int E, int dtype) {
+  if (T < 1 || T > ((int64_t)1 << 31) - 1 || E < 1 || ld < E || !s) return CEEG_EINVAL;
+  if (dtype != CEEG_F32 && dtype != CEEG_BF16) return CEEG_EUNSUPPORTED;
+  if (E > BL_MAX_E) return CEEG_EUNSUPPORTED;
+  if (!ceeg_aligned(s, dtype == CEEG_F32 ? 4 : 2)) return CEEG_EINVAL;
+  return CEEG_OK;
+}
+}  // namespace
+
+#define BL_DISPATCH(KERNEL, ...)                                                          \
+  do {                                                                                    \
+    if (dtype == CEEG_F32) {                                                              \
+      if (vec == 4) {                                                                     \
+        if (nv <= 1) KERNEL<false, 4, 1> __VA_ARGS__;                                     \
+        else if (nv <= 2) KERNEL<false, 4, 2> __VA_ARGS__;                                \
+        else if (nv <= 4) KERNEL<false, 4, 4> __VA_ARGS__;                                \
+        else KERNEL<false, 4, 16> __VA_ARGS__;                                            \
+      } else {                                                                            \
+        if (nv <= 1) KERNEL<false, 1, 1> __VA_ARGS__;                                     \
+        else if (nv <= 4) KERNEL<false, 1, 4> __VA_ARGS__;                                \
+        else if (nv <= 16) KERNEL<false, 1, 16> __VA_ARGS__;                              \
+        else KERNEL<false, 1, 64> __VA_ARGS__;                                            \
+      }                                                                                   \
+    } else {                                                                              \
+      if (vec == 8) {                                                                     \
+        if (nv <= 1) KERNEL<true, 8, 1> __VA_ARGS__;                                      \
+        else if (nv <= 2) KERNEL<true, 8, 2> __VA_ARGS__;                                 \
+        else KERNEL<true, 8, 8> __VA_ARGS__;                                              \
+      } else {                                                                            \
+        if (nv <= 1) KERNEL<true, 1, 1> __VA_ARGS__;                                      \
+        else if (nv <= 4) KERNEL<true, 1, 4> __VA_ARGS__;                                 \
+        else if (nv <= 16) KERNEL<true, 1, 16> __VA_ARGS__;                               \
+        else KERNEL<true, 1, 64> __VA_ARGS__;                                             \
+      }                                                                                   \
+    }                                                                                     \
+  } while (0)
+
+extern "C" size_t ceeg_balance_ws_bytes(int64_t T, int E) {
+  if (T < 1 || E < 1 || E > BL_MAX_E) return 0;
+  int lanes, nv;
+  bl_shape(E, 1, &lanes, &nv);  // one column a piece has the most lanes per row, hence the most workgroups
+  const size_t wgs = (size_t)bl_wgs(T, E, lanes);
+  return ceeg_ws_part(wgs * E, 4) + ceeg_ws_part(wgs * E, 4) + ceeg_ws_part(wgs, 8) + ceeg_ws_part(64, 8);
+}
+
+extern "C" int ceeg_balance_fwd(const void* scores, int64_t ld, int dtype, const void* idx, int idx_bytes, int64_t T, int E, int K, const uint8_t* mask,
+                                float* loss, int64_t* counts, float* stats, void* ws, size_t ws_bytes, void* stream) {
+  const int rc = bl_check(scores, ld, T, E, dtype);
+  if (rc) return rc;
+  if (K < 1 || K > E || !idx || !loss || !counts || !stats || (idx_bytes != 4 && idx_bytes != 8) || !ceeg_aligned(idx, idx_bytes)) return CEEG_EINVAL;
+  if (T > ((int64_t)1 << 38) / K) return CEEG_EUNSUPPORTED;  // a workgroup's counts are 32 bits
+  if (!ws || ws_bytes < ceeg_balance_ws_bytes(T, E) || !ceeg_aligned(ws, 256)) return CEEG_EWORKSPACE;
+  const int vec = bl_vec(scores, ld, E, dtype) ? (dtype == CEEG_BF16 ? 8 : 4) : 1;
+  BlRow a{scores, ld, T, E, 0, mask};
+  int nv;
+  bl_shape(E, vec, &a.lanes, &nv);
+  const int wgs = bl_wgs(T, E, a.lanes);
+  CeegWs w(ws, ws_bytes);
+  float* part_p = w.take<float>((size_t)wgs * E);
+  int32_t* part_c = w.take<int32_t>((size_t)wgs * E);
+  int2* part_n = w.take<int2>(wgs);
+  double* dots = w.take<double>(64);
+  if (!w.ok) return CEEG_EWORKSPACE;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const size_t lds = (size_t)E * 8;  // 32 KB at most
+  BL_DISPATCH(balance_rows_kernel, <<<wgs, BL_THREADS, lds, st>>>(a, idx, idx_bytes == 8, K, part_p, part_c, part_n));
+  CEEG_CHECK_LAUNCH();
+  const int joins = (E + 63) / 64;
+  balance_join_kernel<<<joins, 1024, 0, st>>>(part_p, part_c, part_n, wgs, E, K, counts, stats, dots);
+  CEEG_CHECK_LAUNCH();
+  balance_loss_kernel<<<1, 64, 0, st>>>(dots, joins, E, loss);
+  CEEG_CHECK_LAUNCH();
+  return CEEG_OK;
+}
+
+extern "C" int ceeg_balance_bwd(const void* scores, int64_t ld, int dtype, int64_t T, int E, const uint8_t* mask, const float* stats, const float* g,
+                                void* dscores, void* stream) {
+  const int rc = bl_check(scores, ld, T, E, dtype);
+  if (rc) return rc;
+  if (!stats || !g || !dscores || !ceeg_aligned(dscores, 16)) return CEEG_EINVAL;
+  const int vec = bl_vec(scores, ld, E, dtype) ? (dtype == CEEG_BF16 ? 8 : 4) : 1;
+  BlRow a{scores, ld, T, E, 0, mask};
+  int nv;
+  bl_shape(E, vec, &a.lanes, &nv);
+  const int64_t units = (T + BL_WAVES * (64 / a.lanes) - 1) / (BL_WAVES * (64 / a.lanes));
+  const unsigned wgs = (unsigned)(units < 2048 ? units : 2048);  // eight per compute unit: every lane reads its f once for many rows
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  BL_DISPATCH(balance_grad_kernel, <<<wgs, BL_THREADS, 0, st>>>(a, stats, g, dscores));
+  CEEG_CHECK_LAUNCH();
+  return CEEG_OK;
+}

@@ -54,6 +54,7 @@ __device__ __forceinline__ double ceeg_wave_sum_d(double v) {
 // Philox4x32-10, restated bit for bit in oracle/ceeg_oracle.c
 #define CEEG_TAG_EPS 0x45505300u
 #define CEEG_TAG_NEG 0x4E454700u
+#define CEEG_TAG_ADAMW 0x41444D57u
 __device__ __forceinline__ uint4 ceeg_philox(uint64_t seed, uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3) {
   uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
 #pragma unroll

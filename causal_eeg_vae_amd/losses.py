@@ -1,0 +1,163 @@
+"""Losses at the end of a training step: the token cross entropy behind a vocabulary product (the reference's `recon_loss`,
+scripts/gpt2.py:1080-1084 and scripts/models.py:34, over the hidden states of the caller's language decoder) and the balance loss over an
+assignment to codes or experts.  The kernels are ceeg_linear_ce_fwd / _bwd and ceeg_balance_fwd / _bwd (include/ceeg.h)."""
+import torch
+
+from . import _lib
+
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _dtype(t, what):
+    if t.dtype == torch.float32:
+        return _lib.CEEG_F32
+    if t.dtype == torch.bfloat16:
+        return _lib.CEEG_BF16
+    raise TypeError(f"{what} must be float32 or bfloat16, got {t.dtype}")
+
+
+def _same_device(*tensors):
+    _lib.require_cuda(*tensors)
+    if len({t.device for t in tensors if t is not None}) > 1:
+        raise ValueError(f"all tensors must be on one device, got {[str(t.device) for t in tensors if t is not None]}")
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, target, ignore_index, reduction):
+        L = _lib.lib()
+        dtype = _dtype(hidden, "hidden")
+        (T, H), V = hidden.shape, weight.shape[0]
+        dev = hidden.device
+        if hidden.stride(1) != 1 or (T > 1 and hidden.stride(0) < H):
+            hidden = hidden.contiguous()
+        if weight.stride(1) != 1 or (V > 1 and weight.stride(0) < H) or (dtype == _lib.CEEG_BF16 and (weight.data_ptr() % 16 or weight.stride(0) % 8)):
+            weight = weight.clone(memory_format=torch.contiguous_format)
+        target = target.contiguous()
+        ldh, ldw = max(hidden.stride(0), H), max(weight.stride(0), H)
+        with torch.cuda.device(dev):
+            loss = torch.empty(T if reduction == 0 else 1, dtype=torch.float32, device=dev)
+            lse = torch.empty(T, dtype=torch.float32, device=dev)
+            tokens = torch.empty(3 * T + 1, dtype=torch.int32, device=dev)
+            ws = _lib.workspace(L.ceeg_linear_ce_fwd_ws_bytes(T, H, V, dtype), dev)
+            with _lib.timed("linear_ce_fwd"):
+                _lib.check(L.ceeg_linear_ce_fwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, target.data_ptr(), T, H, V, dtype, ignore_index, reduction,
+                                                loss.data_ptr(), lse.data_ptr(), tokens.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream()),
+                           "ceeg_linear_ce_fwd")
+        ctx.save_for_backward(hidden, weight, lse, tokens)
+        ctx.sizes = T, H, V, ldh, ldw, dtype, reduction
+        return loss if reduction == 0 else loss[0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        hidden, weight, lse, tokens = ctx.saved_tensors
+        T, H, V, ldh, ldw, dtype, reduction = ctx.sizes
+        L = _lib.lib()
+        dev = hidden.device
+        need_h, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        with torch.cuda.device(dev):
+            g = g.to(torch.float32).contiguous()
+            dh = torch.empty(T, H, dtype=hidden.dtype, device=dev) if need_h else None
+            dw = torch.empty(V, H, dtype=weight.dtype, device=dev) if need_w else None
+            ws = _lib.workspace(L.ceeg_linear_ce_bwd_ws_bytes(T, H, V, dtype), dev)
+            with _lib.timed("linear_ce_bwd"):
+                _lib.check(L.ceeg_linear_ce_bwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, T, H, V, dtype, reduction, g.data_ptr(), lse.data_ptr(),
+                                                tokens.data_ptr(), _lib.ptr(dh), _lib.ptr(dw), ws.data_ptr(), ws.numel(), _lib.stream()),
+                           "ceeg_linear_ce_bwd")
+        return dh, dw, None, None, None
+
+
+def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="mean"):
+    """Cross entropy of `hidden @ weight.T` against `target` without the logits in memory, forward and backward.
+
+    hidden [..., H], weight [V, H] (both float32 or both bfloat16), target [...] int64 of hidden's leading shape.  Tokens whose target is
+    `ignore_index` (padding) take no part, whatever their hidden row holds.  reduction: "mean" over the tokens that count (0 where none does),
+    "sum", or "none" (target's shape, 0 where ignored).  The loss is float32; the gradients have their inputs' types, all sums are float32.
+    A target outside [0, V) makes the loss and the gradients it reaches NaN: an error would need a host read of the targets."""
+    if not all(isinstance(t, torch.Tensor) for t in (hidden, weight, target)):
+        raise TypeError("hidden, weight and target must be tensors")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or target.shape != hidden.shape[:-1]:
+        raise ValueError(f"hidden [..., H], weight [V, H] and target [...] expected; got {tuple(hidden.shape)}, {tuple(weight.shape)} and {tuple(target.shape)}")
+    if target.dtype != torch.int64:
+        raise TypeError(f"target must be int64, got {target.dtype}")
+    _dtype(hidden, "hidden")
+    if hidden.dtype != weight.dtype:
+        raise TypeError(f"hidden and weight must have one type, got {hidden.dtype} and {weight.dtype}")
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"weight must have a class and a column at least, got {tuple(weight.shape)}")
+    _same_device(hidden, weight, target)
+    if target.numel() == 0:  # no token: nothing to launch, the gradients are zero
+        none = (hidden.float().sum() + weight.float().sum()) * 0.0
+        return none if reduction != "none" else hidden.float().sum(-1) * 0.0
+    loss = _LinearCrossEntropy.apply(hidden.reshape(-1, hidden.shape[-1]), weight, target.reshape(-1), int(ignore_index), _REDUCTIONS[reduction])
+    return loss.view(target.shape) if reduction == "none" else loss
+
+
+class _Balance(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, scores, indices, mask):
+        L = _lib.lib()
+        dtype = _dtype(scores, "scores")
+        (T, E), K = scores.shape, indices.shape[1]
+        dev = scores.device
+        if scores.stride(1) != 1 or (T > 1 and scores.stride(0) < E):
+            scores = scores.contiguous()
+        indices = indices.contiguous()
+        mask = None if mask is None else mask.contiguous()
+        ld = max(scores.stride(0), E)
+        with torch.cuda.device(dev):
+            loss = torch.empty(1, dtype=torch.float32, device=dev)
+            counts = torch.empty(E, dtype=torch.int64, device=dev)
+            stats = torch.empty(E + 1, dtype=torch.float32, device=dev)
+            ws = _lib.workspace(L.ceeg_balance_ws_bytes(T, E), dev)
+            with _lib.timed("balance_fwd"):
+                _lib.check(L.ceeg_balance_fwd(scores.data_ptr(), ld, dtype, indices.data_ptr(), indices.element_size(), T, E, K, _lib.ptr(mask),
+                                              loss.data_ptr(), counts.data_ptr(), stats.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream()),
+                           "ceeg_balance_fwd")
+        ctx.save_for_backward(scores, mask, stats)
+        ctx.sizes = T, E, ld, dtype
+        ctx.mark_non_differentiable(counts)
+        return loss[0], counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _g_counts):
+        scores, mask, stats = ctx.saved_tensors
+        T, E, ld, dtype = ctx.sizes
+        dev = scores.device
+        with torch.cuda.device(dev):
+            g = g.to(torch.float32).contiguous()
+            ds = torch.empty(T, E, dtype=scores.dtype, device=dev)
+            with _lib.timed("balance_bwd"):
+                _lib.check(_lib.lib().ceeg_balance_bwd(scores.data_ptr(), ld, dtype, T, E, _lib.ptr(mask), stats.data_ptr(), g.data_ptr(), ds.data_ptr(),
+                                                       _lib.stream()), "ceeg_balance_bwd")
+        return ds, None, None
+
+
+def balance_loss(scores, indices, mask=None):
+    """(loss, counts): E * sum_e f_e P_e with f the share of the assignments that code (or expert) e got and P its mean softmax probability - 1 where the
+    codes are used evenly, more where few of them get both - and the assignments per code, int64 [E].
+
+    scores [T, E] float32 or bfloat16, indices [T] or [T, K] int32 / int64 (-1: no assignment), mask [T] bool (False: the row does not
+    count).  The gradient flows to the scores through P.  No row that counts: loss 0.  A code outside [-1, E) makes the loss NaN.  E <= 4096."""
+    if not all(isinstance(t, torch.Tensor) for t in (scores, indices)) or not (mask is None or isinstance(mask, torch.Tensor)):
+        raise TypeError("scores, indices and mask must be tensors")
+    if indices.dim() == 1:
+        indices = indices[:, None]
+    if scores.dim() != 2 or indices.dim() != 2 or indices.shape[0] != scores.shape[0]:
+        raise ValueError(f"scores [T, E] and indices [T] or [T, K] expected; got {tuple(scores.shape)} and {tuple(indices.shape)}")
+    T, E = scores.shape
+    if not 1 <= E <= 4096 or not 1 <= indices.shape[1] <= E:
+        raise ValueError(f"1 <= E <= 4096 and 1 <= K <= E expected, got E = {E}, K = {indices.shape[1]}")
+    if indices.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"indices must be int32 or int64, got {indices.dtype}")
+    if mask is not None and (mask.dtype != torch.bool or mask.shape != (T,)):
+        raise ValueError(f"mask must be bool [{T}], got {mask.dtype} {tuple(mask.shape)}")
+    _dtype(scores, "scores")
+    _same_device(scores, indices, mask)
+    if T == 0:  # no row: nothing to launch, the gradient is empty
+        return scores.float().sum() * 0.0, torch.zeros(E, dtype=torch.int64, device=scores.device)
+    return _Balance.apply(scores, indices, mask)

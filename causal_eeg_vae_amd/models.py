@@ -1344,10 +1344,13 @@ class VGAEVQ(nn.Module):
         vq_loss, z_q, perplexity, _, idx = vector_quantization(z)      (scripts/models.py:32)
         rec = recon_loss(z_q) over the graph's edges and 1:1 permutation-structured negatives
         loss = _loss_sum(rec, kl, vq_loss, N)                                   (loss sum as scripts/run.py:95)
+               + balance * (balance loss over the codes)                       (only with balance > 0; no reference counterpart)
     """
 
-    def __init__(self, in_channels, latent, num_latent_embeddings=512, beta=0.25, seed=0, negatives="sigma", compute_dtype=torch.float32):
-        """negatives: "sigma" = permutation-structured negatives (col[p], sigma(r)) drawn inside the fused decoder (no per-step
+    def __init__(self, in_channels, latent, num_latent_embeddings=512, beta=0.25, seed=0, negatives="sigma", compute_dtype=torch.float32,
+                 balance=0.0, balance_temperature=1.0):
+        """balance: weight of the quantiser's balance loss over the codes (VectorQuantizer.balance) in the training loss; 0 leaves it out.
+        negatives: "sigma" = permutation-structured negatives (col[p], sigma(r)) drawn inside the fused decoder (no per-step
         sort; colliding pairs masked) - the fast path; "uniform" = the literal recon_loss path: E pairs from
         negative_sampling (ceeg_neg_sample_uniform, rejection against the edge set) decoded through the edge-list kernel,
         their per-step CSR built by a device sort for the atomics-free backward."""
@@ -1357,6 +1360,13 @@ class VGAEVQ(nn.Module):
         self.encoder = VariationalGCNEncoder(in_channels, latent, compute_dtype)
         self.vector_quantization = VectorQuantizer(num_latent_embeddings, latent, beta, return_one_hot=False)
         self.latent, self.seed, self.negatives = latent, int(seed), negatives
+        self.balance, self.balance_temperature = float(balance), float(balance_temperature)
+
+    def _with_balance(self, loss, aux):
+        if self.balance == 0.0:
+            return loss, aux
+        aux["balance"], aux["code_counts"] = self.vector_quantization.balance(aux["z"], aux["idx"], self.balance_temperature)
+        return loss + self.balance * aux["balance"], aux
 
     def negative_seed(self, step):
         return (self.seed * 0x9E3779B1 + 0x5851F42D * (int(step) + 1)) & (2**63 - 1)
@@ -1375,7 +1385,7 @@ class VGAEVQ(nn.Module):
                 # both pair sets in code form, one dz; with no list given the pairs are drawn inside the forward kernel
                 rec, sums, neg_edge_index = _UniformRecon.apply(z_q, graph, neg_edge_index, W, code, self.negative_seed(step), n_neg)
                 loss = _loss_sum(rec, kl, vq_loss, N)
-                return loss, dict(rec=rec, kl=kl, vq=vq_loss, ppl=ppl, idx=idx, z=z, ml=ml, dec_sums=sums, neg_edge_index=neg_edge_index)
+                return self._with_balance(loss, dict(rec=rec, kl=kl, vq=vq_loss, ppl=ppl, idx=idx, z=z, ml=ml, dec_sums=sums, neg_edge_index=neg_edge_index))
             if neg_edge_index is None:
                 neg_edge_index = negative_sampling_raw(graph, N, graph.num_edges, self.negative_seed(step))
             if (os.environ.get("CEEG_DEC_CODES", "1") == "1" and graph.num_edges > 0
@@ -1398,7 +1408,7 @@ class VGAEVQ(nn.Module):
             rec, sums = _FusedDecoder.apply(z_q, graph, a, b, ainv, True, None, self.vector_quantization.embedding.weight,
                                             idx.view(-1).to(torch.int32))
         loss = _loss_sum(rec, kl, vq_loss, N)
-        return loss, dict(rec=rec, kl=kl, vq=vq_loss, ppl=ppl, idx=idx, z=z, ml=ml, dec_sums=sums, neg_edge_index=neg_edge_index)
+        return self._with_balance(loss, dict(rec=rec, kl=kl, vq=vq_loss, ppl=ppl, idx=idx, z=z, ml=ml, dec_sums=sums, neg_edge_index=neg_edge_index))
 
 
 class ConditionalVGAEVQ(nn.Module):

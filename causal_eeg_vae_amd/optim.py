@@ -1,0 +1,161 @@
+"""AdamW over many tensors in one launch (ceeg_adamw_step, include/ceeg.h), moments in 32 bits or in 8.  The reference trains with Adam
+(scripts/run.py:56); `Trainer(optimizer="adamw")` takes this one."""
+import ctypes as C
+
+import torch
+
+from . import _lib
+
+BLOCK = 256                 # elements that share a scale of an 8-bit state
+_SPREAD = 0x9E3779B97F4A7C15  # between the random streams of two steps
+_DTYPES = {torch.float32: _lib.CEEG_F32, torch.bfloat16: _lib.CEEG_BF16}
+
+
+def block_state(like):
+    """A zero 8-bit moment of a parameter: (codes float8_e4m3fn of its shape, scales float32, one per 256 consecutive elements)."""
+    return (torch.zeros(like.shape, dtype=torch.float8_e4m3fn, device=like.device),
+            torch.zeros(-(-like.numel() // BLOCK), dtype=torch.float32, device=like.device))
+
+
+def block_values(state, square=False):
+    """What an 8-bit moment stands for, in float32; `square` for the second one, which is held as its root."""
+    codes, scales = state
+    x = codes.reshape(-1).float() * scales.repeat_interleave(BLOCK)[:codes.numel()]
+    return (x * x if square else x).view(codes.shape)
+
+
+def _pointers(tensors):
+    return (C.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def _scalar(x, name, dev):
+    if isinstance(x, torch.Tensor):
+        if x.dtype != torch.float32 or x.numel() != 1 or x.device != dev:
+            raise ValueError(f"{name}: a float32 tensor of one element on {dev} expected, got {x.dtype} {tuple(x.shape)} on {x.device}")
+        return x
+    return None
+
+
+def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, seed=0):
+    """One AdamW step over lists of tensors, in place.
+
+    params and grads: all float32 or all bfloat16, contiguous, one device.  exp_avgs and exp_avg_sqs: float32 tensors, or pairs
+    (codes, scales) as `block_state` makes them, which hold m and sqrt(v) in 8 bits (all tensors alike).  step: the number of this step, from 1.
+    step and lr may be float32 tensors of one element on the device, which a captured graph reads anew at every replay.  seed: of the random
+    numbers that round 8-bit moments; take another one for every step (with a step tensor it changes by itself)."""
+    n = len(params)
+    if not n == len(grads) == len(exp_avgs) == len(exp_avg_sqs):
+        raise ValueError(f"lists of one length expected, got {n}, {len(grads)}, {len(exp_avgs)} and {len(exp_avg_sqs)}")
+    if n == 0:
+        return
+    dtype, dev = params[0].dtype, params[0].device
+    if dtype not in _DTYPES:
+        raise TypeError(f"parameters must be float32 or bfloat16, got {dtype}")
+    held = not isinstance(exp_avgs[0], torch.Tensor)
+    scales = None
+    if held:
+        try:
+            (ms, m_scales), (vs, v_scales) = zip(*exp_avgs), zip(*exp_avg_sqs)
+        except (TypeError, ValueError):
+            raise TypeError("exp_avgs and exp_avg_sqs must be all tensors or all pairs (codes, scales)") from None
+        scales = m_scales + v_scales
+        if not all(isinstance(t, torch.Tensor) for t in scales):
+            raise TypeError("exp_avgs and exp_avg_sqs must be all tensors or all pairs (codes, scales)")
+    else:
+        ms, vs = exp_avgs, exp_avg_sqs
+    state = torch.float8_e4m3fn if held else torch.float32
+    sizes = [p.numel() for p in params]
+    for what, tensors, want in (("params", params, dtype), ("grads", grads, dtype), ("exp_avgs", ms, state), ("exp_avg_sqs", vs, state)):
+        for t, k in zip(tensors, sizes):
+            if not isinstance(t, torch.Tensor) or t.dtype != want or t.device != dev or t.numel() != k or not t.is_contiguous():
+                raise ValueError(f"{what}: contiguous {want} tensors of the parameters' sizes on {dev} expected" +
+                                 (f", got {t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else f", got {type(t).__name__}"))
+    if held:
+        for t, k in zip(scales, sizes + sizes):
+            if t.dtype != torch.float32 or t.device != dev or t.numel() != -(-k // BLOCK) or not t.is_contiguous():
+                raise ValueError(f"scales: contiguous float32 tensors of one element per {BLOCK} on {dev} expected, got {t.dtype} {tuple(t.shape)}")
+    _lib.require_cuda(params[0])
+    where = [t.data_ptr() for ts in (params, ms, vs) + ((scales,) if held else ()) for t in ts if t.numel()]
+    if len(set(where)) < len(where):
+        raise ValueError("a tensor that the step writes is given twice")
+    b1, b2 = betas
+    step_t, lr_t = _scalar(step, "step", dev), _scalar(lr, "lr", dev)
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and (step_t is not None or step >= 1)):
+        raise ValueError(f"betas in [0, 1), eps >= 0 and step >= 1 expected, got {betas}, {eps} and {step}")
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().ceeg_adamw_step(
+            n, (C.c_int64 * n)(*sizes), _pointers(params), _pointers(grads), _pointers(ms), _pointers(vs),
+            _pointers(m_scales) if held else None, _pointers(v_scales) if held else None, _DTYPES[dtype], 8 if held else 32,
+            0.0 if lr_t is not None else float(lr), float(b1), float(b2), float(eps), float(weight_decay), 1 if step_t is not None else int(step),
+            _lib.ptr(lr_t), _lib.ptr(step_t), int(seed) & (2**64 - 1), _lib.stream()), "ceeg_adamw_step")
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's update with one launch for (up to 56) tensors, and, with state_bits=8, moments of one byte an element (+ 4 per 256):
+    an optimizer state of a quarter of the size.  Tensors of fewer than `min_8bit_size` elements keep theirs in 32 bits.
+
+    capturable=True keeps the step count on the device, so that `step()` can be captured into a graph and replayed; lr may then be a float32
+    tensor on the device too.  Parameters: float32 or bfloat16 on the GPU, contiguous, gradients of the same type."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, min_8bit_size=4096, seed=0, capturable=False):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and eps >= 0.0 and weight_decay >= 0.0):
+            raise ValueError(f"betas in [0, 1), eps >= 0 and weight_decay >= 0 expected, got {betas}, {eps} and {weight_decay}")
+        if not isinstance(lr, torch.Tensor) and lr < 0.0:
+            raise ValueError(f"lr >= 0 expected, got {lr}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, min_8bit_size=min_8bit_size,
+                                      seed=seed, capturable=capturable))
+
+    def _new_state(self, p, group):
+        held = group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"]
+        new = block_state if held else lambda t: torch.zeros_like(t, dtype=torch.float32, memory_format=torch.contiguous_format)  # noqa: E731
+        return dict(exp_avg=new(p), exp_avg_sq=new(p))
+
+    def load_state_dict(self, state_dict):
+        """As torch's, with the moments in the types that they were saved in (torch casts them to the parameter's)."""
+        super().load_state_dict(state_dict)
+        kept = lambda x, dev: tuple(t.detach().to(dev, copy=True) for t in x) if isinstance(x, tuple) else x.detach().to(dev, copy=True)  # noqa: E731
+        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            for p, i in zip(group["params"], saved["params"]):
+                if i in state_dict["state"]:
+                    self.state[p] = {k: kept(x, p.device) for k, x in state_dict["state"][i].items()}
+            if isinstance(group.get("step"), torch.Tensor) or (group["capturable"] and "step" in group):
+                count = float(group["step"])
+                group["step"] = torch.full((), count, dtype=torch.float32, device=group["params"][0].device) if group["capturable"] else int(count)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        ordinal = 0
+        for group in self.param_groups:
+            lists = {}  # one call takes tensors of one type, one device and one form of state
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                st = self.state[p]
+                if not st:
+                    st.update(self._new_state(p, group))
+                lists.setdefault((p.dtype, p.device, isinstance(st["exp_avg"], tuple)), []).append(p)
+            if not lists:
+                continue
+            if group["capturable"]:
+                if len({dev for _, dev, _ in lists}) > 1:
+                    raise ValueError("capturable: a group's parameters must be on one device")
+                if not isinstance(group.get("step"), torch.Tensor):
+                    group["step"] = torch.full((), float(group.get("step", 0)), dtype=torch.float32, device=next(iter(lists))[1])
+                group["step"] += 1
+            else:
+                group["step"] = group.get("step", 0) + 1
+            for ps in lists.values():
+                seed = group["seed"] + (ordinal << 32)  # another stream for every list
+                ordinal += 1
+                if not group["capturable"]:
+                    seed += group["step"] * _SPREAD
+                adamw_step_(ps, [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in ps], [self.state[p]["exp_avg"] for p in ps],
+                            [self.state[p]["exp_avg_sq"] for p in ps], group["step"], lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                            weight_decay=group["weight_decay"], seed=seed)
+        return loss

@@ -12,6 +12,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from .losses import balance_loss
 
 
 class _VQFunction(torch.autograd.Function):
@@ -99,3 +100,16 @@ class VectorQuantizer(nn.Module):
             min_encodings = torch.zeros(min_encoding_indices.shape[0], self.n_e, device=z.device)
             min_encodings.scatter_(1, min_encoding_indices, 1)
         return loss, z_q, perplexity, min_encodings, min_encoding_indices
+
+    def balance(self, z, indices, temperature=1.0, mask=None):
+        """(loss, counts): the balance loss over the codes that `indices` [B] or [B, 1] (min_encoding_indices) gives the rows of z, with the
+        softmax of -|z - e|^2 / temperature as each row's probabilities (|z|^2 drops out of it).  Added to the training loss it spreads the
+        rows over codes that are hardly used; its gradient reaches z and the codebook.  mask [B] bool: rows that count."""
+        _lib.require_cuda(z, self.embedding.weight)
+        if z.dim() != 2 or z.shape[1] != self.e_dim:
+            raise ValueError(f"z must be [B, {self.e_dim}], got {tuple(z.shape)}")
+        if not temperature > 0:
+            raise ValueError(f"temperature must be positive, got {temperature}")
+        w = self.embedding.weight
+        scores = torch.addmm((w * w).sum(1), z.to(w.dtype), w.t(), beta=-1.0 / temperature, alpha=2.0 / temperature)
+        return balance_loss(scores, indices, mask=mask)

@@ -23,7 +23,8 @@ from .trainer import Trainer
 
 
 def train_csv(nodes_csv, edges_csv, epochs=5, steps_per_epoch=20, in_dim=32, latent=16, codes=64, beta=0.25, features=None, weighted=True,
-              negatives="uniform", seed=0, device="cuda", log=None):
+              negatives="uniform", seed=0, device="cuda", log=None,
+              optimizer="adam", state_bits=32, balance=0.0):
     """Returns (model, history): history[e] = mean loss of epoch e.  Raises CeegError without a GPU / libceeg.so."""
     g = ingest.load_event_graph_csv(nodes_csv, edges_csv)
     N = g["num_nodes"]
@@ -38,8 +39,8 @@ def train_csv(nodes_csv, edges_csv, epochs=5, steps_per_epoch=20, in_dim=32, lat
         x = torch.randn(N, in_dim, generator=torch.Generator().manual_seed(seed)).to(dev)
     graph = EventGraph(ei, N, edge_weight=ew)
     torch.manual_seed(seed)
-    model = VGAEVQ(x.shape[1], latent, codes, beta, seed=seed, negatives=negatives).to(dev)
-    trainer = Trainer(model, lr=1e-3)
+    model = VGAEVQ(x.shape[1], latent, codes, beta, seed=seed, negatives=negatives, balance=balance).to(dev)
+    trainer = Trainer(model, lr=1e-3, optimizer=optimizer, state_bits=state_bits)
     history = []
     for epoch in range(epochs):
         model.train()
@@ -68,9 +69,12 @@ def main(argv=None):
     ap.add_argument("--features", default=None)
     ap.add_argument("--unweighted", action="store_true")
     ap.add_argument("--negatives", default="uniform", choices=["uniform", "sigma"])
+    ap.add_argument("--optimizer", default="adam", choices=["adam", "adamw"])
+    ap.add_argument("--state-bits", type=int, default=32, choices=[8, 32], help="of AdamW's moments")
+    ap.add_argument("--balance", type=float, default=0.0, help="weight of the balance loss over the codes")
     a = ap.parse_args(argv)
     train_csv(a.nodes_csv, a.edges_csv, a.epochs, a.steps_per_epoch, a.in_dim, a.latent, a.codes, features=a.features,
-              weighted=not a.unweighted, negatives=a.negatives, log=print)
+              weighted=not a.unweighted, negatives=a.negatives, log=print, optimizer=a.optimizer, state_bits=a.state_bits, balance=a.balance)
     return 0
 
 

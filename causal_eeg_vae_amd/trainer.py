@@ -4,6 +4,8 @@ averaging over RCCL (one flat all-reduce per step; one process per GPU, graph sh
 import torch
 import torch.distributed as dist
 
+from .optim import AdamW
+
 
 def allreduce_grads_(params, world_size, force=False):
     """Average gradients across ranks with ONE flat all-reduce (sum) followed by 1/world_size.  force=True runs the exchange
@@ -52,7 +54,11 @@ def broadcast_params_(module, src=0):
 
 
 class Trainer:
-    def __init__(self, model, lr=1e-3, world_size=1, force_exchange=False):
+    def __init__(self, model, lr=1e-3, world_size=1, force_exchange=False, optimizer="adam", weight_decay=1e-2, state_bits=32):
+        """optimizer: "adam" (the reference's, scripts/run.py:56) or "adamw", which takes weight_decay, and with state_bits=8 holds its moments in
+        one byte an element (causal_eeg_vae_amd.AdamW)."""
+        if optimizer not in ("adam", "adamw"):
+            raise ValueError(f"optimizer must be 'adam' or 'adamw', got {optimizer!r}")
         self.model = model
         self.world_size = int(world_size)
         self.force_exchange = bool(force_exchange)   # broadcast + all-reduce even with one rank (one-GPU RCCL rehearsal)
@@ -61,7 +67,10 @@ class Trainer:
             from . import _lib
             _lib.enable_tuned_gemms()   # library kernels picked for the step's GEMM shapes on an MI355X (lookup table, no tuning)
         # scripts/run.py:56; on the GPU the single-kernel (fused) form of the same update: 7 launches -> 1 per step
-        self.opt = torch.optim.Adam(self.params, lr=lr, fused=all(p.is_cuda for p in self.params))
+        if optimizer == "adam":
+            self.opt = torch.optim.Adam(self.params, lr=lr, fused=all(p.is_cuda for p in self.params))
+        else:
+            self.opt = AdamW(self.params, lr=lr, weight_decay=weight_decay, state_bits=state_bits)
         self.sched = torch.optim.lr_scheduler.ReduceLROnPlateau(self.opt)  # scripts/run.py:57 (defaults)
         self.step_idx = 0
         if self.world_size > 1 or self.force_exchange:

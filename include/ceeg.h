@@ -572,6 +572,62 @@ int ceeg_neg_filter_build(const int32_t* rowptr, const int32_t* col, int64_t N, 
 int ceeg_neg_sample_uniform_filtered(const int32_t* rowptr, const int32_t* col, int64_t N, int64_t num, uint64_t seed,
                                      const uint32_t* filter, int filter_bits, int32_t* neg_src, int32_t* neg_dst, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Softmax cross entropy behind a vocabulary product (the reference's recon_loss over a language decoder's hidden states,
+ * scripts/gpt2.py:1080-1084, scripts/models.py:34) and its gradient, without the logits in memory:
+ *   l_tv = <h_t, W_v>;  lse_t = log sum_v exp l_tv;  loss_t = lse_t - l_t,y(t)
+ *   dl_tv = s_t (exp(l_tv - lse_t) - [v = y(t)]);  dh = dl W;  dW = dl^T h        (s_t: what comes back for loss_t)
+ * h [T, H] (row stride ldh), W [V, H] (row stride ldw), y [T] int64, dtype CEEG_F32 or CEEG_BF16 for h, W, dh, dW; every sum, maximum and
+ * accumulator is fp32.  CEEG_F32 runs as six products of bf16 pieces (terms down to 2^-24 of the result).
+ * Tokens with y == ignore_index take no part: loss 0, dh row 0, whatever their row of h holds (also NaN).  A class outside [0, V) that is not
+ * ignore_index is not an error code (that would need a host read): its loss, and every gradient that it reaches, is NaN.
+ * reduction 0: loss [T]; 1: mean over the tokens that count (0 where none does) -> loss [1]; 2: sum -> loss [1].
+ * lse [T] fp32 and tokens [3 T + 1] int32 are written by the forward for the backward: how many tokens count, which, their place and class.
+ * g: what comes back for loss (fp32, [T] or [1]).  dh [T, H] and dW [V, H] contiguous, either may be NULL.
+ * Limits: T <= 2^22, H <= 2^15, V <= 2^28, ldw <= 2^22; bf16 with H a multiple of 64 reads W in place: 16-byte aligned, ldw a multiple of 8.
+ * The backward's workspace holds dl for a piece of the vocabulary; pieces are chosen so that they take about 1 GiB at most together.
+ * ----------------------------------------------------------------------------------------------*/
+size_t ceeg_linear_ce_fwd_ws_bytes(int64_t T, int64_t H, int64_t V, int dtype);
+size_t ceeg_linear_ce_bwd_ws_bytes(int64_t T, int64_t H, int64_t V, int dtype);
+int ceeg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, const int64_t* y, int64_t T, int64_t H, int64_t V, int dtype,
+                       int64_t ignore_index, int reduction, float* loss, float* lse, int32_t* tokens, void* ws, size_t ws_bytes, void* stream);
+int ceeg_linear_ce_bwd(const void* h, int64_t ldh, const void* W, int64_t ldw, int64_t T, int64_t H, int64_t V, int dtype, int reduction,
+                       const float* g, const float* lse, const int32_t* tokens, void* dh, void* dw, void* ws, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Balance loss over an assignment of rows to codes (the quantiser's min_encoding_indices, scripts/quantizer.py:48) or experts, with
+ * the per-code counts; no reference counterpart of its own (the reference only reports the perplexity of the counts, quantizer.py:64-65):
+ *   p = softmax(scores);  n = rows that count;  counts_e = #{(t, j): row t counts, idx[t, j] = e};  f = counts / (n K);  P = sum_t p_t / n
+ *   loss = E sum_e f_e P_e (1 where codes are used evenly);   dscores[t, e] = g E / n * p_te (f_e - sum_e' f_e' p_te')
+ * scores [T, E] (row stride ld, CEEG_F32 or CEEG_BF16), idx [T, K] int32 / int64 (idx_bytes 4 / 8; -1: no assignment; the same code twice in a
+ * row counts twice), mask [T] bytes or NULL (0: the row does not count: no count, no probability, gradient 0).  A row of nothing but -inf has no
+ * probability anywhere.  No row that counts: loss 0, gradient 0.  A code outside [-1, E) makes loss and gradient NaN.
+ * stats [E + 1] fp32 (f and n) is written by the forward for the backward; counts [E] int64; dscores [T, E] contiguous, 16-byte aligned.
+ * Limits: 1 <= E <= 4096, 1 <= K <= E, T < 2^31, T K <= 2^38.
+ * ----------------------------------------------------------------------------------------------*/
+size_t ceeg_balance_ws_bytes(int64_t T, int E);
+int ceeg_balance_fwd(const void* scores, int64_t ld, int dtype, const void* idx, int idx_bytes, int64_t T, int E, int K, const uint8_t* mask,
+                     float* loss, int64_t* counts, float* stats, void* ws, size_t ws_bytes, void* stream);
+int ceeg_balance_bwd(const void* scores, int64_t ld, int dtype, int64_t T, int E, const uint8_t* mask, const float* stats, const float* g,
+                     void* dscores, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * AdamW over a list of tensors (the update of scripts/run.py:56,97 with decoupled weight decay), in place, moments in 32 bits or in 8:
+ *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+ * numel, p, g, m, v (and m_scale, v_scale where state_bits = 8) are HOST arrays of `tensors` entries; the pointers travel in the kernel
+ * arguments, 56 tensors a launch, so nothing has to outlive the call.  dtype: of p and g.  Empty tensors are skipped (and keep their place).
+ * state_bits 32: m, v fp32.  state_bits 8: m and sqrt(v) as e4m3 bytes times one fp32 scale per ceeg_adamw_block() = 256 consecutive elements
+ * (scale = largest finite magnitude * fl(1 / 448); below 2^-100 the block is held as zeros); a magnitude is rounded up with the probability that
+ * keeps the expectation of m, or of v, by 16 bits of Philox 4x32-10 (key seed; counter {element / 4, 0x41444D57, place of the tensor}; word element % 4,
+ * low half for m, high half for v); sqrt(v) > 0 never becomes 0.  A gradient that is not finite makes its element NaN and nothing else.
+ * step >= 1: the number of this step.  lr_dev / step_dev (fp32 on the device, or NULL) replace lr / step where a captured graph replays the call;
+ * with step_dev the key is seed + step * 0x9E3779B97F4A7C15.
+ * ----------------------------------------------------------------------------------------------*/
+int ceeg_adamw_block(void);
+int ceeg_adamw_step(int tensors, const int64_t* numel, void* const* p, const void* const* g, void* const* m, void* const* v,
+                    float* const* m_scale, float* const* v_scale, int dtype, int state_bits, double lr, double beta1, double beta2,
+                    double eps, double weight_decay, int64_t step, const float* lr_dev, const float* step_dev, uint64_t seed, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
