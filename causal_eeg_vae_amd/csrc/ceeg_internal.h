@@ -40,6 +40,13 @@ __device__ __forceinline__ unsigned short ceeg_f32_to_bf16(float f) {
   return (unsigned short)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
 }
 
+// two of them in one 32-bit word (the first in the low half), by the hardware's conversion: the same rounding
+__device__ __forceinline__ unsigned ceeg_f32_to_bf16x2(float a, float b) {
+  using f2 = __attribute__((ext_vector_type(2))) float;
+  using h2 = __attribute__((ext_vector_type(2))) __bf16;
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{a, b}, h2));
+}
+
 __device__ __forceinline__ float ceeg_wave_sum(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);

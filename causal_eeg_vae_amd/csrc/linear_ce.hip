@@ -8,20 +8,20 @@
 //                small ones first - 6/16 of the bf16 rate instead of the 1/16 of the fp32 instruction.
 // Tokens that are ignored are dropped before the first product: their rows are packed away, the grids cover all T tokens and what
 // lies behind the last one that counts leaves at once (its number is read on the device, the host never waits for it).
-// The vocabulary is taken in pieces; of a piece only dl is held (bf16, as it is and transposed), so that every product reads both
-// operands along its summed axis.  No float atomics: the pieces of a sum are added in a fixed order.
+// The vocabulary is taken in pieces; of a piece only dl is held (bf16).  A product whose operand runs across the summed axis (W in dh, h and dl in
+// dW) reads it through the transposing LDS read, so nothing is ever stored transposed.  No float atomics: the pieces of a sum are added in a fixed order.
+#include <limits.h>
 #include "ceeg_internal.h"
 
 namespace {
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using f32x4 = __attribute__((ext_vector_type(4))) float;
+using i32x4 = __attribute__((ext_vector_type(4))) int;
 
-constexpr int BK = 64;                                   // elements of the summed axis per LDS tile
+constexpr int PAD = 64;                                  // rows and columns of the packed operands are padded to this with zeros
 constexpr int64_t CE_CAP = (int64_t)1 << 30;             // bytes that the pieces of the backward pass may take together
 constexpr int64_t CE_MAX_PIECE = (int64_t)1 << 20;       // columns per piece: 32-bit offsets inside a tile
-// planes of A and B in the products (2,0) (0,2) (1,1) | (1,0) (0,1) | (0,0), two bits each; a bar is a factor of 2^-8 on what is summed so far
-constexpr unsigned CE_PAIRS_A = 2u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
-constexpr unsigned CE_PAIRS_B = 0u | 2u << 2 | 1u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
+__host__ __device__ constexpr int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 
 // x = p[0] + 2^-8 p[1] + 2^-16 p[2], each rounded to nearest.  Without the powers of two the lower planes of a small x would fall below what bf16
 // holds (2^-133); with them every fp32 number, subnormal ones too, is held to its last bit.  What rounds past the largest bf16 number is cut
@@ -86,192 +86,355 @@ __global__ __launch_bounds__(1024) void ce_tokens_kernel(const int64_t* __restri
 }
 
 // ------------------------------------------------------------------------------------------------ planes
-// 64 x 64 tiles of a row-major [R, C] matrix (rows taken through `rows` where given, R from the device where `count` is given)
-//   -> planes row by row [P][*][Cp] (`out`, columns C..Cp zero) and / or transposed [P][C][Rp] (`outT`, rows R.. to the next multiple of 64 zero)
+// Row-major [R, C] (rows taken through `rows` where given, R from the device where `count` is given) -> planes [P][*][Cp], columns C..Cp zero; `zeros`:
+// the rows behind the last, up to the next multiple of PAD, zero too (a sum over the rows runs over them).  A thread moves eight columns.
 template <bool F32>
-__global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ src, int64_t ld, const int32_t* __restrict__ rows,
-                                                      const int32_t* __restrict__ count, int R, int C, unsigned short* __restrict__ out, int64_t plane, int Cp,
-                                                      unsigned short* __restrict__ outT, int64_t planeT, int64_t Rp) {
-  __shared__ float s_t[64][65];
-  const int n = count ? count[0] : R;
-  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
-  if (r0 >= n) return;
-  const int cq = (threadIdx.x & 15) * 4, rr = threadIdx.x >> 4;
-  const bool vec = (ld & 3) == 0 && (reinterpret_cast<uintptr_t>(src) & (F32 ? 15 : 7)) == 0;
+__global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ src, int64_t ld, const int32_t* __restrict__ rows, const int32_t* __restrict__ count,
+                                                      int64_t R, int C, int Cp, int zeros, unsigned short* __restrict__ out, int64_t plane) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = Cp / 8;
+  const int64_t r = id / per;
+  const int c = (int)(id % per) * 8;
+  const int64_t n = count ? count[0] : R;
+  if (r >= (zeros ? up(n, PAD) : n)) return;
+  float x[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = r0 + rr + 16 * i, c = c0 + cq;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (r < n) {
-      const int64_t at = (rows ? (int64_t)rows[r] : (int64_t)r) * ld + c;
-      if (F32) {
-        const float* q = static_cast<const float*>(src) + at;
-        if (vec && c + 4 <= C) {
-          const float4 u = *reinterpret_cast<const float4*>(q);
-          x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) x[k] = c + k < C ? q[k] : 0.f;
-        }
+  for (int k = 0; k < 8; ++k) x[k] = 0.f;
+  if (r < n) {
+    const int64_t at = (rows ? (int64_t)rows[r] : r) * ld + c;
+    if (F32) {
+      const float* q = static_cast<const float*>(src) + at;
+      if (c + 8 <= C && (reinterpret_cast<uintptr_t>(q) & 15) == 0) {
+        const float4 u = reinterpret_cast<const float4*>(q)[0], v = reinterpret_cast<const float4*>(q)[1];
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
       } else {
-        const unsigned short* q = static_cast<const unsigned short*>(src) + at;
-        if (vec && c + 4 <= C) {
-          const ushort4 u = *reinterpret_cast<const ushort4*>(q);
-          x[0] = ceeg_bf16_to_f32(u.x); x[1] = ceeg_bf16_to_f32(u.y); x[2] = ceeg_bf16_to_f32(u.z); x[3] = ceeg_bf16_to_f32(u.w);
-        } else {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) x[k] = c + k < C ? ceeg_bf16_to_f32(q[k]) : 0.f;
-        }
+        for (int k = 0; k < 8; ++k) x[k] = c + k < C ? q[k] : 0.f;
       }
-    }
-    if (out && r < n) {
-      unsigned short p[4][3];
+    } else {
+      const unsigned short* q = static_cast<const unsigned short*>(src) + at;
+      if (c + 8 <= C && (reinterpret_cast<uintptr_t>(q) & 15) == 0) {
+        *reinterpret_cast<uint4*>(out + r * Cp + c) = *reinterpret_cast<const uint4*>(q);
+        return;
+      }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) ce_split(x[k], p[k]);
-#pragma unroll
-      for (int a = 0; a < (F32 ? 3 : 1); ++a)
-        *reinterpret_cast<ushort4*>(out + a * plane + (int64_t)r * Cp + c) = make_ushort4(p[0][a], p[1][a], p[2][a], p[3][a]);
-    }
-    if (outT) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) s_t[rr + 16 * i][cq + k] = x[k];
+      for (int k = 0; k < 8; ++k) x[k] = c + k < C ? ceeg_bf16_to_f32(q[k]) : 0.f;
     }
   }
-  if (!outT) return;
-  __syncthreads();
+  unsigned short p[8][3];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = c0 + rr + 16 * i;
-    if (c >= C) continue;
-    unsigned short p[4][3];
+  for (int k = 0; k < 8; ++k) ce_split(x[k], p[k]);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) ce_split(s_t[cq + k][rr + 16 * i], p[k]);
-#pragma unroll
-    for (int a = 0; a < (F32 ? 3 : 1); ++a)
-      *reinterpret_cast<ushort4*>(outT + a * planeT + (int64_t)c * Rp + r0 + cq) = make_ushort4(p[0][a], p[1][a], p[2][a], p[3][a]);
-  }
+  for (int a = 0; a < (F32 ? 3 : 1); ++a)
+    *reinterpret_cast<uint4*>(out + a * plane + r * Cp + c) =
+        make_uint4(p[0][a] | (uint32_t)p[1][a] << 16, p[2][a] | (uint32_t)p[3][a] << 16, p[4][a] | (uint32_t)p[5][a] << 16, p[6][a] | (uint32_t)p[7][a] << 16);
 }
 
 // ------------------------------------------------------------------------------------------------ products
-// C[n][m] = sum over pairs of planes, over k: A[m][k] B[n][k], both row-major along k (k a multiple of 64, zero-padded).  D's layout puts four consecutive m
-// of one n into a lane.  A workgroup computes BM x BN; k tiles of 64 go from HBM / L2 straight into LDS (buffer loads to LDS, 16 bytes a lane), two deep: the
-// next tile is on its way while this one is multiplied.  A row of a tile is 128 bytes = all banks once, so the 16-byte pieces of row r are stored
-// at piece ^ (r & 7): the 16 rows that a wave reads at a time then touch each bank equally.  The swizzle is applied to the address that a
-// lane loads from, since the LDS side of such a load is lane after lane.
+// D[n][m] = sum_k A[m][k] B[n][k].  The 16 x 16 result layout puts four consecutive m of one n into a lane, so D's rows are stored in pieces of four.
+// An operand lies along k ("row r holds r's k", 16-byte LDS reads) or across it ("row k holds all r", transposing LDS reads, which hand a
+// lane four consecutive k of its r).  A workgroup computes BM x BN; tiles of BK elements of k go from HBM / L2 straight into LDS (buffer loads to LDS, 16 bytes a
+// lane), ST deep: while one is multiplied the next ones are on their way, with one barrier a tile.
+// Bank conflicts: the LDS side of such a load is lane after lane, so the swizzle is applied to the address that a lane loads from.  Along k a row of the tile is
+// 64 bytes and its 16-byte pieces are stored at piece ^ (r / 2 mod 4): eight rows read together touch all banks once.  Across k the
+// 32-byte pieces (one 16 x 16 block) of row k are stored at piece ^ (k mod 4 + 4 (k / 8 mod 2)): the eight rows that half a wave reads then lie in eight
+// different pieces.
+// Three planes (fp32): of every k tile all planes are in LDS and the six products run from there; the planes' powers of two keep three accumulators,
+// joined at the end, small ones first.
+#if defined(__HIP_DEVICE_COMPILE__)
+// 16 bytes a lane from a buffer's base + v into LDS, lane after lane.  Written out because the compiler, which knows that such a load writes LDS, would
+// wait for all of them before every transposing read; run() waits for exactly those it needs.  It has no output register; m0, which the
+// compiler sets right before its own uses, takes a wait state to be read.
+__device__ __forceinline__ void ce_to_lds(i32x4 rsrc, uint32_t v, unsigned short* to) {
+  const uint32_t at = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)to);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(v), "s"(rsrc) : "memory");
+}
+#endif
+
+template <int N> struct Int { static constexpr int value = N; };
 struct CeMat {
   const unsigned short* p;
   int64_t ld, plane;
+  int r_end;                   // rows r there are: what lies behind is not read (the buffer's range check) and what it gives is never stored
+  const unsigned short* tail;  // across k: the last rows k, from k_tail on, zero-padded to PAD, lie here where the matrix itself is not padded
+  int k_tail;
 };
 
-template <int BM, int BN, int WM, int WN>
+template <int PL, int BM, int BN, int WM, int WN, int ST, bool AHEAD, bool TA, bool TB>
 struct CeTile {
   static constexpr int WAVES = WM * WN, THREADS = WAVES * 64;
+  static constexpr int BK = 32;  // one matrix instruction deep
   static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
-  static constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;  // 1 KB loads per wave
-  static constexpr int LDS = 2 * (BM + BN) * BK;                  // bf16 elements
+  static constexpr int LA = BM * BK / 512 / WAVES, LB = BN * BK / 512 / WAVES;  // 1 KB loads per wave, tile and plane
+  static constexpr int PLANE = (BM + BN) * BK, STAGE = PL * PLANE;              // bf16 elements of LDS
+  static constexpr int LDS = ST * STAGE;
+  static_assert(LA > 0 && LB > 0 && LA * WAVES * 512 == BM * BK && LB * WAVES * 512 == BN * BK, "whole loads");
+  static_assert(LDS * 2 <= 160 * 1024, "LDS");
   f32x4 acc[MT][NT];
 
-  __device__ __forceinline__ void run(const CeMat& A, const CeMat& B, int m0, int M, int n0, int N, int k0, int k1, int pairs, unsigned short* lds) {
-#if defined(__HIP_DEVICE_COMPILE__)  // the buffer resource's type is the device's alone
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave / WN, wn = wave % WN;
+  // Load i of a wave fetches 64 pieces of 16 bytes of the tile: rows `row(lane) + hop(i)`; a hop changes no bit of a row that the swizzle looks at, so that
+  // a lane's offset is the same for all loads.
+  template <bool T, int BR>
+  static __device__ __forceinline__ int hop(int i) {
+    return !T ? i * WAVES * 16 : BR == 256 ? i * 4 : i * 16;
+  }
+  template <bool T, int BR>
+  static __device__ __forceinline__ int row0(int wave) {
+    return !T ? wave * 16 : BR == 256 ? (wave & 1) * 2 + (wave >> 1) * 8 : wave * (512 / BR);  // 256: eight waves
+  }
+  template <bool T, int BR>
+  static __device__ __forceinline__ uint32_t offset(const CeMat& x, int wave, int lane) {
+    if (T) {
+      constexpr int CPR = BR / 8;  // pieces per row k
+      const int row = row0<T, BR>(wave) + lane / CPR, slot = lane % CPR, g = ((row & 3) | (row >> 3 & 1) << 2) & (BR / 16 - 1);
+      return (uint32_t)(lane / CPR) * (uint32_t)x.ld * 2u + (uint32_t)(((slot >> 1) ^ g) << 1 | (slot & 1)) * 16u;
+    }
+    const int row = lane >> 2;
+    return (uint32_t)row * (uint32_t)x.ld * 2u + (uint32_t)((lane & 3) ^ (row >> 1 & 3)) * 16u;
+  }
+  // bytes that may be read from the tile's first element on: to the end of its last row
+  template <bool T>
+  static __device__ __forceinline__ int64_t range(const CeMat& x, int r0) {
+    return T ? ((BK - 1) * x.ld + x.r_end - r0) * 2 : ((int64_t)(x.r_end - 1 - r0) * x.ld + BK) * 2;
+  }
+
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int nk = (k1 - k0) / BK, total = nk > 0 ? nk * pairs : 0;
-    // rows behind the last one read it again: what they give is never stored
-    uint32_t va[LA], vb[LB];
-    const int rl = lane >> 3, piece = (lane & 7) ^ rl;
-#pragma unroll
-    for (int i = 0; i < LA; ++i) va[i] = (uint32_t)min((i * WAVES + wave) * 8 + rl, M - 1 - m0) * (uint32_t)A.ld * 2u + piece * 16u;
-#pragma unroll
-    for (int i = 0; i < LB; ++i) vb[i] = (uint32_t)min((i * WAVES + wave) * 8 + rl, N - 1 - n0) * (uint32_t)B.ld * 2u + piece * 16u;
-    const unsigned short* const a0 = A.p + (int64_t)m0 * A.ld;
-    const unsigned short* const b0 = B.p + (int64_t)n0 * B.ld;
+  }
 
-    auto stage = [&](int pr, int k, int buf) {
-      const int pa = pairs == 1 ? 0 : CE_PAIRS_A >> (2 * pr) & 3, pb = pairs == 1 ? 0 : CE_PAIRS_B >> (2 * pr) & 3;
-      const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned short*>(a0 + pa * A.plane), 0, 0xffffffff, 0x00020000);
-      const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned short*>(b0 + pb * B.plane), 0, 0xffffffff, 0x00020000);
-      unsigned short* const sa = lds + buf * (BM + BN) * BK;
-      unsigned short* const sb = sa + BM * BK;
+  // k0 < k1, both multiples of PAD: at least two tiles, and an even number of them
+  __device__ __forceinline__ void run(const CeMat& A, const CeMat& B, int m0, int n0, int k0, int k1, unsigned short* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)  // the buffer resource's type is the device's alone
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN, l15 = lane & 15, q = lane >> 4;
+    clear();
+    f32x4 low[PL == 3 ? 2 : 1][MT][NT];
+    if constexpr (PL == 3) {
 #pragma unroll
-      for (int i = 0; i < LA; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(sa + (i * WAVES + wave) * 512), 16, va[i], k * 2, 0, 0);
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int i = 0; i < LB; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void*)(sb + (i * WAVES + wave) * 512), 16, vb[i], k * 2, 0, 0);
+        for (int j = 0; j < NT; ++j) low[0][i][j] = low[1][i][j] = acc[i][j];
+    }
+    const int total = (k1 - k0) / BK;
+    const uint32_t va = offset<TA, BM>(A, wave, lane), vb = offset<TB, BN>(B, wave, lane);
+    const int64_t na = range<TA>(A, m0), nb = range<TB>(B, n0);
+
+    auto fetch = [&](auto t, auto br, auto n, const CeMat& x, const unsigned short* p, int64_t bytes, uint32_t v, unsigned short* to) {
+#pragma unroll
+      for (int a = 0; a < PL; ++a) {
+#pragma unroll
+        for (int i = 0; i < n.value; ++i) {
+          const int r = row0<t.value != 0, br.value>(wave) + hop<t.value != 0, br.value>(i);
+          const uint64_t base = reinterpret_cast<uint64_t>(p + a * x.plane + r * x.ld);
+          const int64_t left = bytes - r * x.ld * 2;
+          const i32x4 rs = {(int)(uint32_t)base, (int)(uint32_t)(base >> 32), left < 0 ? 0 : left > 0x7fffffff ? 0x7fffffff : (int)left, 0x00020000};
+          ce_to_lds(rs, v, to + a * PLANE + r * (t.value ? br.value : BK));
+        }
+      }
     };
+    auto stage = [&](int it) {
+      const int k = k0 + it * BK;
+      unsigned short* const to = lds + it % ST * STAGE;
+      const unsigned short* pa = A.p + (TA ? (int64_t)k * A.ld + m0 : (int64_t)m0 * A.ld + k);
+      if (TA && k >= A.k_tail) pa = A.tail + (int64_t)(k - A.k_tail) * A.ld + m0;
+      fetch(Int<TA>{}, Int<BM>{}, Int<LA>{}, A, pa, na, va, to);
+      fetch(Int<TB>{}, Int<BN>{}, Int<LB>{}, B, B.p + (TB ? (int64_t)k * B.ld + n0 : (int64_t)n0 * B.ld + k), nb, vb, to + BM * BK);
+    };
+    // waits until tile `it` is there for every wave; `ahead`: how many tiles behind it have been asked for.  Every wave has then read all that it read before.
+    auto arrive = [&](int it, auto ahead) {
+      if (it + ahead.value < total) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ahead.value * PL * (LA + LB)) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last tiles: nothing is asked for behind them
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    };
+    const int g = (l15 >> 2) | (q & 1) << 2, at = (q ^ (l15 >> 1 & 3)) * 8, row = 8 * q + (l15 >> 2);
+    auto read_a = [&](int it, int p, int i) { return read<TA, BM>(lds + it % ST * STAGE + p * PLANE, wm * MT + i, l15, at, row, g); };
+    auto read_b = [&](int it, int p, int j) { return read<TB, BN>(lds + it % ST * STAGE + p * PLANE + BM * BK, wn * NT + j, l15, at, row, g); };
 
-    int pr = 0, k = k0;  // of the tile that is fetched next
-    if (total > 0) stage(0, k0, 0);
-    const int r = lane & 15, q = lane >> 4;
-    for (int it = 0; it < total; ++it) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();  // this tile is there, and nobody reads the other buffer any more
-      if (pairs > 1 && k == k0 && (pr == 3 || pr == 5)) {  // the first tile of a product that the ones so far are 2^-8 of
+    if constexpr (AHEAD) {
+      // The next tile's fragments are read while this one's are multiplied, so that after a barrier no wave waits for LDS before it can go on.
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int j = 0; j < NT; ++j) acc[i][j] *= 0x1p-8f;
-      }
-      k += BK;
-      if (k >= k1) { k = k0; ++pr; }
-      if (it + 1 < total) stage(pr, k, (it + 1) & 1);
-      const unsigned short* const sa = lds + (it & 1) * (BM + BN) * BK + (wm * MT * 16 + r) * BK;
-      const unsigned short* const sb = lds + (it & 1) * (BM + BN) * BK + BM * BK + (wn * NT * 16 + r) * BK;
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const int at = ((kk * 4 + q) ^ (r & 7)) * 8;
+      for (int s = 0; s < ST; ++s)
+        if (s < total) stage(s);
+      struct Frag {
         bf16x8 a[MT], b[NT];
+      };
+      auto load = [&](Frag& f, int it) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) a[i] = *reinterpret_cast<const bf16x8*>(sa + i * 16 * BK + at);
+        for (int j = 0; j < NT; ++j) f.b[j] = read_b(it, 0, j);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) b[j] = *reinterpret_cast<const bf16x8*>(sb + j * 16 * BK + at);
+        for (int i = 0; i < MT; ++i) f.a[i] = read_a(it, 0, i);
+      };
+      auto mul = [&](const Frag& f) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
+          for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.a[i], f.b[j], acc[i][j], 0, 0, 0);
+      };
+      Frag f0, f1;
+      arrive(0, Int<ST - 1>{});
+      load(f0, 0);
+      auto step = [&](int it, const Frag& now, Frag& next) {
+        arrive(it + 1, Int<ST - 2>{});
+        if (it + ST < total) stage(it + ST);
+        load(next, it + 1);
+        mul(now);
+        constexpr int READS = MT * (TA ? 2 : 1) + NT * (TB ? 2 : 1), EACH = MT * NT / READS;
+#pragma unroll
+        for (int i = 0; i < READS; ++i) {  // a read between every few products
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+        }
+      };
+      for (int it = 0; it + 2 < total; it += 2) {
+        step(it, f0, f1);
+        step(it + 1, f1, f0);
       }
+      step(total - 2, f0, f1);
+      mul(f1);
+    } else {
+#pragma unroll
+      for (int s = 0; s < ST - 1; ++s)
+        if (s < total) stage(s);
+      for (int it = 0; it < total; ++it) {
+        arrive(it, Int<ST - 2>{});
+        if (it + ST - 1 < total) stage(it + ST - 1);
+        bf16x8 a[PL][MT], b[PL][NT];
+#pragma unroll
+        for (int p = 0; p < PL; ++p) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j) b[p][j] = read_b(it, p, j);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) a[p][i] = read_a(it, p, i);
+        }
+        auto mul = [&](f32x4 (&to)[MT][NT], int pa, int pb) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) to[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[pa][i], b[pb][j], to[i][j], 0, 0, 0);
+        };
+        if constexpr (PL == 3) {
+          mul(low[1], 2, 0); mul(low[1], 0, 2); mul(low[1], 1, 1);
+          mul(low[0], 1, 0); mul(low[0], 0, 1);
+        }
+        mul(acc, 0, 0);
+      }
+    }
+    if constexpr (PL == 3) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] += (low[0][i][j] + low[1][i][j] * 0x1p-8f) * 0x1p-8f;
     }
     __syncthreads();
 #endif
   }
+
+#if defined(__HIP_DEVICE_COMPILE__)
+  template <bool T, int BR>
+  static __device__ __forceinline__ bf16x8 read(const unsigned short* s, int block, int l15, int at, int row, int g) {
+    if (!T) return *reinterpret_cast<const bf16x8*>(s + (block * 16 + l15) * BK + at);
+    using s16x4 = __attribute__((ext_vector_type(4))) short;
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    const unsigned short* const p = s + row * BR + ((block ^ (g & (BR / 16 - 1))) * 16 + (l15 & 3) * 4);
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p);
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * BR));  // rows 4 further swizzle the same
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+#endif
 };
 
-// Workgroups go to the eight XCDs in turn: give each XCD a run of consecutive tiles, which share operands in its L2
-__device__ __forceinline__ int ce_xcd(int b, int n) {
-  const int per = n / 8, rest = n % 8, x = b % 8, i = b / 8;
-  return x * per + (x < rest ? x : rest) + i;
+// The tile shapes.  256 x 256 on eight waves reads LDS least per product and fills the chip from 256 tiles up (one workgroup per compute unit); 128 x 128 halves what is lost on
+// smaller grids; 64 x 64 spreads the smallest, which are bound by latency, and keeps more tiles on their way.
+template <int PL, bool TA, bool TB> struct CeBig { using Tile = CeTile<1, 256, 256, 2, 4, 4, false, TA, TB>; };
+template <int PL, bool TA, bool TB> struct CeMid { using Tile = CeTile<1, 128, 128, 2, 2, 4, true, TA, TB>; };
+template <bool TA, bool TB> struct CeMid<3, TA, TB> { using Tile = CeTile<3, 128, 128, 4, 2, 3, false, TA, TB>; };
+template <int PL, bool TA, bool TB> struct CeSmall { using Tile = CeTile<1, 64, 64, 2, 2, 8, true, TA, TB>; };
+template <bool TA, bool TB> struct CeSmall<3, TA, TB> { using Tile = CeTile<3, 64, 64, 2, 2, 4, false, TA, TB>; };
+
+// exp(x - base).  bf16: one fused multiply-add in front of the instruction, whose rounding of base * log2(e) is worth 2^-24 |base| of the result; fp32: the difference first.
+template <int PL>
+__device__ __forceinline__ float ce_exp(float x, float base) {
+  constexpr float LOG2E = 1.44269504088896341f;
+  return __builtin_amdgcn_exp2f(PL == 1 ? __fmaf_rn(x, LOG2E, -base * LOG2E) : (x - base) * LOG2E);
 }
 
-template <int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void ce_stats_kernel(CeMat W, CeMat h, const int32_t* __restrict__ n, const int32_t* __restrict__ yc, int v0, int Vc, int K,
-                                                                int pairs, int tiles_n, int part0, int parts, float2* __restrict__ part, float* __restrict__ at_y) {
-  using G = CeTile<BM, BN, WM, WN>;
+// four consecutive values of a row of H (left: how many of them there are), in the output's type
+template <bool F32>
+__device__ __forceinline__ void ce_store4(void* to, int64_t at, int left, int H, float a, float b, float c, float d) {
+  const float x[4] = {a, b, c, d};
+  if ((H & 3) == 0) {
+    if (F32) *reinterpret_cast<float4*>(static_cast<float*>(to) + at) = make_float4(a, b, c, d);
+    else *reinterpret_cast<ushort4*>(static_cast<unsigned short*>(to) + at) = make_ushort4(ceeg_f32_to_bf16(a), ceeg_f32_to_bf16(b), ceeg_f32_to_bf16(c), ceeg_f32_to_bf16(d));
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (k >= left) continue;
+    if (F32) static_cast<float*>(to)[at + k] = x[k];
+    else static_cast<unsigned short*>(to)[at + k] = ceeg_f32_to_bf16(x[k]);
+  }
+}
+
+// Workgroups go to the eight XCDs in turn: each XCD gets a run of consecutive tiles (-1: none left for this workgroup) ...
+__device__ __forceinline__ int ce_xcd(int b, int n) {
+  const int per = n / 8, rest = n % 8, x = b % 8, i = b / 8;
+  return i < per + (x < rest) ? x * per + (x < rest ? x : rest) + i : -1;
+}
+// ... which are taken in bands of six along n, so that the 32 tiles which the XCD's compute units work on at a time share six by five operands in its L2
+__device__ __forceinline__ void ce_band(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
+  constexpr int W = 6;
+  const int band = id / (W * tiles_m), in = id - band * W * tiles_m, w = min(W, tiles_n - band * W);
+  tm = in / w;
+  tn = band * W + in - tm * w;
+}
+
+template <class G, int PL, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(G::THREADS, 1) void ce_stats_kernel(CeMat W, CeMat h, const int32_t* __restrict__ n, const int32_t* __restrict__ yc, int v0, int K, int part0,
+                                                              int parts, float2* __restrict__ part, float* __restrict__ at_y) {
   __shared__ __align__(16) unsigned short lds[G::LDS];
-  const int id = ce_xcd(blockIdx.x, gridDim.x);
-  const int tm = id / tiles_n, m0 = tm * BM, n0 = id % tiles_n * BN, N = n[0];
-  if (n0 >= N) return;
+  const int N = n[0], Vc = W.r_end, tiles_m = (Vc + BM - 1) / BM, tiles_n = (N + BN - 1) / BN;
+  const int id = ce_xcd(blockIdx.x, tiles_m * tiles_n);
+  if (id < 0) return;
+  int tm, tn;
+  ce_band(id, tiles_m, tiles_n, tm, tn);
+  const int m0 = tm * BM, n0 = tn * BN;
+  h.r_end = N;
   G g;
-  g.run(W, h, m0, Vc, n0, N, 0, K, pairs, lds);
+  g.run(W, h, m0, n0, 0, K, lds);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN, q = lane >> 4;
   float2* const s = reinterpret_cast<float2*>(lds);  // [WM][BN]
-#pragma unroll
-  for (int j = 0; j < G::NT; ++j) {
-    const int cl = (wn * G::NT + j) * 16 + (lane & 15), t = n0 + cl;
-    const int y = t < N ? yc[t] - v0 : -1;
-    float top = -INFINITY;
+  const int vb = m0 + wm * G::MT * 16;
+  // About 7 instructions a logit are a fifth of the product's time at H = 1024: the mask of the last tile and the search for the tokens' own classes
+  // run only where a wave has some.
+  if (vb + G::MT * 16 > Vc) {
 #pragma unroll
     for (int i = 0; i < G::MT; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int v = m0 + (wm * G::MT + i) * 16 + 4 * q + k;
-        if (v >= Vc) g.acc[i][j][k] = -INFINITY;
-        else if (v == y) at_y[t] = g.acc[i][j][k];
-        top = fmaxf(top, g.acc[i][j][k]);
-      }
+      for (int k = 0; k < 4; ++k)
+        if (vb + i * 16 + 4 * q + k >= Vc) {
+#pragma unroll
+          for (int j = 0; j < G::NT; ++j) g.acc[i][j][k] = -INFINITY;
+        }
+  }
+#pragma unroll
+  for (int j = 0; j < G::NT; ++j) {
+    const int cl = (wn * G::NT + j) * 16 + (lane & 15), t = n0 + cl;
+    const int y = t < N ? yc[t] - v0 - vb : -1;
+    if (__any(y >= 0 && y < G::MT * 16)) {
+#pragma unroll
+      for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i * 16 + 4 * q + k == y) at_y[t] = g.acc[i][j][k];
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < G::MT; ++i) top = fmaxf(top, fmaxf(fmaxf(g.acc[i][j][0], g.acc[i][j][1]), fmaxf(g.acc[i][j][2], g.acc[i][j][3])));
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float base = top == -INFINITY ? 0.f : top;
@@ -279,7 +442,7 @@ __global__ __launch_bounds__(WM * WN * 64) void ce_stats_kernel(CeMat W, CeMat h
 #pragma unroll
     for (int i = 0; i < G::MT; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum += __expf(g.acc[i][j][k] - base);
+      for (int k = 0; k < 4; ++k) sum += ce_exp<PL>(g.acc[i][j][k], base);
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
     if (q == 0) s[wm * BN + cl] = make_float2(top, sum);
@@ -366,88 +529,126 @@ __global__ __launch_bounds__(1024) void ce_scale_kernel(const int32_t* __restric
   if (threadIdx.x == 0) scale[0] = reduction == 0 ? top : reduction == 1 ? g[0] / (float)(N > 0 ? N : 1) : g[0];
 }
 
-// dl of one piece of the vocabulary, [P][T][ldv] and [P][ldv][Tp]
-template <int P, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void ce_dlogits_kernel(CeMat W, CeMat h, const int32_t* __restrict__ n, const int32_t* __restrict__ yc,
-                                                                  const float* __restrict__ lse, const float* __restrict__ r, int v0, int Vc, int ldv, int64_t T, int64_t Tp,
-                                                                  int K, int pairs, int tiles_n, unsigned short* __restrict__ dl, unsigned short* __restrict__ dlT) {
-  using G = CeTile<BM, BN, WM, WN>;
+// dl of one piece of the vocabulary, [P][T][ldv]; columns behind the piece and the rows up to the next multiple of PAD are zero
+template <class G, int PL, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(G::THREADS, 1) void ce_dlogits_kernel(CeMat W, CeMat h, const int32_t* __restrict__ n, const int32_t* __restrict__ yc, const float* __restrict__ lse,
+                                                                const float* __restrict__ r, int v0, int ldv, int64_t plane, int K, unsigned short* __restrict__ dl) {
   __shared__ __align__(16) unsigned short lds[G::LDS];
-  const int id = ce_xcd(blockIdx.x, gridDim.x);
-  const int m0 = id / tiles_n * BM, n0 = id % tiles_n * BN, N = n[0];
-  if (n0 >= N) return;
+  const int N = n[0], Vc = W.r_end, tiles_m = (Vc + BM - 1) / BM, tiles_n = (N + BN - 1) / BN;
+  const int id = ce_xcd(blockIdx.x, tiles_m * tiles_n);
+  if (id < 0) return;
+  int tm, tn;
+  ce_band(id, tiles_m, tiles_n, tm, tn);
+  const int m0 = tm * BM, n0 = tn * BN;
+  h.r_end = N;
   G g;
-  g.run(W, h, m0, Vc, n0, N, 0, K, pairs, lds);
+  g.run(W, h, m0, n0, 0, K, lds);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN, q = lane >> 4;
-  const int Nz = (N + 63) & ~63;  // the transposed copy is summed over its tokens in steps of 64: zero behind the last
+  const int Nz = (int)up(N, PAD), vb = m0 + wm * G::MT * 16;
 #pragma unroll
   for (int j = 0; j < G::NT; ++j) {
     const int t = n0 + (wn * G::NT + j) * 16 + (lane & 15);
-    const int y = t < N ? yc[t] - v0 : -1;
+    const int y = t < N ? yc[t] - v0 - vb : -1;
     const float l = t < N ? lse[t] : 0.f, rt = t < N ? r[t] : 0.f;
 #pragma unroll
+    for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) g.acc[i][j][k] = rt * ce_exp<PL>(g.acc[i][j][k], l);
+    if (__any(y >= 0 && y < G::MT * 16)) {
+#pragma unroll
+      for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i * 16 + 4 * q + k == y) g.acc[i][j][k] -= rt;
+    }
+    if (vb + G::MT * 16 > Vc || n0 + BN > N) {
+#pragma unroll
+      for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (t >= N || vb + i * 16 + 4 * q + k >= Vc) g.acc[i][j][k] = 0.f;  // whatever was multiplied there
+    }
+    if (t >= Nz) continue;
+#pragma unroll
     for (int i = 0; i < G::MT; ++i) {
-      const int v = m0 + (wm * G::MT + i) * 16 + 4 * q;
+      const int v = vb + i * 16 + 4 * q;
       if (v >= ldv) continue;
-      unsigned short p[4][3];
+      f32x4 x = g.acc[i][j];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float x = 0.f;
-        if (t < N && v + k < Vc) x = rt * (__expf(g.acc[i][j][k] - l) - (v + k == y ? 1.f : 0.f));
-        if (P == 3) ce_split(x, p[k]); else p[k][0] = ceeg_f32_to_bf16(x);
-      }
-#pragma unroll
-      for (int a = 0; a < P; ++a) {
-        if (t < N) *reinterpret_cast<ushort4*>(dl + (a * T + t) * ldv + v) = make_ushort4(p[0][a], p[1][a], p[2][a], p[3][a]);
-        if (t < Nz) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) dlT[((int64_t)a * ldv + v + k) * Tp + t] = p[k][a];
+      for (int a = 0; a < PL; ++a) {
+        const uint2 p = make_uint2(ceeg_f32_to_bf16x2(x[0], x[1]), ceeg_f32_to_bf16x2(x[2], x[3]));
+        *reinterpret_cast<uint2*>(dl + a * plane + (int64_t)t * ldv + v) = p;
+        if (a + 1 < PL) {  // what the plane leaves, 2^8 times
+          x[0] = (x[0] - __uint_as_float(p.x << 16)) * 256.f;
+          x[1] = (x[1] - __uint_as_float(p.x & 0xffff0000u)) * 256.f;
+          x[2] = (x[2] - __uint_as_float(p.y << 16)) * 256.f;
+          x[3] = (x[3] - __uint_as_float(p.y & 0xffff0000u)) * 256.f;
         }
       }
     }
   }
 }
 
-// dh += dl W of one piece: split over the vocabulary into slots that are joined at the end, [slots][T][H]
-template <int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void ce_dh_kernel(CeMat WT, CeMat dl, const int32_t* __restrict__ n, int H, int64_t T, int K, int k_slot, int pairs,
-                                                             int tiles_m, int tiles, int add, float* __restrict__ slots) {
-  using G = CeTile<BM, BN, WM, WN>;
+// D of a product into fp32 slots [slots][rows][H], each holding a stretch of the sum (k_slot elements): dh += dl W (rows: tokens, A = W, B = dl) or dW = dl^T h (rows:
+// classes, A = h, B = dl).  A slot keeps its sum over the pieces (`add`).
+template <class G, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(G::THREADS, 1) void ce_slots_kernel(CeMat A, CeMat B, const int32_t* __restrict__ n, int by_tokens, int H, int64_t rows, int K, int slots, int add,
+                                                              float* __restrict__ out) {
   __shared__ __align__(16) unsigned short lds[G::LDS];
-  const int id = ce_xcd(blockIdx.x, gridDim.x);
-  const int slot = id / tiles, rest = id % tiles;
-  const int m0 = rest % tiles_m * BM, n0 = rest / tiles_m * BN, N = n[0];
-  if (n0 >= N) return;
-  const int k0 = min(slot * k_slot, K), k1 = min(k0 + k_slot, K);
+  const int N = n[0], end = by_tokens ? N : (int)rows;
+  const int tiles_m = (H + BM - 1) / BM, tiles = tiles_m * ((end + BN - 1) / BN), id = ce_xcd(blockIdx.x, tiles * slots);
+  if (id < 0) return;
+  const int slot = id / tiles, rest = id - slot * tiles;
+  const int m0 = rest % tiles_m * BM, n0 = rest / tiles_m * BN;
+  if (by_tokens) {   // the rows are tokens
+    B.r_end = N;
+  } else {           // the sum is over tokens
+    K = (int)up(N, PAD);
+  }
+  const int k_slot = (int)up((K + slots - 1) / slots, PAD), k0 = min(slot * k_slot, K), k1 = min(k0 + k_slot, K);
   G g;
-  g.run(WT, dl, m0, H, n0, N, k0, k1, pairs, lds);
+  if (k0 < k1) {
+    g.run(A, B, m0, n0, k0, k1, lds);
+  } else {
+    if (add) return;
+    g.clear();
+  }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN, q = lane >> 4;
 #pragma unroll
   for (int j = 0; j < G::NT; ++j) {
-    const int t = n0 + (wn * G::NT + j) * 16 + (lane & 15);
-    if (t >= N) continue;
-    float* const row = slots + (slot * T + t) * H;
+    const int r = n0 + (wn * G::NT + j) * 16 + (lane & 15);
+    if (r >= end) continue;
+    float* const to = out + (slot * rows + r) * H;
 #pragma unroll
     for (int i = 0; i < G::MT; ++i) {
       const int c = m0 + (wm * G::MT + i) * 16 + 4 * q;
+      if ((H & 3) == 0) {
+        if (c < H) {
+          float4* const f = reinterpret_cast<float4*>(to + c);
+          float4 x = make_float4(g.acc[i][j][0], g.acc[i][j][1], g.acc[i][j][2], g.acc[i][j][3]);
+          if (add) { const float4 y = *f; x = make_float4(y.x + x.x, y.y + x.y, y.z + x.z, y.w + x.w); }
+          *f = x;
+        }
+      } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (c + k < H) row[c + k] = add ? row[c + k] + g.acc[i][j][k] : g.acc[i][j][k];
+        for (int k = 0; k < 4; ++k)
+          if (c + k < H) to[c + k] = add ? to[c + k] + g.acc[i][j][k] : g.acc[i][j][k];
+      }
     }
   }
 }
 
-// dW = s dl^T h of one piece
-template <bool F32, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void ce_dw_kernel(CeMat hT, CeMat dlT, const int32_t* __restrict__ n, const float* __restrict__ scale, int H, int Vc, int pairs,
-                                                             int tiles_m, void* __restrict__ dw) {
-  using G = CeTile<BM, BN, WM, WN>;
+// dW = s dl^T h of one piece, the whole sum in one workgroup
+template <class G, bool F32, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(G::THREADS, 1) void ce_dw_kernel(CeMat h, CeMat dl, const int32_t* __restrict__ n, const float* __restrict__ scale, int H, int Vc,
+                                                           void* __restrict__ dw) {
   __shared__ __align__(16) unsigned short lds[G::LDS];
-  const int id = ce_xcd(blockIdx.x, gridDim.x);
-  const int m0 = id % tiles_m * BM, n0 = id / tiles_m * BN, K = (n[0] + 63) & ~63;
+  const int tiles_m = (H + BM - 1) / BM, id = ce_xcd(blockIdx.x, gridDim.x);
+  const int m0 = id % tiles_m * BM, n0 = id / tiles_m * BN, K = (int)up(n[0], PAD);
   G g;
-  g.run(hT, dlT, m0, H, n0, Vc, 0, K, pairs, lds);
-  const float s = scale[0];
+  if (K > 0) g.run(h, dl, m0, n0, 0, K, lds);
+  else g.clear();
+  const float s = K == 0 ? 0.f : scale[0];  // no token counts: the empty sum is zero whatever comes back
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN, q = lane >> 4;
 #pragma unroll
   for (int j = 0; j < G::NT; ++j) {
@@ -456,16 +657,23 @@ __global__ __launch_bounds__(WM * WN * 64) void ce_dw_kernel(CeMat hT, CeMat dlT
 #pragma unroll
     for (int i = 0; i < G::MT; ++i) {
       const int c = m0 + (wm * G::MT + i) * 16 + 4 * q;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (c + k >= H) continue;
-        // no token counts: the empty sum is zero whatever comes back
-        const float x = K == 0 ? 0.f : s * g.acc[i][j][k];
-        if (F32) static_cast<float*>(dw)[(int64_t)v * H + c + k] = x;
-        else static_cast<unsigned short*>(dw)[(int64_t)v * H + c + k] = ceeg_f32_to_bf16(x);
-      }
+      if (c >= H) continue;
+      ce_store4<F32>(dw, (int64_t)v * H + c, H - c, H, s * g.acc[i][j][0], s * g.acc[i][j][1], s * g.acc[i][j][2], s * g.acc[i][j][3]);
     }
   }
+}
+
+// the slots of dW joined
+template <bool F32>
+__global__ __launch_bounds__(256) void ce_dw_join_kernel(const float* __restrict__ part, int slots, const int32_t* __restrict__ n, const float* __restrict__ scale, int64_t count,
+                                                         void* __restrict__ dw) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= count) return;
+  float x = 0.f;
+  for (int k = 0; k < slots; ++k) x += part[k * count + i];
+  x = n[0] == 0 ? 0.f : x * scale[0];
+  if (F32) static_cast<float*>(dw)[i] = x;
+  else static_cast<unsigned short*>(dw)[i] = ceeg_f32_to_bf16(x);
 }
 
 template <bool F32>
@@ -486,39 +694,58 @@ __global__ __launch_bounds__(256) void ce_dh_join_kernel(const float* __restrict
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-constexpr int TB = 128;  // tile
-inline int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
+constexpr int TMIN = 64;  // the smallest tile: what is counted in tiles is sized for it
+
+// Tile edge for a grid of rows x columns (x the ways its sum may be cut): the largest that gives every compute unit a workgroup
+int ce_edge(int planes, int64_t rows, int64_t cols, int64_t cuts) {
+  const auto tiles = [&](int64_t e) { return ((rows + e - 1) / e) * ((cols + e - 1) / e); };
+  if (planes == 1 && tiles(256) * cuts >= 200) return 256;
+  if (tiles(128) * cuts >= 200) return 128;
+  return 64;
+}
 
 struct CePlan {
-  int P, pairs;
+  int P;
   bool direct;           // W is read where it is
   int64_t Kp, Tp;        // padded H, padded T
   int64_t piece, ldv;    // columns of a piece of the vocabulary, padded
-  int pieces, slots;
+  int pieces;
+  int e_logits, e_dh, e_dw;         // tile edges
+  int dh_slots, dw_slots;           // stretches that the sums are cut into
 };
+
+// how often a sum of k elements is cut for a grid of `tiles`: until the compute units hold as many workgroups as their LDS allows, 256 elements a stretch at least
+int ce_cuts(int planes, int edge, int64_t tiles, int64_t k) {
+  const int64_t want = planes == 3 || edge == 256 ? 256 : 512;
+  int64_t s = (want + tiles - 1) / tiles;
+  if (s > k / 256) s = k / 256;
+  if (s > 64) s = 64;
+  return (int)(s < 1 ? 1 : s);
+}
 
 CePlan ce_plan(int64_t T, int64_t H, int64_t V, int dtype, bool backward) {
   CePlan c;
   c.P = dtype == CEEG_F32 ? 3 : 1;
-  c.pairs = dtype == CEEG_F32 ? 6 : 1;
-  c.direct = dtype == CEEG_BF16 && H % BK == 0;
-  c.Kp = up(H, BK);
-  c.Tp = up(T, BK);
-  const int64_t column = c.P * ((backward ? 4 * c.Tp + 2 * H : 0) + (c.direct ? 0 : 2 * c.Kp));
+  c.direct = dtype == CEEG_BF16 && H % PAD == 0;
+  c.Kp = up(H, PAD);
+  c.Tp = up(T, PAD);
+  const int64_t column = c.P * ((backward ? 2 * c.Tp : 0) + (c.direct ? 0 : 2 * c.Kp));
   int64_t piece = V;
   if (column > 0 && piece > CE_CAP / column) piece = CE_CAP / column;
   if (piece > CE_MAX_PIECE) piece = CE_MAX_PIECE;
-  if (piece < TB) piece = TB;
+  if (piece < 256) piece = 256;
   c.pieces = (int)((V + piece - 1) / piece);
-  c.piece = up((V + c.pieces - 1) / c.pieces, TB);
+  c.piece = up((V + c.pieces - 1) / c.pieces, 256);
   c.pieces = (int)((V + c.piece - 1) / c.piece);
-  c.ldv = up(c.piece < V ? c.piece : V, BK);
-  // dh: few tiles (T H against V columns of sum), so the sum is cut until about two workgroups per compute unit are busy
-  const int64_t tiles = ((T + TB - 1) / TB) * ((H + TB - 1) / TB);
-  int64_t s = (512 + tiles - 1) / tiles;
-  if (s > c.ldv / (4 * BK)) s = c.ldv / (4 * BK);
-  if (s > 64) s = 64;
-  c.slots = (int)(s < 1 ? 1 : s);
+  c.ldv = up(c.piece < V ? c.piece : V, PAD);
+  const int64_t cols = c.piece < V ? c.piece : V;
+  c.e_logits = ce_edge(c.P, cols, T, 1);
+  const auto tiles = [&](int64_t a, int64_t b, int64_t e) { return ((a + e - 1) / e) * ((b + e - 1) / e); };
+  c.e_dh = ce_edge(c.P, H, T, c.ldv / 1024 + 1);
+  c.dh_slots = ce_cuts(c.P, c.e_dh, tiles(H, T, c.e_dh), c.ldv);
+  c.e_dw = ce_edge(c.P, H, cols, T / 1024 + 1);
+  c.dw_slots = ce_cuts(c.P, c.e_dw, tiles(H, cols, c.e_dw), T);
+  if (tiles(H, cols, c.e_dw) >= 200) c.dw_slots = 1;
   return c;
 }
 
@@ -530,30 +757,45 @@ int ce_check(const void* h, int64_t ldh, const void* W, int64_t ldw, int64_t T, 
   if (!ce_sizes_ok(T, H, V) || ldw > (1 << 22)) return CEEG_EUNSUPPORTED;
   const size_t e = dtype == CEEG_F32 ? 4 : 2;
   if (!ceeg_aligned(h, e) || !ceeg_aligned(W, e)) return CEEG_EINVAL;
-  if (dtype == CEEG_BF16 && H % BK == 0 && (ldw % 8 || !ceeg_aligned(W, 16))) return CEEG_EINVAL;
+  if (dtype == CEEG_BF16 && H % PAD == 0 && (ldw != H || !ceeg_aligned(W, 16))) return CEEG_EINVAL;
   return CEEG_OK;
 }
 
 size_t ce_fwd_bytes(int64_t T, int64_t H, int64_t V, int dtype) {
   const CePlan c = ce_plan(T, H, V, dtype, false);
-  const size_t parts = (size_t)(V + TB - 1) / TB;
-  return ceeg_ws_part((size_t)c.P * T * c.Kp, 2) + (c.direct ? 0 : ceeg_ws_part((size_t)c.P * c.piece * c.Kp, 2)) + ceeg_ws_part((size_t)T * parts, 8) +
+  const size_t parts = (size_t)(V + TMIN - 1) / TMIN;
+  return ceeg_ws_part((size_t)c.P * c.Tp * c.Kp, 2) + (c.direct ? 0 : ceeg_ws_part((size_t)c.P * c.piece * c.Kp, 2)) + ceeg_ws_part((size_t)T * parts, 8) +
          2 * ceeg_ws_part(T, 4);
 }
 size_t ce_bwd_bytes(int64_t T, int64_t H, int64_t V, int dtype) {
   const CePlan c = ce_plan(T, H, V, dtype, true);
-  return ceeg_ws_part((size_t)c.P * T * c.Kp, 2) + ceeg_ws_part((size_t)c.P * H * c.Tp, 2) + (c.direct ? 0 : ceeg_ws_part((size_t)c.P * c.piece * c.Kp, 2)) +
-         ceeg_ws_part((size_t)c.P * H * c.ldv, 2) + ceeg_ws_part((size_t)c.P * T * c.ldv, 2) + ceeg_ws_part((size_t)c.P * c.ldv * c.Tp, 2) +
-         ceeg_ws_part((size_t)c.slots * T * H, 4) + ceeg_ws_part(1, 4) + ceeg_ws_part(T, 4);
+  return ceeg_ws_part((size_t)c.P * c.Tp * c.Kp, 2) + (c.direct ? ceeg_ws_part((size_t)PAD * c.Kp, 2) : ceeg_ws_part((size_t)c.P * c.piece * c.Kp, 2)) + ceeg_ws_part((size_t)c.P * c.Tp * c.ldv, 2) +
+         ceeg_ws_part((size_t)c.dh_slots * T * H, 4) + (c.dw_slots > 1 ? ceeg_ws_part((size_t)c.dw_slots * c.piece * H, 4) : 0) + ceeg_ws_part(1, 4) + ceeg_ws_part(T, 4);
 }
 
-void ce_pack(int dtype, const void* src, int64_t ld, const int32_t* rows, const int32_t* count, int64_t R, int64_t C, unsigned short* out, int64_t plane, int64_t Cp,
-             unsigned short* outT, int64_t planeT, int64_t Rp, hipStream_t st) {
-  const dim3 grid((unsigned)((R + 63) / 64), (unsigned)((C + 63) / 64));
-  if (dtype == CEEG_F32) ce_pack_kernel<true><<<grid, 256, 0, st>>>(src, ld, rows, count, (int)R, (int)C, out, plane, (int)Cp, outT, planeT, Rp);
-  else ce_pack_kernel<false><<<grid, 256, 0, st>>>(src, ld, rows, count, (int)R, (int)C, out, plane, (int)Cp, outT, planeT, Rp);
+void ce_pack(int dtype, const void* src, int64_t ld, const int32_t* rows, const int32_t* count, int64_t R, int64_t C, int64_t Cp, bool zeros, unsigned short* out, int64_t plane,
+             hipStream_t st) {
+  const unsigned grid = (unsigned)(((zeros ? up(R, PAD) : R) * (Cp / 8) + 255) / 256);
+  if (dtype == CEEG_F32) ce_pack_kernel<true><<<grid, 256, 0, st>>>(src, ld, rows, count, R, (int)C, (int)Cp, zeros, out, plane);
+  else ce_pack_kernel<false><<<grid, 256, 0, st>>>(src, ld, rows, count, R, (int)C, (int)Cp, zeros, out, plane);
 }
 inline const void* ce_at(const void* p, int64_t n, int dtype) { return static_cast<const char*>(p) + n * (dtype == CEEG_F32 ? 4 : 2); }
+
+// CALL with (tile, edge in classes, edge in tokens, waves in each): the planes and the edge chosen
+#define CE_TILES(PLANES, EDGE, TA, TB, CALL)                                    \
+  do {                                                                          \
+    if ((PLANES) == 3) {                                                        \
+      if ((EDGE) == 128) { CALL(3, 128, 4, 2, (CeMid<3, TA, TB>::Tile)); }      \
+      else { CALL(3, 64, 2, 2, (CeSmall<3, TA, TB>::Tile)); }                   \
+    } else {                                                                    \
+      if ((EDGE) == 256) { CALL(1, 256, 2, 4, (CeBig<1, TA, TB>::Tile)); }      \
+      else if ((EDGE) == 128) { CALL(1, 128, 2, 2, (CeMid<1, TA, TB>::Tile)); } \
+      else { CALL(1, 64, 2, 2, (CeSmall<1, TA, TB>::Tile)); }                   \
+    }                                                                           \
+  } while (0)
+template <class> struct CeArg;
+template <class X> struct CeArg<void(X)> { using type = X; };
+#define CE_TILE_OF(T) typename CeArg<void T>::type
 }  // namespace
 
 extern "C" size_t ceeg_linear_ce_fwd_ws_bytes(int64_t T, int64_t H, int64_t V, int dtype) {
@@ -570,9 +812,9 @@ extern "C" int ceeg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int
   if (!y || !ceeg_aligned(y, 8) || !loss || !lse || !tokens || reduction < 0 || reduction > 2) return CEEG_EINVAL;
   if (!ws || !ceeg_aligned(ws, 256) || ws_bytes < ce_fwd_bytes(T, H, V, dtype)) return CEEG_EWORKSPACE;
   const CePlan c = ce_plan(T, H, V, dtype, false);
-  const int parts = (int)((V + TB - 1) / TB);
+  const int parts = (int)((V + c.e_logits - 1) / c.e_logits);
   CeegWs w(ws, ws_bytes);
-  unsigned short* hc = w.take<unsigned short>((size_t)c.P * T * c.Kp);
+  unsigned short* hc = w.take<unsigned short>((size_t)c.P * c.Tp * c.Kp);
   unsigned short* wc = c.direct ? nullptr : w.take<unsigned short>((size_t)c.P * c.piece * c.Kp);
   float2* part = w.take<float2>((size_t)T * parts);
   float* at_y = w.take<float>(T);
@@ -582,20 +824,23 @@ extern "C" int ceeg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int
   const hipStream_t st = static_cast<hipStream_t>(stream);
   ce_tokens_kernel<<<1, 1024, 0, st>>>(y, T, V, ignore_index, n, rows, pos, yc);
   CEEG_CHECK_LAUNCH();
-  ce_pack(dtype, h, ldh, rows, n, T, H, hc, T * c.Kp, c.Kp, nullptr, 0, 0, st);
+  ce_pack(dtype, h, ldh, rows, n, T, H, c.Kp, false, hc, c.Tp * c.Kp, st);
   CEEG_CHECK_LAUNCH();
-  const int tiles_n = (int)((T + TB - 1) / TB);
-  const CeMat Bm{hc, c.Kp, T * c.Kp};
+  const int e = c.e_logits, tiles_n = (int)((T + e - 1) / e);
+  const CeMat Bm{hc, c.Kp, c.Tp * c.Kp, 0, nullptr, INT_MAX};
   for (int p = 0; p < c.pieces; ++p) {
     const int64_t v0 = p * c.piece, Vc = V - v0 < c.piece ? V - v0 : c.piece;
-    CeMat A{static_cast<const unsigned short*>(W) + v0 * ldw, ldw, 0};
+    CeMat A{static_cast<const unsigned short*>(W) + v0 * ldw, ldw, 0, (int)Vc, nullptr, INT_MAX};
     if (!c.direct) {
-      ce_pack(dtype, ce_at(W, v0 * ldw, dtype), ldw, nullptr, nullptr, Vc, H, wc, c.piece * c.Kp, c.Kp, nullptr, 0, 0, st);
+      ce_pack(dtype, ce_at(W, v0 * ldw, dtype), ldw, nullptr, nullptr, Vc, H, c.Kp, false, wc, c.piece * c.Kp, st);
       CEEG_CHECK_LAUNCH();
-      A = CeMat{wc, c.Kp, c.piece * c.Kp};
+      A = CeMat{wc, c.Kp, c.piece * c.Kp, (int)Vc, nullptr, INT_MAX};
     }
-    const int tiles_m = (int)((Vc + TB - 1) / TB);
-    ce_stats_kernel<TB, TB, 2, 2><<<tiles_m * tiles_n, 256, 0, st>>>(A, Bm, n, yc, (int)v0, (int)Vc, (int)c.Kp, c.pairs, tiles_n, (int)(v0 / TB), parts, part, at_y);
+    const int tiles_m = (int)((Vc + e - 1) / e);
+#define CE_CALL(PL, E, WM, WN, TILE) \
+  ce_stats_kernel<CE_TILE_OF(TILE), PL, E, E, WM, WN><<<tiles_m * tiles_n, WM * WN * 64, 0, st>>>(A, Bm, n, yc, (int)v0, (int)c.Kp, (int)(v0 / E), parts, part, at_y)
+    CE_TILES(c.P, e, false, false, CE_CALL);
+#undef CE_CALL
     CEEG_CHECK_LAUNCH();
   }
   ce_lse_kernel<<<(unsigned)((T + 3) / 4), 256, 0, st>>>(n, part, parts, at_y, yc, lse, rowloss);
@@ -613,13 +858,12 @@ extern "C" int ceeg_linear_ce_bwd(const void* h, int64_t ldh, const void* W, int
   if (!ws || !ceeg_aligned(ws, 256) || ws_bytes < ce_bwd_bytes(T, H, V, dtype)) return CEEG_EWORKSPACE;
   const CePlan c = ce_plan(T, H, V, dtype, true);
   CeegWs w(ws, ws_bytes);
-  unsigned short* hc = w.take<unsigned short>((size_t)c.P * T * c.Kp);
-  unsigned short* hT = w.take<unsigned short>((size_t)c.P * H * c.Tp);
+  unsigned short* hc = w.take<unsigned short>((size_t)c.P * c.Tp * c.Kp);
   unsigned short* wc = c.direct ? nullptr : w.take<unsigned short>((size_t)c.P * c.piece * c.Kp);
-  unsigned short* WT = w.take<unsigned short>((size_t)c.P * H * c.ldv);
-  unsigned short* dl = w.take<unsigned short>((size_t)c.P * T * c.ldv);
-  unsigned short* dlT = w.take<unsigned short>((size_t)c.P * c.ldv * c.Tp);
-  float* slots = w.take<float>((size_t)c.slots * T * H);
+  unsigned short* tail = c.direct ? w.take<unsigned short>((size_t)PAD * c.Kp) : nullptr;
+  unsigned short* dl = w.take<unsigned short>((size_t)c.P * c.Tp * c.ldv);
+  float* dh_slots = w.take<float>((size_t)c.dh_slots * T * H);
+  float* dw_slots = c.dw_slots > 1 ? w.take<float>((size_t)c.dw_slots * c.piece * H) : nullptr;
   float* scale = w.take<float>(1);
   float* r = w.take<float>(T);
   if (!w.ok) return CEEG_EWORKSPACE;
@@ -627,40 +871,61 @@ extern "C" int ceeg_linear_ce_bwd(const void* h, int64_t ldh, const void* W, int
   const hipStream_t st = static_cast<hipStream_t>(stream);
   ce_scale_kernel<<<1, 1024, 0, st>>>(n, rows, yc, g, reduction, scale, r);
   CEEG_CHECK_LAUNCH();
-  ce_pack(dtype, h, ldh, rows, n, T, H, hc, T * c.Kp, c.Kp, hT, H * c.Tp, c.Tp, st);
+  ce_pack(dtype, h, ldh, rows, n, T, H, c.Kp, true, hc, c.Tp * c.Kp, st);
   CEEG_CHECK_LAUNCH();
-  const int tiles_t = (int)((T + TB - 1) / TB), tiles_h = (int)((H + TB - 1) / TB);
+  const auto tiles = [](int64_t x, int e) { return (int)((x + e - 1) / e); };
+  const CeMat hm{hc, c.Kp, c.Tp * c.Kp, 0, nullptr, INT_MAX}, hk{hc, c.Kp, c.Tp * c.Kp, (int)c.Kp, nullptr, INT_MAX};
   for (int p = 0; p < c.pieces; ++p) {
-    const int64_t v0 = p * c.piece, Vc = V - v0 < c.piece ? V - v0 : c.piece, ldv = up(Vc, BK);
-    CeMat A{static_cast<const unsigned short*>(W) + v0 * ldw, ldw, 0};
-    ce_pack(dtype, ce_at(W, v0 * ldw, dtype), ldw, nullptr, nullptr, Vc, H, wc, c.piece * c.Kp, c.Kp, WT, H * ldv, ldv, st);
-    CEEG_CHECK_LAUNCH();
-    if (!c.direct) A = CeMat{wc, c.Kp, c.piece * c.Kp};
-    const int tiles_v = (int)((Vc + TB - 1) / TB);
-    const CeMat Bm{hc, c.Kp, T * c.Kp};
-    if (c.P == 3)
-      ce_dlogits_kernel<3, TB, TB, 2, 2><<<tiles_v * tiles_t, 256, 0, st>>>(A, Bm, n, yc, lse, r, (int)v0, (int)Vc, (int)ldv, T, c.Tp, (int)c.Kp, c.pairs, tiles_t, dl, dlT);
-    else
-      ce_dlogits_kernel<1, TB, TB, 2, 2><<<tiles_v * tiles_t, 256, 0, st>>>(A, Bm, n, yc, lse, r, (int)v0, (int)Vc, (int)ldv, T, c.Tp, (int)c.Kp, c.pairs, tiles_t, dl, dlT);
+    const int64_t v0 = p * c.piece, Vc = V - v0 < c.piece ? V - v0 : c.piece, ldv = up(Vc, PAD), plane = c.Tp * c.ldv;
+    CeMat A{static_cast<const unsigned short*>(W) + v0 * ldw, ldw, 0, (int)Vc, nullptr, INT_MAX};
+    if (!c.direct) {
+      ce_pack(dtype, ce_at(W, v0 * ldw, dtype), ldw, nullptr, nullptr, Vc, H, c.Kp, true, wc, c.piece * c.Kp, st);
+      CEEG_CHECK_LAUNCH();
+      A = CeMat{wc, c.Kp, c.piece * c.Kp, (int)Vc, nullptr, INT_MAX};
+    }
+    const int tiles_t = tiles(T, c.e_logits), tiles_v = tiles(ldv, c.e_logits);
+#define CE_CALL(PL, E, WM, WN, TILE)                                                                                                                                     \
+  ce_dlogits_kernel<CE_TILE_OF(TILE), PL, E, E, WM, WN><<<tiles_v * tiles_t, WM * WN * 64, 0, st>>>(A, hm, n, yc, lse, r, (int)v0, (int)ldv, plane, (int)c.Kp, dl)
+    CE_TILES(c.P, c.e_logits, false, false, CE_CALL);
+#undef CE_CALL
     CEEG_CHECK_LAUNCH();
     if (dh) {
-      const int k_slot = (int)up((ldv + c.slots - 1) / c.slots, BK);
-      ce_dh_kernel<TB, TB, 2, 2><<<tiles_h * tiles_t * c.slots, 256, 0, st>>>(CeMat{WT, ldv, H * ldv}, CeMat{dl, ldv, T * ldv}, n, (int)H, T, (int)ldv, k_slot, c.pairs, tiles_h,
-                                                                              tiles_h * tiles_t, p > 0, slots);
+      const CeMat Wk{A.p, A.ld, A.plane, (int)c.Kp, tail, c.direct && Vc % PAD ? (int)(Vc / PAD * PAD) : INT_MAX}, dlm{dl, ldv, plane, 0, nullptr, INT_MAX};
+      if (Wk.k_tail != INT_MAX) {
+        ce_pack(dtype, ce_at(W, (v0 + Wk.k_tail) * ldw, dtype), ldw, nullptr, nullptr, Vc % PAD, H, c.Kp, true, tail, 0, st);
+        CEEG_CHECK_LAUNCH();
+      }
+      const int all = tiles(H, c.e_dh) * tiles(T, c.e_dh);
+#define CE_CALL(PL, E, WM, WN, TILE)                                                                                                                                              \
+  ce_slots_kernel<CE_TILE_OF(TILE), E, E, WM, WN><<<all * c.dh_slots, WM * WN * 64, 0, st>>>(Wk, dlm, n, 1, (int)H, T, (int)ldv, c.dh_slots, p > 0, dh_slots)
+      CE_TILES(c.P, c.e_dh, true, false, CE_CALL);
+#undef CE_CALL
       CEEG_CHECK_LAUNCH();
     }
     if (dw) {
-      const CeMat At{hT, c.Tp, H * c.Tp}, Bt{dlT, c.Tp, ldv * c.Tp};
-      if (dtype == CEEG_F32)
-        ce_dw_kernel<true, TB, TB, 2, 2><<<tiles_h * tiles_v, 256, 0, st>>>(At, Bt, n, scale, (int)H, (int)Vc, c.pairs, tiles_h, static_cast<float*>(dw) + v0 * H);
-      else
-        ce_dw_kernel<false, TB, TB, 2, 2><<<tiles_h * tiles_v, 256, 0, st>>>(At, Bt, n, scale, (int)H, (int)Vc, c.pairs, tiles_h, static_cast<unsigned short*>(dw) + v0 * H);
+      const CeMat dlk{dl, ldv, plane, (int)ldv, nullptr, INT_MAX};
+      const int all = tiles(H, c.e_dw) * tiles(Vc, c.e_dw);
+      void* const to = const_cast<void*>(ce_at(dw, v0 * H, dtype));
+      if (c.dw_slots > 1) {
+#define CE_CALL(PL, E, WM, WN, TILE)                                                                                                                                      \
+  ce_slots_kernel<CE_TILE_OF(TILE), E, E, WM, WN><<<all * c.dw_slots, WM * WN * 64, 0, st>>>(hk, dlk, n, 0, (int)H, Vc, 0, c.dw_slots, 0, dw_slots)
+        CE_TILES(c.P, c.e_dw, true, true, CE_CALL);
+#undef CE_CALL
+        CEEG_CHECK_LAUNCH();
+        const unsigned grid = (unsigned)((Vc * H + 255) / 256);
+        if (dtype == CEEG_F32) ce_dw_join_kernel<true><<<grid, 256, 0, st>>>(dw_slots, c.dw_slots, n, scale, Vc * H, to);
+        else ce_dw_join_kernel<false><<<grid, 256, 0, st>>>(dw_slots, c.dw_slots, n, scale, Vc * H, to);
+      } else {
+#define CE_CALL(PL, E, WM, WN, TILE) ce_dw_kernel<CE_TILE_OF(TILE), PL == 3, E, E, WM, WN><<<all, WM * WN * 64, 0, st>>>(hk, dlk, n, scale, (int)H, (int)Vc, to)
+        CE_TILES(c.P, c.e_dw, true, true, CE_CALL);
+#undef CE_CALL
+      }
       CEEG_CHECK_LAUNCH();
     }
   }
   if (dh) {
-    if (dtype == CEEG_F32) ce_dh_join_kernel<true><<<(unsigned)T, 256, 0, st>>>(slots, c.slots, pos, scale, T, (int)H, dh);
-    else ce_dh_join_kernel<false><<<(unsigned)T, 256, 0, st>>>(slots, c.slots, pos, scale, T, (int)H, dh);
+    if (dtype == CEEG_F32) ce_dh_join_kernel<true><<<(unsigned)T, 256, 0, st>>>(dh_slots, c.dh_slots, pos, scale, T, (int)H, dh);
+    else ce_dh_join_kernel<false><<<(unsigned)T, 256, 0, st>>>(dh_slots, c.dh_slots, pos, scale, T, (int)H, dh);
     CEEG_CHECK_LAUNCH();
   }
   return CEEG_OK;

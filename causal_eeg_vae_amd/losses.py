@@ -31,10 +31,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
         dev = hidden.device
         if hidden.stride(1) != 1 or (T > 1 and hidden.stride(0) < H):
             hidden = hidden.contiguous()
-        if weight.stride(1) != 1 or (V > 1 and weight.stride(0) < H) or (dtype == _lib.CEEG_BF16 and (weight.data_ptr() % 16 or weight.stride(0) % 8)):
+        if weight.stride(1) != 1 or (V > 1 and weight.stride(0) < H) or (dtype == _lib.CEEG_BF16 and (weight.data_ptr() % 16 or not weight.is_contiguous())):
             weight = weight.clone(memory_format=torch.contiguous_format)
         target = target.contiguous()
-        ldh, ldw = max(hidden.stride(0), H), max(weight.stride(0), H)
+        ldh, ldw = max(hidden.stride(0), H), H if weight.is_contiguous() else weight.stride(0)
         with torch.cuda.device(dev):
             loss = torch.empty(T if reduction == 0 else 1, dtype=torch.float32, device=dev)
             lse = torch.empty(T, dtype=torch.float32, device=dev)

@@ -84,6 +84,15 @@ def test_mean_and_its_gradients(T, H, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("T,H,V", [(2100, 576, 25701), (700, 640, 9001), (3001, 129, 5003)])
+def test_every_tile_shape(T, H, V, dtype):
+    """Grids large enough for the larger tiles in each of the four products, with edges inside the last tile on every side."""
+    h, w, y = _inputs(T, H, V, dtype, ignored=0.1)
+    loss, dh, dw, g = _run(h, w, y)
+    _check(h, w, y, loss, dh, dw, "mean", g)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
 def test_reductions_and_upstream_gradients(reduction, dtype):
     h, w, y = _inputs(200, 72, 777, dtype, seed=3)

@@ -36,7 +36,7 @@ def test_linear_cross_entropy_entries_refuse():
     for entry, good, cases in (
             (L.ceeg_linear_ce_fwd, fwd, [(0, None, -1), (2, None, -1), (4, None, -1), (11, None, -1), (12, None, -1), (13, None, -1), (14, None, -3), (14, P + 1, -3),
                                          (15, 16, -3), (5, 0, -1), (6, 0, -1), (7, 0, -1), (1, 63, -1), (3, 63, -1), (8, 2, -2), (10, 3, -1), (10, -1, -1),
-                                         (5, (1 << 22) + 1, -2), (7, (1 << 28) + 1, -2), (3, 1 << 23, -2), (2, P + 2, -1), (3, 68, -1), (4, P + 4, -1)]),
+                                         (5, (1 << 22) + 1, -2), (7, (1 << 28) + 1, -2), (3, 1 << 23, -2), (2, P + 2, -1), (3, 72, -1), (4, P + 4, -1)]),
             (L.ceeg_linear_ce_bwd, bwd, [(0, None, -1), (2, None, -1), (9, None, -1), (10, None, -1), (11, None, -1), (14, None, -3), (15, 16, -3), (7, 5, -2), (8, 3, -1),
                                          (4, 0, -1), (2, P + 8, -1)])):
         for at, value, code in cases:
