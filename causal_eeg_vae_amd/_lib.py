@@ -3,6 +3,7 @@
 There is NO CPU fallback: if the shared library is missing or the call fails, this raises.  PyTorch is
 used only for device memory (tensors own every buffer, workspaces included) and the current stream.
 """
+import contextlib
 import ctypes as C
 import os
 
@@ -113,8 +114,9 @@ SIGNATURES = {
     "ceeg_neg_sample_uniform_filtered": (_c_int, [_vp, _vp, _c_i64, _c_i64, _c_u64, _vp, _c_int, _vp, _vp, _vp]),
     "ceeg_linear_ce_fwd_ws_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_int]),
     "ceeg_linear_ce_bwd_ws_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_int]),
-    "ceeg_linear_ce_fwd": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _vp, _vp, _vp, _vp, _c_sz, _vp]),
-    "ceeg_linear_ce_bwd": (_c_int, [_vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _c_sz, _vp]),
+    "ceeg_linear_ce_packed_bytes": (_c_sz, [_c_i64, _c_i64, _c_int]),
+    "ceeg_linear_ce_fwd": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _vp, _vp, _vp, _vp, _vp, _c_sz, _vp]),
+    "ceeg_linear_ce_bwd": (_c_int, [_vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _c_sz, _vp]),
     "ceeg_balance_ws_bytes": (_c_sz, [_c_i64, _c_int]),
     "ceeg_balance_fwd": (_c_int, [_vp, _c_i64, _c_int, _vp, _c_int, _c_i64, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _c_sz, _vp]),
     "ceeg_balance_bwd": (_c_int, [_vp, _c_i64, _c_int, _c_i64, _c_int, _vp, _vp, _vp, _vp, _vp]),
@@ -168,6 +170,11 @@ def ptr(t):
 
 def stream():
     return torch.cuda.current_stream().cuda_stream
+
+
+def on(device):
+    """Context in which `device` is the current one (nothing to enter where it is already)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def workspace(nbytes, device):

@@ -74,14 +74,27 @@ __device__ __forceinline__ void bl_softmax(int lanes, float (&x)[N]) {
   for (int k = 0; k < N; ++k) x[k] *= inv;
 }
 
-// per workgroup: part_p[wg][E] (column sums of p), part_c[wg][E] (counts), part_n[wg] = {rows that count, a code out of range was seen}
+struct BlOut {
+  float* loss;
+  int64_t* counts;
+  float* stats;
+};
+
+// f = counts / (n K) of one code, NaN where a code outside [-1, E) was seen: that cannot raise an error from here, so loss and gradient say it
+__device__ __forceinline__ double bl_share(long long c, double rows, int K, bool bad) {
+  return bad ? __longlong_as_double(0x7ff8000000000000LL) : (double)c / (rows * K);
+}
+
+// per workgroup: part_p[wg][E] (column sums of p), part_c[wg][E] (counts), part_n[wg] = {rows that count, a code out of range was seen}.
+// A grid of one workgroup (small calls, which launches would dominate) finishes by itself.
 template <bool BF16, int VEC, int NV>
 __global__ __launch_bounds__(BL_THREADS) void balance_rows_kernel(BlRow a, const void* __restrict__ idx, int idx64, int K, float* __restrict__ part_p,
-                                                                  int32_t* __restrict__ part_c, int2* __restrict__ part_n) {
+                                                                  int32_t* __restrict__ part_c, int2* __restrict__ part_n, BlOut out) {
   extern __shared__ int s_mem[];
   int* s_c = s_mem;                                    // [E]
   float* s_p = reinterpret_cast<float*>(s_mem + a.E);  // [E]
   __shared__ int s_n[2];
+  __shared__ double s_d[BL_WAVES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int e = threadIdx.x; e < a.E; e += BL_THREADS) s_c[e] = 0;
   if (threadIdx.x < 2) s_n[threadIdx.x] = 0;
@@ -135,6 +148,25 @@ __global__ __launch_bounds__(BL_THREADS) void balance_rows_kernel(BlRow a, const
   if (rows) atomicAdd(&s_n[0], rows);
   if (bad) atomicOr(&s_n[1], 1);
   __syncthreads();
+  if (gridDim.x == 1) {
+    const double n = s_n[0] > 0 ? (double)s_n[0] : 1.0;
+    double d = 0.0;
+    for (int e = threadIdx.x; e < a.E; e += BL_THREADS) {
+      const double f = bl_share(s_c[e], n, K, s_n[1] != 0);
+      out.counts[e] = s_c[e];
+      out.stats[e] = (float)f;
+      d += f * ((double)s_p[e] / n);
+    }
+    d = ceeg_wave_sum_d(d);
+    if (lane == 0) s_d[wave] = d;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < BL_WAVES; ++w) d += s_d[w];
+      out.stats[a.E] = (float)n;
+      out.loss[0] = (float)(d * a.E);
+    }
+    return;
+  }
   for (int e = threadIdx.x; e < a.E; e += BL_THREADS) {
     part_p[(int64_t)blockIdx.x * a.E + e] = s_p[e];
     part_c[(int64_t)blockIdx.x * a.E + e] = s_c[e];
@@ -176,10 +208,8 @@ __global__ __launch_bounds__(1024) void balance_join_kernel(const float* __restr
   if (w == 0) {
     p = 0.0; c = 0; n = 0;
     for (int k = 0; k < 16; ++k) { p += s_p[k][lane]; c += s_c[k][lane]; n += s_n[k]; }
-    // no row that counts: loss and gradient are zero.  A code outside [-1, E) cannot raise an error from here: it makes the loss and the gradient NaN.
-    const double rows = n > 0 ? (double)n : 1.0;
-    double f = (double)c / (rows * K);
-    if (s_bad) f = __longlong_as_double(0x7ff8000000000000LL);
+    const double rows = n > 0 ? (double)n : 1.0;  // no row that counts: loss and gradient are zero
+    const double f = bl_share(c, rows, K, s_bad != 0);
     double d = 0.0;
     if (e < E) {
       counts[e] = c;
@@ -337,8 +367,9 @@ extern "C" int ceeg_balance_fwd(const void* scores, int64_t ld, int dtype, const
   if (!w.ok) return CEEG_EWORKSPACE;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const size_t lds = (size_t)E * 8;  // 32 KB at most
-  BL_DISPATCH(balance_rows_kernel, <<<wgs, BL_THREADS, lds, st>>>(a, idx, idx_bytes == 8, K, part_p, part_c, part_n));
+  BL_DISPATCH(balance_rows_kernel, <<<wgs, BL_THREADS, lds, st>>>(a, idx, idx_bytes == 8, K, part_p, part_c, part_n, BlOut{loss, counts, stats}));
   CEEG_CHECK_LAUNCH();
+  if (wgs == 1) return CEEG_OK;
   const int joins = (E + 63) / 64;
   balance_join_kernel<<<joins, 1024, 0, st>>>(part_p, part_c, part_n, wgs, E, K, counts, stats, dots);
   CEEG_CHECK_LAUNCH();

@@ -20,6 +20,7 @@ using i32x4 = __attribute__((ext_vector_type(4))) int;
 
 constexpr int PAD = 64;                                  // rows and columns of the packed operands are padded to this with zeros
 constexpr int64_t CE_CAP = (int64_t)1 << 30;             // bytes that the pieces of the backward pass may take together
+constexpr int CE_SCAN = 4096;                           // tokens whose places a workgroup finds by itself
 constexpr int64_t CE_MAX_PIECE = (int64_t)1 << 20;       // columns per piece: 32-bit offsets inside a tile
 __host__ __device__ constexpr int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 
@@ -38,20 +39,29 @@ __device__ __forceinline__ void ce_split(float x, unsigned short (&p)[3]) {
 }
 
 // ------------------------------------------------------------------------------------------------ which tokens count
-// One workgroup: rows[j] = j-th token that counts, pos[t] = j or -1, yc[j] = its class (-1: outside [0, V)), n[0] = how many.
-__global__ __launch_bounds__(1024) void ce_tokens_kernel(const int64_t* __restrict__ y, int64_t T, int64_t V, int64_t ignore, int32_t* __restrict__ n,
-                                                         int32_t* __restrict__ rows, int32_t* __restrict__ pos, int32_t* __restrict__ yc) {
-  __shared__ int s_sum[16];
+// rows[j] = j-th token that counts, pos[t] = j or -1, yc[j] = its class (-1: outside [0, V)), n[0] = how many; `zeros`, where given, is cleared where a token does not.
+struct CeTokens {
+  const int64_t* y;
+  int64_t T, V, ignore;
+  int32_t *n, *rows, *pos, *yc;
+  float* zeros;
+};
+
+// All of them by one workgroup; `write`: into memory; `places` (LDS): pos, for up to CE_SCAN tokens.  Returns how many count.
+template <int THREADS>
+__device__ __forceinline__ int ce_scan(const CeTokens& a, bool write, int32_t* places) {
+  constexpr int WAVES = THREADS / 64;
+  __shared__ int s_sum[WAVES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int base = 0;
-  for (int64_t t0 = 0; t0 < T; t0 += 4096) {
+  for (int64_t t0 = 0; t0 < a.T; t0 += THREADS * 4) {
     const int64_t t = t0 + 4 * threadIdx.x;
     int64_t v[4];
     int mine = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      v[k] = t + k < T ? y[t + k] : ignore;
-      mine += v[k] != ignore;
+      v[k] = t + k < a.T ? a.y[t + k] : a.ignore;
+      mine += v[k] != a.ignore;
     }
     int pre = mine;
 #pragma unroll
@@ -63,47 +73,46 @@ __global__ __launch_bounds__(1024) void ce_tokens_kernel(const int64_t* __restri
     __syncthreads();
     int before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       before += w < wave ? s_sum[w] : 0;
       all += s_sum[w];
     }
     int j = base + before + pre - mine;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (t + k >= T) continue;
-      if (v[k] != ignore) {
-        rows[j] = (int32_t)(t + k);
-        yc[j] = v[k] >= 0 && v[k] < V ? (int32_t)v[k] : -1;
-        pos[t + k] = j++;
-      } else {
-        pos[t + k] = -1;
+      if (t + k >= a.T) continue;
+      const bool on = v[k] != a.ignore;
+      if (places) places[t + k] = on ? j : -1;
+      if (write) {
+        a.pos[t + k] = on ? j : -1;
+        if (on) {
+          a.rows[j] = (int32_t)(t + k);
+          a.yc[j] = v[k] >= 0 && v[k] < a.V ? (int32_t)v[k] : -1;
+        } else if (a.zeros) {
+          a.zeros[t + k] = 0.f;
+        }
       }
+      j += on;
     }
     base += all;
     __syncthreads();
   }
-  if (threadIdx.x == 0) n[0] = base;
+  if (write && threadIdx.x == 0) a.n[0] = base;
+  return base;
 }
 
+__global__ __launch_bounds__(1024) void ce_tokens_kernel(CeTokens a) { ce_scan<1024>(a, true, nullptr); }
+
 // ------------------------------------------------------------------------------------------------ planes
-// Row-major [R, C] (rows taken through `rows` where given, R from the device where `count` is given) -> planes [P][*][Cp], columns C..Cp zero; `zeros`:
-// the rows behind the last, up to the next multiple of PAD, zero too (a sum over the rows runs over them).  A thread moves eight columns.
+// eight columns c.. of a row of C at `src` (NULL: zeros) -> the planes at out
 template <bool F32>
-__global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ src, int64_t ld, const int32_t* __restrict__ rows, const int32_t* __restrict__ count,
-                                                      int64_t R, int C, int Cp, int zeros, unsigned short* __restrict__ out, int64_t plane) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int per = Cp / 8;
-  const int64_t r = id / per;
-  const int c = (int)(id % per) * 8;
-  const int64_t n = count ? count[0] : R;
-  if (r >= (zeros ? up(n, PAD) : n)) return;
+__device__ __forceinline__ void ce_pack8(const void* src, int c, int C, unsigned short* out, int64_t plane) {
   float x[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) x[k] = 0.f;
-  if (r < n) {
-    const int64_t at = (rows ? (int64_t)rows[r] : r) * ld + c;
+  if (src) {
     if (F32) {
-      const float* q = static_cast<const float*>(src) + at;
+      const float* q = static_cast<const float*>(src) + c;
       if (c + 8 <= C && (reinterpret_cast<uintptr_t>(q) & 15) == 0) {
         const float4 u = reinterpret_cast<const float4*>(q)[0], v = reinterpret_cast<const float4*>(q)[1];
         x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
@@ -112,9 +121,9 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ s
         for (int k = 0; k < 8; ++k) x[k] = c + k < C ? q[k] : 0.f;
       }
     } else {
-      const unsigned short* q = static_cast<const unsigned short*>(src) + at;
+      const unsigned short* q = static_cast<const unsigned short*>(src) + c;
       if (c + 8 <= C && (reinterpret_cast<uintptr_t>(q) & 15) == 0) {
-        *reinterpret_cast<uint4*>(out + r * Cp + c) = *reinterpret_cast<const uint4*>(q);
+        *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(q);
         return;
       }
 #pragma unroll
@@ -126,8 +135,45 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ s
   for (int k = 0; k < 8; ++k) ce_split(x[k], p[k]);
 #pragma unroll
   for (int a = 0; a < (F32 ? 3 : 1); ++a)
-    *reinterpret_cast<uint4*>(out + a * plane + r * Cp + c) =
+    *reinterpret_cast<uint4*>(out + a * plane) =
         make_uint4(p[0][a] | (uint32_t)p[1][a] << 16, p[2][a] | (uint32_t)p[3][a] << 16, p[4][a] | (uint32_t)p[5][a] << 16, p[6][a] | (uint32_t)p[7][a] << 16);
+}
+
+// Row-major [R, C] -> planes [P][*][Cp], columns C..Cp zero; `zeros`: the rows behind the last, up to the next multiple of PAD, zero too (a sum over the rows runs over them).
+template <bool F32>
+__global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ src, int64_t ld, int64_t R, int C, int Cp, int zeros, unsigned short* __restrict__ out, int64_t plane) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = Cp / 8;
+  const int64_t r = id / per;
+  const int c = (int)(id % per) * 8;
+  if (r >= (zeros ? up(R, PAD) : R)) return;
+  ce_pack8<F32>(r < R ? static_cast<const char*>(src) + r * ld * (F32 ? 4 : 2) : nullptr, c, C, out + r * Cp + c, plane);
+}
+
+// The hidden states of the tokens that count, packed; `each` tokens per workgroup, the last workgroup adds the zero rows.  SCAN: up to CE_SCAN tokens, whose places every
+// workgroup finds for itself (a few KB from L2) - one launch instead of two; otherwise ce_tokens_kernel has found them.
+template <bool F32, bool SCAN>
+__global__ __launch_bounds__(256) void ce_prepare_kernel(CeTokens a, const void* __restrict__ h, int64_t ld, int H, int Kp, int each, unsigned short* __restrict__ out, int64_t plane) {
+  __shared__ int32_t s_pos[SCAN ? CE_SCAN : 1];
+  int n;
+  if (SCAN) {
+    n = ce_scan<256>(a, blockIdx.x == 0, s_pos);
+    __syncthreads();
+  } else {
+    n = a.n[0];
+  }
+  const int per = Kp / 8;
+  const int64_t t0 = (int64_t)blockIdx.x * each;
+  for (int i = threadIdx.x; i < each * per; i += 256) {
+    const int64_t t = t0 + i / per;
+    if (t >= a.T) break;
+    const int j = SCAN ? s_pos[t] : a.pos[t], c = i % per * 8;
+    if (j >= 0) ce_pack8<F32>(static_cast<const char*>(h) + t * ld * (F32 ? 4 : 2), c, H, out + (int64_t)j * Kp + c, plane);
+  }
+  if (blockIdx.x == gridDim.x - 1) {
+    const int rows = (int)up(n, PAD) - n;
+    for (int i = threadIdx.x; i < rows * per; i += 256) ce_pack8<F32>(nullptr, i % per * 8, H, out + (int64_t)(n + i / per) * Kp + i % per * 8, plane);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ products
@@ -461,12 +507,8 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_stats_kernel(CeMat W, CeMat 
   }
 }
 
-// one wave per token that counts: joins the pieces' maxima and sums
-__global__ __launch_bounds__(256) void ce_lse_kernel(const int32_t* __restrict__ n, const float2* __restrict__ part, int parts, const float* __restrict__ at_y,
-                                                     const int32_t* __restrict__ yc, float* __restrict__ lse, float* __restrict__ loss) {
-  const int lane = threadIdx.x & 63;
-  const int64_t j = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (j >= n[0]) return;
+// A wave joins the pieces' maxima and sums of token j
+__device__ __forceinline__ float ce_join(const float2* __restrict__ part, int64_t j, int parts, int lane) {
   float top = -INFINITY;
   for (int c = lane; c < parts; c += 64) top = fmaxf(top, part[j * parts + c].x);
 #pragma unroll
@@ -477,62 +519,81 @@ __global__ __launch_bounds__(256) void ce_lse_kernel(const int32_t* __restrict__
     const float2 u = part[j * parts + c];
     sum += u.y * __expf(u.x - base);
   }
-  sum = ceeg_wave_sum(sum);
+  return base + logf(ceeg_wave_sum(sum));
+}
+// a class outside [0, V) cannot raise an error from here: its loss is NaN
+__device__ __forceinline__ float ce_row_loss(float lse, const float* __restrict__ at_y, const int32_t* __restrict__ yc, int64_t j) {
+  return yc[j] >= 0 ? lse - at_y[j] : __uint_as_float(0x7fc00000u);
+}
+
+// loss of token j to rowloss[j] (rows NULL) or to rowloss[rows[j]]
+__global__ __launch_bounds__(256) void ce_lse_kernel(const int32_t* __restrict__ n, const float2* __restrict__ part, int parts, const float* __restrict__ at_y,
+                                                     const int32_t* __restrict__ yc, const int32_t* __restrict__ rows, float* __restrict__ lse, float* __restrict__ rowloss) {
+  const int lane = threadIdx.x & 63;
+  const int64_t j = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (j >= n[0]) return;
+  const float l = ce_join(part, j, parts, lane);
   if (lane == 0) {
-    const float l = base + logf(sum);
     lse[j] = l;
-    loss[j] = yc[j] >= 0 ? l - at_y[j] : __uint_as_float(0x7fc00000u);  // a class outside [0, V) cannot raise an error from here: its loss is NaN
+    rowloss[rows ? rows[j] : j] = ce_row_loss(l, at_y, yc, j);
   }
 }
 
-// reduction 0: loss[t] for every token (0 where ignored); 1: mean over the tokens that count (0 where none does); 2: sum
-__global__ __launch_bounds__(1024) void ce_loss_kernel(const int32_t* __restrict__ n, const float* __restrict__ rowloss, const int32_t* __restrict__ pos, int64_t T,
-                                                       int reduction, float* __restrict__ loss) {
-  if (reduction == 0) {
-    const int64_t t = (int64_t)blockIdx.x * 1024 + threadIdx.x;
-    if (t < T) loss[t] = pos[t] >= 0 ? rowloss[pos[t]] : 0.f;
-    return;
-  }
+// Mean over the tokens that count (0 where none does) or sum, one workgroup.  JOIN: few tokens, whose lse it finds on the way; otherwise their losses are there.
+template <bool JOIN>
+__global__ __launch_bounds__(1024) void ce_loss_kernel(const int32_t* __restrict__ n, const float2* __restrict__ part, int parts, const float* __restrict__ at_y,
+                                                       const int32_t* __restrict__ yc, const float* __restrict__ rowloss, int reduction, float* __restrict__ lse, float* __restrict__ loss) {
   __shared__ double s[16];
+  const int N = n[0], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   double v = 0.0;
-  for (int j = threadIdx.x; j < n[0]; j += 1024) v += (double)rowloss[j];
+  if (JOIN) {
+    for (int j = wave; j < N; j += 16) {
+      const float l = ce_join(part, j, parts, lane);
+      if (lane == 0) {
+        lse[j] = l;
+        v += (double)ce_row_loss(l, at_y, yc, j);
+      }
+    }
+  } else {
+    for (int j = threadIdx.x; j < N; j += 1024) v += (double)rowloss[j];
+  }
   v = ceeg_wave_sum_d(v);
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+  if (lane == 0) s[wave] = v;
   __syncthreads();
   if (threadIdx.x == 0) {
     v = 0.0;
     for (int k = 0; k < 16; ++k) v += s[k];
-    loss[0] = (float)(reduction == 1 ? v / (n[0] > 0 ? n[0] : 1) : v);
+    loss[0] = (float)(reduction == 1 ? v / (N > 0 ? N : 1) : v);
   }
 }
 
-// scale[0] = s, r[j]: what comes back for token j is s r_j.  Mean and sum: r = 1, so that rounding r (p - [v = y]) to bf16 does not round the common factor too.
-__global__ __launch_bounds__(1024) void ce_scale_kernel(const int32_t* __restrict__ n, const int32_t* __restrict__ rows, const int32_t* __restrict__ yc,
-                                                        const float* __restrict__ g, int reduction, float* __restrict__ scale, float* __restrict__ r) {
+// What comes back for token j is s r_j.  Mean and sum: r = 1, so that rounding r (p - [v = y]) to bf16 does not round the common factor too.
+struct CeScale {
+  const float* g;
+  int reduction;
+  const float *top, *r;  // no reduction: s = the largest |g|, r_j = g_j / s
+  __device__ __forceinline__ float s(int N) const { return reduction == 0 ? top[0] : reduction == 1 ? g[0] / (float)(N > 0 ? N : 1) : g[0]; }
+  __device__ __forceinline__ float row(int j, int y) const { return y < 0 ? __uint_as_float(0x7fc00000u) : reduction == 0 ? r[j] : 1.f; }
+};
+__global__ __launch_bounds__(1024) void ce_scale_kernel(const int32_t* __restrict__ n, const int32_t* __restrict__ rows, const float* __restrict__ g, float* __restrict__ scale,
+                                                        float* __restrict__ r) {
   __shared__ float s[16];
   const int N = n[0];
-  float top = 1.f;
-  if (reduction == 0) {
-    top = 0.f;
-    for (int j = threadIdx.x; j < N; j += 1024) top = fmaxf(top, fabsf(g[rows[j]]));
+  float top = 0.f;
+  for (int j = threadIdx.x; j < N; j += 1024) top = fmaxf(top, fabsf(g[rows[j]]));
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = top;
-    __syncthreads();
-    for (int k = 0; k < 16; ++k) top = fmaxf(top, s[k]);
-  }
-  for (int j = threadIdx.x; j < N; j += 1024) {
-    float v = reduction == 0 ? (top > 0.f ? g[rows[j]] / top : g[rows[j]]) : 1.f;
-    if (yc[j] < 0) v = __uint_as_float(0x7fc00000u);
-    r[j] = v;
-  }
-  if (threadIdx.x == 0) scale[0] = reduction == 0 ? top : reduction == 1 ? g[0] / (float)(N > 0 ? N : 1) : g[0];
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = top;
+  __syncthreads();
+  for (int k = 0; k < 16; ++k) top = fmaxf(top, s[k]);
+  for (int j = threadIdx.x; j < N; j += 1024) r[j] = top > 0.f ? g[rows[j]] / top : g[rows[j]];
+  if (threadIdx.x == 0) scale[0] = top;
 }
 
 // dl of one piece of the vocabulary, [P][T][ldv]; columns behind the piece and the rows up to the next multiple of PAD are zero
 template <class G, int PL, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(G::THREADS, 1) void ce_dlogits_kernel(CeMat W, CeMat h, const int32_t* __restrict__ n, const int32_t* __restrict__ yc, const float* __restrict__ lse,
-                                                                const float* __restrict__ r, int v0, int ldv, int64_t plane, int K, unsigned short* __restrict__ dl) {
+                                                                CeScale scale, int v0, int ldv, int64_t plane, int K, unsigned short* __restrict__ dl) {
   __shared__ __align__(16) unsigned short lds[G::LDS];
   const int N = n[0], Vc = W.r_end, tiles_m = (Vc + BM - 1) / BM, tiles_n = (N + BN - 1) / BN;
   const int id = ce_xcd(blockIdx.x, tiles_m * tiles_n);
@@ -548,8 +609,8 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_dlogits_kernel(CeMat W, CeMa
 #pragma unroll
   for (int j = 0; j < G::NT; ++j) {
     const int t = n0 + (wn * G::NT + j) * 16 + (lane & 15);
-    const int y = t < N ? yc[t] - v0 - vb : -1;
-    const float l = t < N ? lse[t] : 0.f, rt = t < N ? r[t] : 0.f;
+    const int class_t = t < N ? yc[t] : -1, y = class_t - v0 - vb;
+    const float l = t < N ? lse[t] : 0.f, rt = t < N ? scale.row(t, class_t) : 0.f;
 #pragma unroll
     for (int i = 0; i < G::MT; ++i)
 #pragma unroll
@@ -640,7 +701,7 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_slots_kernel(CeMat A, CeMat 
 
 // dW = s dl^T h of one piece, the whole sum in one workgroup
 template <class G, bool F32, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(G::THREADS, 1) void ce_dw_kernel(CeMat h, CeMat dl, const int32_t* __restrict__ n, const float* __restrict__ scale, int H, int Vc,
+__global__ __launch_bounds__(G::THREADS, 1) void ce_dw_kernel(CeMat h, CeMat dl, const int32_t* __restrict__ n, CeScale scale, int H, int Vc,
                                                            void* __restrict__ dw) {
   __shared__ __align__(16) unsigned short lds[G::LDS];
   const int tiles_m = (H + BM - 1) / BM, id = ce_xcd(blockIdx.x, gridDim.x);
@@ -648,7 +709,7 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_dw_kernel(CeMat h, CeMat dl,
   G g;
   if (K > 0) g.run(h, dl, m0, n0, 0, K, lds);
   else g.clear();
-  const float s = K == 0 ? 0.f : scale[0];  // no token counts: the empty sum is zero whatever comes back
+  const float s = K == 0 ? 0.f : scale.s(n[0]);  // no token counts: the empty sum is zero whatever comes back
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN, q = lane >> 4;
 #pragma unroll
   for (int j = 0; j < G::NT; ++j) {
@@ -665,23 +726,23 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_dw_kernel(CeMat h, CeMat dl,
 
 // the slots of dW joined
 template <bool F32>
-__global__ __launch_bounds__(256) void ce_dw_join_kernel(const float* __restrict__ part, int slots, const int32_t* __restrict__ n, const float* __restrict__ scale, int64_t count,
+__global__ __launch_bounds__(256) void ce_dw_join_kernel(const float* __restrict__ part, int slots, const int32_t* __restrict__ n, CeScale scale, int64_t count,
                                                          void* __restrict__ dw) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= count) return;
   float x = 0.f;
   for (int k = 0; k < slots; ++k) x += part[k * count + i];
-  x = n[0] == 0 ? 0.f : x * scale[0];
+  x = n[0] == 0 ? 0.f : x * scale.s(n[0]);
   if (F32) static_cast<float*>(dw)[i] = x;
   else static_cast<unsigned short*>(dw)[i] = ceeg_f32_to_bf16(x);
 }
 
 template <bool F32>
-__global__ __launch_bounds__(256) void ce_dh_join_kernel(const float* __restrict__ part, int slots, const int32_t* __restrict__ pos, const float* __restrict__ scale, int64_t T,
+__global__ __launch_bounds__(256) void ce_dh_join_kernel(const float* __restrict__ part, int slots, const int32_t* __restrict__ n, const int32_t* __restrict__ pos, CeScale scale, int64_t T,
                                                          int H, void* __restrict__ dh) {
   const int64_t t = blockIdx.x;
   const int j = pos[t];
-  const float s = scale[0];
+  const float s = scale.s(n[0]);
   for (int c = threadIdx.x; c < H; c += 256) {
     float x = 0.f;
     if (j >= 0) {
@@ -761,23 +822,22 @@ int ce_check(const void* h, int64_t ldh, const void* W, int64_t ldw, int64_t T, 
   return CEEG_OK;
 }
 
+size_t ce_packed_bytes(const CePlan& c) { return ceeg_ws_part((size_t)c.P * c.Tp * c.Kp, 2); }
 size_t ce_fwd_bytes(int64_t T, int64_t H, int64_t V, int dtype) {
   const CePlan c = ce_plan(T, H, V, dtype, false);
   const size_t parts = (size_t)(V + TMIN - 1) / TMIN;
-  return ceeg_ws_part((size_t)c.P * c.Tp * c.Kp, 2) + (c.direct ? 0 : ceeg_ws_part((size_t)c.P * c.piece * c.Kp, 2)) + ceeg_ws_part((size_t)T * parts, 8) +
-         2 * ceeg_ws_part(T, 4);
+  return (c.direct ? 0 : ceeg_ws_part((size_t)c.P * c.piece * c.Kp, 2)) + ceeg_ws_part((size_t)T * parts, 8) + 2 * ceeg_ws_part(T, 4);
 }
 size_t ce_bwd_bytes(int64_t T, int64_t H, int64_t V, int dtype) {
   const CePlan c = ce_plan(T, H, V, dtype, true);
-  return ceeg_ws_part((size_t)c.P * c.Tp * c.Kp, 2) + (c.direct ? ceeg_ws_part((size_t)PAD * c.Kp, 2) : ceeg_ws_part((size_t)c.P * c.piece * c.Kp, 2)) + ceeg_ws_part((size_t)c.P * c.Tp * c.ldv, 2) +
+  return (c.direct ? ceeg_ws_part((size_t)PAD * c.Kp, 2) : ceeg_ws_part((size_t)c.P * c.piece * c.Kp, 2)) + ceeg_ws_part((size_t)c.P * c.Tp * c.ldv, 2) +
          ceeg_ws_part((size_t)c.dh_slots * T * H, 4) + (c.dw_slots > 1 ? ceeg_ws_part((size_t)c.dw_slots * c.piece * H, 4) : 0) + ceeg_ws_part(1, 4) + ceeg_ws_part(T, 4);
 }
 
-void ce_pack(int dtype, const void* src, int64_t ld, const int32_t* rows, const int32_t* count, int64_t R, int64_t C, int64_t Cp, bool zeros, unsigned short* out, int64_t plane,
-             hipStream_t st) {
+void ce_pack(int dtype, const void* src, int64_t ld, int64_t R, int64_t C, int64_t Cp, bool zeros, unsigned short* out, int64_t plane, hipStream_t st) {
   const unsigned grid = (unsigned)(((zeros ? up(R, PAD) : R) * (Cp / 8) + 255) / 256);
-  if (dtype == CEEG_F32) ce_pack_kernel<true><<<grid, 256, 0, st>>>(src, ld, rows, count, R, (int)C, (int)Cp, zeros, out, plane);
-  else ce_pack_kernel<false><<<grid, 256, 0, st>>>(src, ld, rows, count, R, (int)C, (int)Cp, zeros, out, plane);
+  if (dtype == CEEG_F32) ce_pack_kernel<true><<<grid, 256, 0, st>>>(src, ld, R, (int)C, (int)Cp, zeros, out, plane);
+  else ce_pack_kernel<false><<<grid, 256, 0, st>>>(src, ld, R, (int)C, (int)Cp, zeros, out, plane);
 }
 inline const void* ce_at(const void* p, int64_t n, int dtype) { return static_cast<const char*>(p) + n * (dtype == CEEG_F32 ? 4 : 2); }
 
@@ -805,16 +865,21 @@ extern "C" size_t ceeg_linear_ce_bwd_ws_bytes(int64_t T, int64_t H, int64_t V, i
   return ce_sizes_ok(T, H, V) ? ce_bwd_bytes(T, H, V, dtype) : 0;
 }
 
+extern "C" size_t ceeg_linear_ce_packed_bytes(int64_t T, int64_t H, int dtype) {
+  return ce_sizes_ok(T, H, 1) ? ce_packed_bytes(ce_plan(T, H, 1, dtype, false)) : 0;
+}
+
 extern "C" int ceeg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, const int64_t* y, int64_t T, int64_t H, int64_t V, int dtype, int64_t ignore_index,
-                                  int reduction, float* loss, float* lse, int32_t* tokens, void* ws, size_t ws_bytes, void* stream) {
+                                  int reduction, float* loss, float* lse, int32_t* tokens, void* packed, void* ws, size_t ws_bytes, void* stream) {
   const int rc = ce_check(h, ldh, W, ldw, T, H, V, dtype);
   if (rc) return rc;
   if (!y || !ceeg_aligned(y, 8) || !loss || !lse || !tokens || reduction < 0 || reduction > 2) return CEEG_EINVAL;
+  if (!packed || !ceeg_aligned(packed, 256)) return CEEG_EINVAL;
   if (!ws || !ceeg_aligned(ws, 256) || ws_bytes < ce_fwd_bytes(T, H, V, dtype)) return CEEG_EWORKSPACE;
   const CePlan c = ce_plan(T, H, V, dtype, false);
   const int parts = (int)((V + c.e_logits - 1) / c.e_logits);
   CeegWs w(ws, ws_bytes);
-  unsigned short* hc = w.take<unsigned short>((size_t)c.P * c.Tp * c.Kp);
+  unsigned short* const hc = static_cast<unsigned short*>(packed);
   unsigned short* wc = c.direct ? nullptr : w.take<unsigned short>((size_t)c.P * c.piece * c.Kp);
   float2* part = w.take<float2>((size_t)T * parts);
   float* at_y = w.take<float>(T);
@@ -822,9 +887,21 @@ extern "C" int ceeg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int
   if (!w.ok) return CEEG_EWORKSPACE;
   int32_t *n = tokens, *rows = tokens + 1, *pos = rows + T, *yc = pos + T;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  ce_tokens_kernel<<<1, 1024, 0, st>>>(y, T, V, ignore_index, n, rows, pos, yc);
-  CEEG_CHECK_LAUNCH();
-  ce_pack(dtype, h, ldh, rows, n, T, H, c.Kp, false, hc, c.Tp * c.Kp, st);
+  const CeTokens tk{y, T, V, ignore_index, n, rows, pos, yc, reduction == 0 ? loss : nullptr};
+  const bool scan = T <= CE_SCAN;
+  if (!scan) {
+    ce_tokens_kernel<<<1, 1024, 0, st>>>(tk);
+    CEEG_CHECK_LAUNCH();
+  }
+  const int each = c.Kp / 8 >= 128 ? 8 : (int)(1024 / (c.Kp / 8));  // about 1024 pieces of 16 bytes a workgroup
+  const unsigned grid = (unsigned)((T + each - 1) / each);
+  if (dtype == CEEG_F32) {
+    if (scan) ce_prepare_kernel<true, true><<<grid, 256, 0, st>>>(tk, h, ldh, (int)H, (int)c.Kp, each, hc, c.Tp * c.Kp);
+    else ce_prepare_kernel<true, false><<<grid, 256, 0, st>>>(tk, h, ldh, (int)H, (int)c.Kp, each, hc, c.Tp * c.Kp);
+  } else {
+    if (scan) ce_prepare_kernel<false, true><<<grid, 256, 0, st>>>(tk, h, ldh, (int)H, (int)c.Kp, each, hc, c.Tp * c.Kp);
+    else ce_prepare_kernel<false, false><<<grid, 256, 0, st>>>(tk, h, ldh, (int)H, (int)c.Kp, each, hc, c.Tp * c.Kp);
+  }
   CEEG_CHECK_LAUNCH();
   const int e = c.e_logits, tiles_n = (int)((T + e - 1) / e);
   const CeMat Bm{hc, c.Kp, c.Tp * c.Kp, 0, nullptr, INT_MAX};
@@ -832,7 +909,7 @@ extern "C" int ceeg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int
     const int64_t v0 = p * c.piece, Vc = V - v0 < c.piece ? V - v0 : c.piece;
     CeMat A{static_cast<const unsigned short*>(W) + v0 * ldw, ldw, 0, (int)Vc, nullptr, INT_MAX};
     if (!c.direct) {
-      ce_pack(dtype, ce_at(W, v0 * ldw, dtype), ldw, nullptr, nullptr, Vc, H, c.Kp, false, wc, c.piece * c.Kp, st);
+      ce_pack(dtype, ce_at(W, v0 * ldw, dtype), ldw, Vc, H, c.Kp, false, wc, c.piece * c.Kp, st);
       CEEG_CHECK_LAUNCH();
       A = CeMat{wc, c.Kp, c.piece * c.Kp, (int)Vc, nullptr, INT_MAX};
     }
@@ -843,56 +920,66 @@ extern "C" int ceeg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int
 #undef CE_CALL
     CEEG_CHECK_LAUNCH();
   }
-  ce_lse_kernel<<<(unsigned)((T + 3) / 4), 256, 0, st>>>(n, part, parts, at_y, yc, lse, rowloss);
+  // few tokens and pieces: one workgroup finds lse and loss (a launch less); more: a wave a token first
+  if (reduction != 0 && T * parts <= 32768) {
+    ce_loss_kernel<true><<<1, 1024, 0, st>>>(n, part, parts, at_y, yc, nullptr, reduction, lse, loss);
+    CEEG_CHECK_LAUNCH();
+    return CEEG_OK;
+  }
+  ce_lse_kernel<<<(unsigned)((T + 3) / 4), 256, 0, st>>>(n, part, parts, at_y, yc, reduction == 0 ? rows : nullptr, lse, reduction == 0 ? loss : rowloss);
   CEEG_CHECK_LAUNCH();
-  ce_loss_kernel<<<reduction == 0 ? (unsigned)((T + 1023) / 1024) : 1u, 1024, 0, st>>>(n, rowloss, pos, T, reduction, loss);
-  CEEG_CHECK_LAUNCH();
+  if (reduction != 0) {
+    ce_loss_kernel<false><<<1, 1024, 0, st>>>(n, nullptr, 0, nullptr, nullptr, rowloss, reduction, nullptr, loss);
+    CEEG_CHECK_LAUNCH();
+  }
   return CEEG_OK;
 }
 
-extern "C" int ceeg_linear_ce_bwd(const void* h, int64_t ldh, const void* W, int64_t ldw, int64_t T, int64_t H, int64_t V, int dtype, int reduction, const float* g,
-                                  const float* lse, const int32_t* tokens, void* dh, void* dw, void* ws, size_t ws_bytes, void* stream) {
-  const int rc = ce_check(h, ldh, W, ldw, T, H, V, dtype);
+extern "C" int ceeg_linear_ce_bwd(const void* packed, const void* W, int64_t ldw, int64_t T, int64_t H, int64_t V, int dtype, int reduction, const float* g, const float* lse,
+                                  const int32_t* tokens, void* dh, void* dw, void* ws, size_t ws_bytes, void* stream) {
+  const int rc = ce_check(packed, H, W, ldw, T, H, V, dtype);
   if (rc) return rc;
+  if (!ceeg_aligned(packed, 256)) return CEEG_EINVAL;
   if (!g || !lse || !tokens || (!dh && !dw) || reduction < 0 || reduction > 2) return CEEG_EINVAL;
   if (!ws || !ceeg_aligned(ws, 256) || ws_bytes < ce_bwd_bytes(T, H, V, dtype)) return CEEG_EWORKSPACE;
   const CePlan c = ce_plan(T, H, V, dtype, true);
   CeegWs w(ws, ws_bytes);
-  unsigned short* hc = w.take<unsigned short>((size_t)c.P * c.Tp * c.Kp);
+  const unsigned short* const hc = static_cast<const unsigned short*>(packed);
   unsigned short* wc = c.direct ? nullptr : w.take<unsigned short>((size_t)c.P * c.piece * c.Kp);
   unsigned short* tail = c.direct ? w.take<unsigned short>((size_t)PAD * c.Kp) : nullptr;
   unsigned short* dl = w.take<unsigned short>((size_t)c.P * c.Tp * c.ldv);
   float* dh_slots = w.take<float>((size_t)c.dh_slots * T * H);
   float* dw_slots = c.dw_slots > 1 ? w.take<float>((size_t)c.dw_slots * c.piece * H) : nullptr;
-  float* scale = w.take<float>(1);
+  float* top = w.take<float>(1);
   float* r = w.take<float>(T);
   if (!w.ok) return CEEG_EWORKSPACE;
   const int32_t *n = tokens, *rows = tokens + 1, *pos = rows + T, *yc = pos + T;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  ce_scale_kernel<<<1, 1024, 0, st>>>(n, rows, yc, g, reduction, scale, r);
-  CEEG_CHECK_LAUNCH();
-  ce_pack(dtype, h, ldh, rows, n, T, H, c.Kp, true, hc, c.Tp * c.Kp, st);
-  CEEG_CHECK_LAUNCH();
+  const CeScale scale{g, reduction, top, r};
+  if (reduction == 0) {
+    ce_scale_kernel<<<1, 1024, 0, st>>>(n, rows, g, top, r);
+    CEEG_CHECK_LAUNCH();
+  }
   const auto tiles = [](int64_t x, int e) { return (int)((x + e - 1) / e); };
   const CeMat hm{hc, c.Kp, c.Tp * c.Kp, 0, nullptr, INT_MAX}, hk{hc, c.Kp, c.Tp * c.Kp, (int)c.Kp, nullptr, INT_MAX};
   for (int p = 0; p < c.pieces; ++p) {
     const int64_t v0 = p * c.piece, Vc = V - v0 < c.piece ? V - v0 : c.piece, ldv = up(Vc, PAD), plane = c.Tp * c.ldv;
     CeMat A{static_cast<const unsigned short*>(W) + v0 * ldw, ldw, 0, (int)Vc, nullptr, INT_MAX};
     if (!c.direct) {
-      ce_pack(dtype, ce_at(W, v0 * ldw, dtype), ldw, nullptr, nullptr, Vc, H, c.Kp, true, wc, c.piece * c.Kp, st);
+      ce_pack(dtype, ce_at(W, v0 * ldw, dtype), ldw, Vc, H, c.Kp, true, wc, c.piece * c.Kp, st);
       CEEG_CHECK_LAUNCH();
       A = CeMat{wc, c.Kp, c.piece * c.Kp, (int)Vc, nullptr, INT_MAX};
     }
     const int tiles_t = tiles(T, c.e_logits), tiles_v = tiles(ldv, c.e_logits);
 #define CE_CALL(PL, E, WM, WN, TILE)                                                                                                                                     \
-  ce_dlogits_kernel<CE_TILE_OF(TILE), PL, E, E, WM, WN><<<tiles_v * tiles_t, WM * WN * 64, 0, st>>>(A, hm, n, yc, lse, r, (int)v0, (int)ldv, plane, (int)c.Kp, dl)
+  ce_dlogits_kernel<CE_TILE_OF(TILE), PL, E, E, WM, WN><<<tiles_v * tiles_t, WM * WN * 64, 0, st>>>(A, hm, n, yc, lse, scale, (int)v0, (int)ldv, plane, (int)c.Kp, dl)
     CE_TILES(c.P, c.e_logits, false, false, CE_CALL);
 #undef CE_CALL
     CEEG_CHECK_LAUNCH();
     if (dh) {
       const CeMat Wk{A.p, A.ld, A.plane, (int)c.Kp, tail, c.direct && Vc % PAD ? (int)(Vc / PAD * PAD) : INT_MAX}, dlm{dl, ldv, plane, 0, nullptr, INT_MAX};
       if (Wk.k_tail != INT_MAX) {
-        ce_pack(dtype, ce_at(W, (v0 + Wk.k_tail) * ldw, dtype), ldw, nullptr, nullptr, Vc % PAD, H, c.Kp, true, tail, 0, st);
+        ce_pack(dtype, ce_at(W, (v0 + Wk.k_tail) * ldw, dtype), ldw, Vc % PAD, H, c.Kp, true, tail, 0, st);
         CEEG_CHECK_LAUNCH();
       }
       const int all = tiles(H, c.e_dh) * tiles(T, c.e_dh);
@@ -924,8 +1011,8 @@ extern "C" int ceeg_linear_ce_bwd(const void* h, int64_t ldh, const void* W, int
     }
   }
   if (dh) {
-    if (dtype == CEEG_F32) ce_dh_join_kernel<true><<<(unsigned)T, 256, 0, st>>>(dh_slots, c.dh_slots, pos, scale, T, (int)H, dh);
-    else ce_dh_join_kernel<false><<<(unsigned)T, 256, 0, st>>>(dh_slots, c.dh_slots, pos, scale, T, (int)H, dh);
+    if (dtype == CEEG_F32) ce_dh_join_kernel<true><<<(unsigned)T, 256, 0, st>>>(dh_slots, c.dh_slots, n, pos, scale, T, (int)H, dh);
+    else ce_dh_join_kernel<false><<<(unsigned)T, 256, 0, st>>>(dh_slots, c.dh_slots, n, pos, scale, T, (int)H, dh);
     CEEG_CHECK_LAUNCH();
   }
   return CEEG_OK;

@@ -35,34 +35,35 @@ class _LinearCrossEntropy(torch.autograd.Function):
             weight = weight.clone(memory_format=torch.contiguous_format)
         target = target.contiguous()
         ldh, ldw = max(hidden.stride(0), H), H if weight.is_contiguous() else weight.stride(0)
-        with torch.cuda.device(dev):
+        with _lib.on(dev):
             loss = torch.empty(T if reduction == 0 else 1, dtype=torch.float32, device=dev)
             lse = torch.empty(T, dtype=torch.float32, device=dev)
             tokens = torch.empty(3 * T + 1, dtype=torch.int32, device=dev)
+            packed = _lib.workspace(L.ceeg_linear_ce_packed_bytes(T, H, dtype), dev)
             ws = _lib.workspace(L.ceeg_linear_ce_fwd_ws_bytes(T, H, V, dtype), dev)
             with _lib.timed("linear_ce_fwd"):
                 _lib.check(L.ceeg_linear_ce_fwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, target.data_ptr(), T, H, V, dtype, ignore_index, reduction,
-                                                loss.data_ptr(), lse.data_ptr(), tokens.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream()),
+                                                loss.data_ptr(), lse.data_ptr(), tokens.data_ptr(), packed.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream()),
                            "ceeg_linear_ce_fwd")
-        ctx.save_for_backward(hidden, weight, lse, tokens)
-        ctx.sizes = T, H, V, ldh, ldw, dtype, reduction
+        ctx.save_for_backward(packed, weight, lse, tokens)
+        ctx.sizes = T, H, V, ldw, dtype, reduction, hidden.dtype
         return loss if reduction == 0 else loss[0]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        hidden, weight, lse, tokens = ctx.saved_tensors
-        T, H, V, ldh, ldw, dtype, reduction = ctx.sizes
+        packed, weight, lse, tokens = ctx.saved_tensors
+        T, H, V, ldw, dtype, reduction, hidden_dtype = ctx.sizes
         L = _lib.lib()
-        dev = hidden.device
+        dev = weight.device
         need_h, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        with torch.cuda.device(dev):
+        with _lib.on(dev):
             g = g.to(torch.float32).contiguous()
-            dh = torch.empty(T, H, dtype=hidden.dtype, device=dev) if need_h else None
+            dh = torch.empty(T, H, dtype=hidden_dtype, device=dev) if need_h else None
             dw = torch.empty(V, H, dtype=weight.dtype, device=dev) if need_w else None
             ws = _lib.workspace(L.ceeg_linear_ce_bwd_ws_bytes(T, H, V, dtype), dev)
             with _lib.timed("linear_ce_bwd"):
-                _lib.check(L.ceeg_linear_ce_bwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, T, H, V, dtype, reduction, g.data_ptr(), lse.data_ptr(),
+                _lib.check(L.ceeg_linear_ce_bwd(packed.data_ptr(), weight.data_ptr(), ldw, T, H, V, dtype, reduction, g.data_ptr(), lse.data_ptr(),
                                                 tokens.data_ptr(), _lib.ptr(dh), _lib.ptr(dw), ws.data_ptr(), ws.numel(), _lib.stream()),
                            "ceeg_linear_ce_bwd")
         return dh, dw, None, None, None
@@ -108,7 +109,7 @@ class _Balance(torch.autograd.Function):
         indices = indices.contiguous()
         mask = None if mask is None else mask.contiguous()
         ld = max(scores.stride(0), E)
-        with torch.cuda.device(dev):
+        with _lib.on(dev):
             loss = torch.empty(1, dtype=torch.float32, device=dev)
             counts = torch.empty(E, dtype=torch.int64, device=dev)
             stats = torch.empty(E + 1, dtype=torch.float32, device=dev)
@@ -128,7 +129,7 @@ class _Balance(torch.autograd.Function):
         scores, mask, stats = ctx.saved_tensors
         T, E, ld, dtype = ctx.sizes
         dev = scores.device
-        with torch.cuda.device(dev):
+        with _lib.on(dev):
             g = g.to(torch.float32).contiguous()
             ds = torch.empty(T, E, dtype=scores.dtype, device=dev)
             with _lib.timed("balance_bwd"):

@@ -82,7 +82,7 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9,
     step_t, lr_t = _scalar(step, "step", dev), _scalar(lr, "lr", dev)
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and (step_t is not None or step >= 1)):
         raise ValueError(f"betas in [0, 1), eps >= 0 and step >= 1 expected, got {betas}, {eps} and {step}")
-    with torch.cuda.device(dev):
+    with _lib.on(dev):
         _lib.check(_lib.lib().ceeg_adamw_step(
             n, (C.c_int64 * n)(*sizes), _pointers(params), _pointers(grads), _pointers(ms), _pointers(vs),
             _pointers(m_scales) if held else None, _pointers(v_scales) if held else None, _DTYPES[dtype], 8 if held else 32,

@@ -582,17 +582,19 @@ int ceeg_neg_sample_uniform_filtered(const int32_t* rowptr, const int32_t* col, 
  * Tokens with y == ignore_index take no part: loss 0, dh row 0, whatever their row of h holds (also NaN).  A class outside [0, V) that is not
  * ignore_index is not an error code (that would need a host read): its loss, and every gradient that it reaches, is NaN.
  * reduction 0: loss [T]; 1: mean over the tokens that count (0 where none does) -> loss [1]; 2: sum -> loss [1].
- * lse [T] fp32 and tokens [3 T + 1] int32 are written by the forward for the backward: how many tokens count, which, their place and class.
+ * lse [T] fp32, tokens [3 T + 1] int32 (how many tokens count, which, their place and class) and packed (ceeg_linear_ce_packed_bytes(), 256-byte aligned: their
+ * rows of h as the products read them) are written by the forward for the backward.
  * g: what comes back for loss (fp32, [T] or [1]).  dh [T, H] and dW [V, H] contiguous, either may be NULL.
  * Limits: T <= 2^22, H <= 2^15, V <= 2^28, ldw <= 2^22; bf16 with H a multiple of 64 reads W in place: 16-byte aligned, ldw = H.
  * The backward's workspace holds dl for a piece of the vocabulary; pieces are chosen so that they take about 1 GiB at most together.
  * ----------------------------------------------------------------------------------------------*/
 size_t ceeg_linear_ce_fwd_ws_bytes(int64_t T, int64_t H, int64_t V, int dtype);
 size_t ceeg_linear_ce_bwd_ws_bytes(int64_t T, int64_t H, int64_t V, int dtype);
-int ceeg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, const int64_t* y, int64_t T, int64_t H, int64_t V, int dtype,
-                       int64_t ignore_index, int reduction, float* loss, float* lse, int32_t* tokens, void* ws, size_t ws_bytes, void* stream);
-int ceeg_linear_ce_bwd(const void* h, int64_t ldh, const void* W, int64_t ldw, int64_t T, int64_t H, int64_t V, int dtype, int reduction,
-                       const float* g, const float* lse, const int32_t* tokens, void* dh, void* dw, void* ws, size_t ws_bytes, void* stream);
+size_t ceeg_linear_ce_packed_bytes(int64_t T, int64_t H, int dtype);
+int ceeg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, const int64_t* y, int64_t T, int64_t H, int64_t V, int dtype, int64_t ignore_index,
+                       int reduction, float* loss, float* lse, int32_t* tokens, void* packed, void* ws, size_t ws_bytes, void* stream);
+int ceeg_linear_ce_bwd(const void* packed, const void* W, int64_t ldw, int64_t T, int64_t H, int64_t V, int dtype, int reduction, const float* g,
+                       const float* lse, const int32_t* tokens, void* dh, void* dw, void* ws, size_t ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Balance loss over an assignment of rows to codes (the quantiser's min_encoding_indices, scripts/quantizer.py:48) or experts, with

@@ -31,20 +31,20 @@ def test_linear_cross_entropy_refuses():
 
 def test_linear_cross_entropy_entries_refuse():
     L = _lib()
-    fwd = [P, 64, P, 64, P, 10, 64, 100, 1, -100, 1, P, P, P, P, L.ceeg_linear_ce_fwd_ws_bytes(10, 64, 100, 1), None]
-    bwd = [P, 64, P, 64, 10, 64, 100, 1, 1, P, P, P, P, P, P, L.ceeg_linear_ce_bwd_ws_bytes(10, 64, 100, 1), None]
+    fwd = [P, 64, P, 64, P, 10, 64, 100, 1, -100, 1, P, P, P, P, P, L.ceeg_linear_ce_fwd_ws_bytes(10, 64, 100, 1), None]
+    bwd = [P, P, 64, 10, 64, 100, 1, 1, P, P, P, P, P, P, L.ceeg_linear_ce_bwd_ws_bytes(10, 64, 100, 1), None]
     for entry, good, cases in (
-            (L.ceeg_linear_ce_fwd, fwd, [(0, None, -1), (2, None, -1), (4, None, -1), (11, None, -1), (12, None, -1), (13, None, -1), (14, None, -3), (14, P + 1, -3),
-                                         (15, 16, -3), (5, 0, -1), (6, 0, -1), (7, 0, -1), (1, 63, -1), (3, 63, -1), (8, 2, -2), (10, 3, -1), (10, -1, -1),
-                                         (5, (1 << 22) + 1, -2), (7, (1 << 28) + 1, -2), (3, 1 << 23, -2), (2, P + 2, -1), (3, 72, -1), (4, P + 4, -1)]),
-            (L.ceeg_linear_ce_bwd, bwd, [(0, None, -1), (2, None, -1), (9, None, -1), (10, None, -1), (11, None, -1), (14, None, -3), (15, 16, -3), (7, 5, -2), (8, 3, -1),
-                                         (4, 0, -1), (2, P + 8, -1)])):
+            (L.ceeg_linear_ce_fwd, fwd, [(0, None, -1), (2, None, -1), (4, None, -1), (11, None, -1), (12, None, -1), (13, None, -1), (14, None, -1), (14, P + 16, -1),
+                                         (15, None, -3), (15, P + 1, -3), (16, 16, -3), (5, 0, -1), (6, 0, -1), (7, 0, -1), (1, 63, -1), (3, 63, -1), (8, 2, -2), (10, 3, -1),
+                                         (10, -1, -1), (5, (1 << 22) + 1, -2), (7, (1 << 28) + 1, -2), (3, 1 << 23, -2), (2, P + 2, -1), (3, 72, -1), (4, P + 4, -1)]),
+            (L.ceeg_linear_ce_bwd, bwd, [(0, None, -1), (0, P + 16, -1), (1, None, -1), (8, None, -1), (9, None, -1), (10, None, -1), (13, None, -3), (14, 16, -3), (6, 5, -2),
+                                         (7, 3, -1), (3, 0, -1), (1, P + 8, -1), (2, 72, -1)])):
         for at, value, code in cases:
             args = list(good)
             args[at] = value
             assert entry(*args) == code, (entry.__name__, at, value)
     args = list(bwd)
-    args[12] = args[13] = None                        # neither gradient wanted
+    args[11] = args[12] = None                        # neither gradient wanted
     assert L.ceeg_linear_ce_bwd(*args) == -1
     for sizes in ((0, 8, 8, 0), (8, 0, 8, 0), (8, 8, 0, 0), (8, 1 << 16, 8, 0)):
         assert L.ceeg_linear_ce_fwd_ws_bytes(*sizes) == 0 and L.ceeg_linear_ce_bwd_ws_bytes(*sizes) == 0
