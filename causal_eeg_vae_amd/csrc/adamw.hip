@@ -101,39 +101,57 @@ __device__ __forceinline__ void aw_put_codes4(uint8_t* p, int64_t i, int64_t n, 
       if (i + k < n) p[i + k] = (uint8_t)(w >> (8 * k));
   }
 }
-// e4m3 (1 sign, 4 exponent bits with bias 7, 3 mantissa bits, no infinities, 0x7f NaN) -> fp32, exact
-__device__ __forceinline__ float aw_e4m3(uint32_t c) {
-  const uint32_t a = c & 0x7fu;
-  float x = a < 8u ? (float)a * 0x1p-9f : __uint_as_float((a << 20) + (120u << 23));
-  if (a == 0x7fu) x = __uint_as_float(0x7fc00000u);
-  return (c & 0x80u) ? -x : x;
-}
-__device__ __forceinline__ float aw_finite_abs(float x) {
-  const float a = fabsf(x);
-  return a <= 3.402823466e38f ? a : 0.f;  // infinities and NaN do not set a block's scale
-}
-__device__ __forceinline__ float aw_wave_max(float v) {
+// ceeg_philox with each 32 x 32 product as one 64-bit instruction
+__device__ __forceinline__ uint4 aw_philox(uint64_t seed, uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3) {
+  uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0; c1 = (uint32_t)b;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1; c3 = (uint32_t)a;
+    k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
 }
-// x / scale as an e4m3 number, rounded by the 16 random bits r so that the expectation of its magnitude (SECOND: of its square) is kept
+__device__ __forceinline__ bool aw_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+// the largest of 64 lanes' values >= 0, the same in every lane: six steps in registers
+__device__ __forceinline__ float aw_wave_max(float v) {
+  int x = __float_as_int(v);  // of values >= 0 the larger one has the larger bits
+#define AW_MAX(CTRL, ROWS) x = max(x, __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, true))
+  AW_MAX(0x111, 0xf);  // row_shr 1, 2, 4, 8: lane 15 of each row of 16
+  AW_MAX(0x112, 0xf);
+  AW_MAX(0x114, 0xf);
+  AW_MAX(0x118, 0xf);
+  AW_MAX(0x142, 0xa);  // row_bcast 15 into rows 1 and 3, row_bcast 31 into rows 2 and 3: lane 63
+  AW_MAX(0x143, 0xc);
+#undef AW_MAX
+  return __int_as_float(__builtin_amdgcn_readlane(x, 63));
+}
+// a / b, correctly rounded, from the (nearly) rounded reciprocal r of b: a quotient within a unit and one exact remainder
+__device__ __forceinline__ float aw_quotient(float a, float b, float r) {
+  const float q = a * r;
+  return __fmaf_rn(__fmaf_rn(-q, b, a), r, q);
+}
+// x / scale as an e4m3 number, rounded by the 16 random bits `rnd` so that the expectation of its magnitude (SECOND: of its square) is kept.  per_scale: 1 / scale,
+// 0 where the scale is.  Between the numbers L s and (L + 1) s (s: their distance, L < 16) the magnitude is (L + share) s, and
+//   (y^2 - low^2) / (high^2 - low^2) = share (2 L + share) / (2 L + 1).
 template <bool SECOND>
-__device__ __forceinline__ uint32_t aw_round(float x, float scale, uint32_t r) {
-  const uint32_t sign = (__float_as_uint(x) >> 24) & 0x80u;
-  if (!(fabsf(x) <= 3.402823466e38f)) return sign | 0x7fu;  // stays a NaN
-  if (scale == 0.f) return sign;
-  const float y = fminf(fabsf(x) / scale, AW_TOP);
+__device__ __forceinline__ uint32_t aw_round(float x, float scale, float per_scale, float rnd) {
+  const float a = fabsf(x), y = fminf(aw_quotient(a, scale, per_scale), AW_TOP);
   const uint32_t u = __float_as_uint(y);
   const bool small = y < 0x1p-6f;  // there the numbers are 2^-9 apart
-  uint32_t c = small ? (uint32_t)(y * 512.f) : (u >> 20) - (120u << 3);  // the number below
-  const float low = small ? (float)c * 0x1p-9f : __uint_as_float(u & 0xfff00000u);
-  const float step = small ? 0x1p-9f : __uint_as_float((u & 0x7f800000u) - (3u << 23));
-  float share = (y - low) * (small ? 512.f : __uint_as_float((257u << 23) - (u & 0x7f800000u)));  // (y - low) / step, exact
-  if (SECOND) share = share * (y + low) / (low + low + step);
-  if (share * 65536.f + (float)r >= 65536.f) ++c;
+  const float t = y * 512.f, below = floorf(t);
+  float share = small ? t - below : (float)(u & 0xfffffu) * 0x1p-20f;
+  uint32_t c = small ? (uint32_t)below : (u >> 20) - (120u << 3);
+  if (SECOND) {
+    const float l2 = small ? below + below : (float)(16u + 2u * (c & 7u)), d = l2 + 1.f;
+    const float r0 = __builtin_amdgcn_rcpf(d), r = __fmaf_rn(__fmaf_rn(-d, r0, 1.f), r0, r0);
+    share = aw_quotient(share * (l2 + share), d, r);
+  }
+  c += share * 65536.f + rnd >= 65536.f;
   if (SECOND && c == 0u && y > 0.f) c = 1u;
-  return sign | c;
+  if (!aw_finite(x)) c = 0x7fu;  // stays a NaN
+  return c | (__float_as_uint(x) >> 24 & 0x80u);
 }
 
 template <bool BF16, int BITS>
@@ -171,29 +189,32 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_kernel(AwList L, AwHyper h) 
 
   for (int64_t b0 = begin + (int64_t)wave * AW_BLOCK; b0 < end; b0 += AW_THREADS / 64 * AW_BLOCK) {
     const int64_t i = b0 + 4 * lane;
-    float pv[4], gv[4], mo[4], vo[4];
+    float pv[4], gv[4], mo[4], vo[4], root[4];
     aw_load4<BF16>(p, i, n, vec, pv);
     aw_load4<BF16>(g, i, n, vec, gv);
     if (BITS == 8) {
       const float sm = L.ms[lo][b0 / AW_BLOCK], sv = L.vs[lo][b0 / AW_BLOCK];
       const uint32_t cm = aw_codes4(static_cast<const uint8_t*>(m), i, n, svec), cv = aw_codes4(static_cast<const uint8_t*>(v), i, n, svec);
+      mo[0] = __builtin_amdgcn_cvt_f32_fp8(cm, 0); mo[1] = __builtin_amdgcn_cvt_f32_fp8(cm, 1);
+      mo[2] = __builtin_amdgcn_cvt_f32_fp8(cm, 2); mo[3] = __builtin_amdgcn_cvt_f32_fp8(cm, 3);
+      root[0] = __builtin_amdgcn_cvt_f32_fp8(cv, 0); root[1] = __builtin_amdgcn_cvt_f32_fp8(cv, 1);
+      root[2] = __builtin_amdgcn_cvt_f32_fp8(cv, 2); root[3] = __builtin_amdgcn_cvt_f32_fp8(cv, 3);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        mo[k] = aw_e4m3(cm >> (8 * k) & 0xffu) * sm;
-        const float u = aw_e4m3(cv >> (8 * k) & 0xffu) * sv;
+        const float u = root[k] * sv;
+        mo[k] *= sm;
         vo[k] = u * u;
       }
     } else {
       aw_load4<false>(m, i, n, svec, mo);
       aw_load4<false>(v, i, n, svec, vo);
     }
-    float root[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       mo[k] = h.b1 * mo[k] + h.omb1 * gv[k];
       vo[k] = h.b2 * vo[k] + h.omb2 * (gv[k] * gv[k]);
       root[k] = sqrtf(vo[k]);
-      pv[k] = pv[k] * decay - step_size * (mo[k] / (root[k] * inv_sqrt_c2 + h.eps));
+      pv[k] = pv[k] * decay - step_size * (mo[k] * __builtin_amdgcn_rcpf(root[k] * inv_sqrt_c2 + h.eps));
     }
     aw_store4<BF16>(p, i, n, vec, pv);
     if (BITS == 8) {
@@ -201,20 +222,21 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_kernel(AwList L, AwHyper h) 
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (i + k >= n) mo[k] = root[k] = 0.f;
-        tm = fmaxf(tm, aw_finite_abs(mo[k]));
-        tv = fmaxf(tv, aw_finite_abs(root[k]));
+        tm = fmaxf(tm, aw_finite(mo[k]) ? fabsf(mo[k]) : 0.f);  // infinities and NaN do not set a block's scale
+        tv = fmaxf(tv, aw_finite(root[k]) ? root[k] : 0.f);
       }
       tm = aw_wave_max(tm);
       tv = aw_wave_max(tv);
       const float sm = tm < AW_TINY ? 0.f : tm * AW_PER_TOP, sv = tv < AW_TINY ? 0.f : tv * AW_PER_TOP;
+      const float pm = sm > 0.f ? 1.f / sm : 0.f, pr = sv > 0.f ? 1.f / sv : 0.f;
       const uint64_t quad = (uint64_t)i >> 2;
-      const uint4 r = ceeg_philox(seed, (uint32_t)quad, (uint32_t)(quad >> 32), CEEG_TAG_ADAMW, h.ordinal + lo);
+      const uint4 r = aw_philox(seed, (uint32_t)quad, (uint32_t)(quad >> 32), CEEG_TAG_ADAMW, h.ordinal + lo);
       const uint32_t w[4] = {r.x, r.y, r.z, r.w};
       uint32_t cm = 0, cv = 0;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        cm |= aw_round<false>(mo[k], sm, w[k] & 0xffffu) << (8 * k);
-        cv |= aw_round<true>(root[k], sv, w[k] >> 16) << (8 * k);
+        cm |= aw_round<false>(mo[k], sm, pm, (float)(w[k] & 0xffffu)) << (8 * k);
+        cv |= aw_round<true>(root[k], sv, pr, (float)(w[k] >> 16)) << (8 * k);
       }
       aw_put_codes4(static_cast<uint8_t*>(m), i, n, svec, cm);
       aw_put_codes4(static_cast<uint8_t*>(v), i, n, svec, cv);

@@ -1,6 +1,7 @@
 """AdamW over many tensors in one launch (ceeg_adamw_step, include/ceeg.h), moments in 32 bits or in 8.  The reference trains with Adam
 (scripts/run.py:56); `Trainer(optimizer="adamw")` takes this one."""
 import ctypes as C
+import operator
 
 import torch
 
@@ -24,8 +25,11 @@ def block_values(state, square=False):
     return (x * x if square else x).view(codes.shape)
 
 
-def _pointers(tensors):
-    return (C.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+_dtype_of = operator.attrgetter("dtype")
+
+
+def _addresses(tensors):
+    return list(map(torch.Tensor.data_ptr, tensors))
 
 
 def _scalar(x, name, dev):
@@ -64,28 +68,38 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9,
     else:
         ms, vs = exp_avgs, exp_avg_sqs
     state = torch.float8_e4m3fn if held else torch.float32
-    sizes = [p.numel() for p in params]
-    for what, tensors, want in (("params", params, dtype), ("grads", grads, dtype), ("exp_avgs", ms, state), ("exp_avg_sqs", vs, state)):
-        for t, k in zip(tensors, sizes):
-            if not isinstance(t, torch.Tensor) or t.dtype != want or t.device != dev or t.numel() != k or not t.is_contiguous():
-                raise ValueError(f"{what}: contiguous {want} tensors of the parameters' sizes on {dev} expected" +
-                                 (f", got {t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else f", got {type(t).__name__}"))
+    every = (("params", params, dtype), ("grads", grads, dtype), ("exp_avgs", ms, state), ("exp_avg_sqs", vs, state))
+    T = torch.Tensor
+    for what, tensors, _ in every:
+        if not all(isinstance(t, T) for t in tensors):
+            raise ValueError(f"{what}: tensors expected")
+    sizes = list(map(T.numel, params))   # a call goes through hundreds of small tensors: mapped methods, no loop of attributes
+    at = params[0].get_device()
+    for what, tensors, want in every:
+        if list(map(T.numel, tensors)) != sizes or not all(map(T.is_contiguous, tensors)) or set(map(_dtype_of, tensors)) != {want} or \
+                set(map(T.get_device, tensors)) != {at}:
+            raise ValueError(f"{what}: contiguous {want} tensors of the parameters' sizes on {dev} expected, got " +
+                             ", ".join(f"{t.dtype} {tuple(t.shape)} on {t.device}" for t in tensors[:4]))
     if held:
-        for t, k in zip(scales, sizes + sizes):
-            if t.dtype != torch.float32 or t.device != dev or t.numel() != -(-k // BLOCK) or not t.is_contiguous():
-                raise ValueError(f"scales: contiguous float32 tensors of one element per {BLOCK} on {dev} expected, got {t.dtype} {tuple(t.shape)}")
+        if list(map(T.numel, scales)) != [-(-k // BLOCK) for k in sizes] * 2 or not all(map(T.is_contiguous, scales)) or \
+                set(map(_dtype_of, scales)) != {torch.float32} or set(map(T.get_device, scales)) != {at}:
+            raise ValueError(f"scales: contiguous float32 tensors of one element per {BLOCK} on {dev} expected, got " +
+                             ", ".join(f"{t.dtype} {tuple(t.shape)} on {t.device}" for t in scales[:4]))
     _lib.require_cuda(params[0])
-    where = [t.data_ptr() for ts in (params, ms, vs) + ((scales,) if held else ()) for t in ts if t.numel()]
+    pp, mp, vp = _addresses(params), _addresses(ms), _addresses(vs)
+    sp = _addresses(scales) if held else []
+    where = [a for a in pp + mp + vp + sp if a]   # an empty tensor has no address
     if len(set(where)) < len(where):
         raise ValueError("a tensor that the step writes is given twice")
     b1, b2 = betas
     step_t, lr_t = _scalar(step, "step", dev), _scalar(lr, "lr", dev)
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and (step_t is not None or step >= 1)):
         raise ValueError(f"betas in [0, 1), eps >= 0 and step >= 1 expected, got {betas}, {eps} and {step}")
+    array = C.c_void_p * n
     with _lib.on(dev):
         _lib.check(_lib.lib().ceeg_adamw_step(
-            n, (C.c_int64 * n)(*sizes), _pointers(params), _pointers(grads), _pointers(ms), _pointers(vs),
-            _pointers(m_scales) if held else None, _pointers(v_scales) if held else None, _DTYPES[dtype], 8 if held else 32,
+            n, (C.c_int64 * n)(*sizes), array(*pp), array(*_addresses(grads)), array(*mp), array(*vp),
+            array(*sp[:n]) if held else None, array(*sp[n:]) if held else None, _DTYPES[dtype], 8 if held else 32,
             0.0 if lr_t is not None else float(lr), float(b1), float(b2), float(eps), float(weight_decay), 1 if step_t is not None else int(step),
             _lib.ptr(lr_t), _lib.ptr(step_t), int(seed) & (2**64 - 1), _lib.stream()), "ceeg_adamw_step")
 
