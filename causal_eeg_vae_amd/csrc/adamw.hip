@@ -40,11 +40,11 @@ struct AwHyper {
   uint32_t per_wg;        // elements per workgroup
 };
 
-template <bool BF16>
+template <bool FULL, bool BF16>
 __device__ __forceinline__ void aw_load4(const void* p, int64_t i, int64_t n, bool vec, float (&x)[4]) {
   if (BF16) {
     const unsigned short* q = static_cast<const unsigned short*>(p) + i;
-    if (vec && i + 4 <= n) {
+    if (FULL || (vec && i + 4 <= n)) {
       const ushort4 u = *reinterpret_cast<const ushort4*>(q);
       x[0] = ceeg_bf16_to_f32(u.x); x[1] = ceeg_bf16_to_f32(u.y); x[2] = ceeg_bf16_to_f32(u.z); x[3] = ceeg_bf16_to_f32(u.w);
     } else {
@@ -53,7 +53,7 @@ __device__ __forceinline__ void aw_load4(const void* p, int64_t i, int64_t n, bo
     }
   } else {
     const float* q = static_cast<const float*>(p) + i;
-    if (vec && i + 4 <= n) {
+    if (FULL || (vec && i + 4 <= n)) {
       const float4 u = *reinterpret_cast<const float4*>(q);
       x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
     } else {
@@ -62,11 +62,11 @@ __device__ __forceinline__ void aw_load4(const void* p, int64_t i, int64_t n, bo
     }
   }
 }
-template <bool BF16>
+template <bool FULL, bool BF16>
 __device__ __forceinline__ void aw_store4(void* p, int64_t i, int64_t n, bool vec, const float (&x)[4]) {
   if (BF16) {  // a bf16 parameter is rounded to nearest, as every bf16 result of this library
     unsigned short* q = static_cast<unsigned short*>(p) + i;
-    if (vec && i + 4 <= n) {
+    if (FULL || (vec && i + 4 <= n)) {
       *reinterpret_cast<ushort4*>(q) = make_ushort4(ceeg_f32_to_bf16(x[0]), ceeg_f32_to_bf16(x[1]), ceeg_f32_to_bf16(x[2]), ceeg_f32_to_bf16(x[3]));
     } else {
 #pragma unroll
@@ -75,7 +75,7 @@ __device__ __forceinline__ void aw_store4(void* p, int64_t i, int64_t n, bool ve
     }
   } else {
     float* q = static_cast<float*>(p) + i;
-    if (vec && i + 4 <= n) {
+    if (FULL || (vec && i + 4 <= n)) {
       *reinterpret_cast<float4*>(q) = make_float4(x[0], x[1], x[2], x[3]);
     } else {
 #pragma unroll
@@ -84,16 +84,18 @@ __device__ __forceinline__ void aw_store4(void* p, int64_t i, int64_t n, bool ve
     }
   }
 }
+template <bool FULL>
 __device__ __forceinline__ uint32_t aw_codes4(const uint8_t* p, int64_t i, int64_t n, bool vec) {
-  if (vec && i + 4 <= n) return *reinterpret_cast<const uint32_t*>(p + i);
+  if (FULL || (vec && i + 4 <= n)) return *reinterpret_cast<const uint32_t*>(p + i);
   uint32_t w = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     if (i + k < n) w |= (uint32_t)p[i + k] << (8 * k);
   return w;
 }
+template <bool FULL>
 __device__ __forceinline__ void aw_put_codes4(uint8_t* p, int64_t i, int64_t n, bool vec, uint32_t w) {
-  if (vec && i + 4 <= n) {
+  if (FULL || (vec && i + 4 <= n)) {
     *reinterpret_cast<uint32_t*>(p + i) = w;
   } else {
 #pragma unroll
@@ -115,8 +117,7 @@ __device__ __forceinline__ uint4 aw_philox(uint64_t seed, uint32_t c0, uint32_t 
 }
 __device__ __forceinline__ bool aw_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 // the largest of 64 lanes' values >= 0, the same in every lane: six steps in registers
-__device__ __forceinline__ float aw_wave_max(float v) {
-  int x = __float_as_int(v);  // of values >= 0 the larger one has the larger bits
+__device__ __forceinline__ float aw_wave_max(int x) {  // bits of values >= 0: the larger value has the larger bits, infinities and NaN the largest
 #define AW_MAX(CTRL, ROWS) x = max(x, __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, true))
   AW_MAX(0x111, 0xf);  // row_shr 1, 2, 4, 8: lane 15 of each row of 16
   AW_MAX(0x112, 0xf);
@@ -135,7 +136,7 @@ __device__ __forceinline__ float aw_quotient(float a, float b, float r) {
 // x / scale as an e4m3 number, rounded by the 16 random bits `rnd` so that the expectation of its magnitude (SECOND: of its square) is kept.  per_scale: 1 / scale,
 // 0 where the scale is.  Between the numbers L s and (L + 1) s (s: their distance, L < 16) the magnitude is (L + share) s, and
 //   (y^2 - low^2) / (high^2 - low^2) = share (2 L + share) / (2 L + 1).
-template <bool SECOND>
+template <bool SECOND, bool FINITE>
 __device__ __forceinline__ uint32_t aw_round(float x, float scale, float per_scale, float rnd) {
   const float a = fabsf(x), y = fminf(aw_quotient(a, scale, per_scale), AW_TOP);
   const uint32_t u = __float_as_uint(y);
@@ -150,9 +151,11 @@ __device__ __forceinline__ uint32_t aw_round(float x, float scale, float per_sca
   }
   c += share * 65536.f + rnd >= 65536.f;
   if (SECOND && c == 0u && y > 0.f) c = 1u;
-  if (!aw_finite(x)) c = 0x7fu;  // stays a NaN
+  if (!FINITE && !aw_finite(x)) c = 0x7fu;  // stays a NaN
   return c | (__float_as_uint(x) >> 24 & 0x80u);
 }
+
+template <bool B> struct AwBool { static constexpr bool value = B; };
 
 template <bool BF16, int BITS>
 __global__ __launch_bounds__(AW_THREADS) void adamw_kernel(AwList L, AwHyper h) {
@@ -187,14 +190,16 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_kernel(AwList L, AwHyper h) 
   const uintptr_t mv = reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v);
   const bool vec = (pg & (BF16 ? 7 : 15)) == 0, svec = (mv & (BITS == 8 ? 3 : 15)) == 0;
 
-  for (int64_t b0 = begin + (int64_t)wave * AW_BLOCK; b0 < end; b0 += AW_THREADS / 64 * AW_BLOCK) {
+  // FULL: a block of 256 elements on aligned addresses, without a check per element
+  auto block = [&](auto full, int64_t b0) {
+    constexpr bool FULL = decltype(full)::value;
     const int64_t i = b0 + 4 * lane;
     float pv[4], gv[4], mo[4], vo[4], root[4];
-    aw_load4<BF16>(p, i, n, vec, pv);
-    aw_load4<BF16>(g, i, n, vec, gv);
+    aw_load4<FULL, BF16>(p, i, n, vec, pv);
+    aw_load4<FULL, BF16>(g, i, n, vec, gv);
     if (BITS == 8) {
       const float sm = L.ms[lo][b0 / AW_BLOCK], sv = L.vs[lo][b0 / AW_BLOCK];
-      const uint32_t cm = aw_codes4(static_cast<const uint8_t*>(m), i, n, svec), cv = aw_codes4(static_cast<const uint8_t*>(v), i, n, svec);
+      const uint32_t cm = aw_codes4<FULL>(static_cast<const uint8_t*>(m), i, n, svec), cv = aw_codes4<FULL>(static_cast<const uint8_t*>(v), i, n, svec);
       mo[0] = __builtin_amdgcn_cvt_f32_fp8(cm, 0); mo[1] = __builtin_amdgcn_cvt_f32_fp8(cm, 1);
       mo[2] = __builtin_amdgcn_cvt_f32_fp8(cm, 2); mo[3] = __builtin_amdgcn_cvt_f32_fp8(cm, 3);
       root[0] = __builtin_amdgcn_cvt_f32_fp8(cv, 0); root[1] = __builtin_amdgcn_cvt_f32_fp8(cv, 1);
@@ -206,8 +211,8 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_kernel(AwList L, AwHyper h) 
         vo[k] = u * u;
       }
     } else {
-      aw_load4<false>(m, i, n, svec, mo);
-      aw_load4<false>(v, i, n, svec, vo);
+      aw_load4<FULL, false>(m, i, n, svec, mo);
+      aw_load4<FULL, false>(v, i, n, svec, vo);
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -216,38 +221,60 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_kernel(AwList L, AwHyper h) 
       root[k] = sqrtf(vo[k]);
       pv[k] = pv[k] * decay - step_size * (mo[k] * __builtin_amdgcn_rcpf(root[k] * inv_sqrt_c2 + h.eps));
     }
-    aw_store4<BF16>(p, i, n, vec, pv);
-    if (BITS == 8) {
-      float tm = 0.f, tv = 0.f;
+    aw_store4<FULL, BF16>(p, i, n, vec, pv);
+    if (BITS == 32) {
+      aw_store4<FULL, false>(m, i, n, svec, mo);
+      aw_store4<FULL, false>(v, i, n, svec, vo);
+      return;
+    }
+    int bm = 0, bv = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (!FULL && i + k >= n) mo[k] = root[k] = 0.f;
+      bm = max(bm, __float_as_int(fabsf(mo[k])));
+      bv = max(bv, __float_as_int(fabsf(root[k])));
+    }
+    float tm = aw_wave_max(bm), tv = aw_wave_max(bv);
+    const bool finite = aw_finite(tm) && aw_finite(tv);
+    if (!finite) {  // infinities and NaN do not set a block's scale
+      bm = bv = 0;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (i + k >= n) mo[k] = root[k] = 0.f;
-        tm = fmaxf(tm, aw_finite(mo[k]) ? fabsf(mo[k]) : 0.f);  // infinities and NaN do not set a block's scale
-        tv = fmaxf(tv, aw_finite(root[k]) ? root[k] : 0.f);
+        bm = max(bm, aw_finite(mo[k]) ? __float_as_int(fabsf(mo[k])) : 0);
+        bv = max(bv, aw_finite(root[k]) ? __float_as_int(root[k]) : 0);
       }
-      tm = aw_wave_max(tm);
-      tv = aw_wave_max(tv);
-      const float sm = tm < AW_TINY ? 0.f : tm * AW_PER_TOP, sv = tv < AW_TINY ? 0.f : tv * AW_PER_TOP;
-      const float pm = sm > 0.f ? 1.f / sm : 0.f, pr = sv > 0.f ? 1.f / sv : 0.f;
-      const uint64_t quad = (uint64_t)i >> 2;
-      const uint4 r = aw_philox(seed, (uint32_t)quad, (uint32_t)(quad >> 32), CEEG_TAG_ADAMW, h.ordinal + lo);
-      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-      uint32_t cm = 0, cv = 0;
+      tm = aw_wave_max(bm);
+      tv = aw_wave_max(bv);
+    }
+    const float sm = tm < AW_TINY ? 0.f : tm * AW_PER_TOP, sv = tv < AW_TINY ? 0.f : tv * AW_PER_TOP;
+    const float pm = sm > 0.f ? 1.f / sm : 0.f, pr = sv > 0.f ? 1.f / sv : 0.f;
+    const uint64_t quad = (uint64_t)i >> 2;
+    const uint4 r = aw_philox(seed, (uint32_t)quad, (uint32_t)(quad >> 32), CEEG_TAG_ADAMW, h.ordinal + lo);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    uint32_t cm = 0, cv = 0;
+    if (finite) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        cm |= aw_round<false>(mo[k], sm, pm, (float)(w[k] & 0xffffu)) << (8 * k);
-        cv |= aw_round<true>(root[k], sv, pr, (float)(w[k] >> 16)) << (8 * k);
-      }
-      aw_put_codes4(static_cast<uint8_t*>(m), i, n, svec, cm);
-      aw_put_codes4(static_cast<uint8_t*>(v), i, n, svec, cv);
-      if (lane == 0) {
-        L.ms[lo][b0 / AW_BLOCK] = sm;
-        L.vs[lo][b0 / AW_BLOCK] = sv;
+        cm |= aw_round<false, true>(mo[k], sm, pm, (float)(w[k] & 0xffffu)) << (8 * k);
+        cv |= aw_round<true, true>(root[k], sv, pr, (float)(w[k] >> 16)) << (8 * k);
       }
     } else {
-      aw_store4<false>(m, i, n, svec, mo);
-      aw_store4<false>(v, i, n, svec, vo);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        cm |= aw_round<false, false>(mo[k], sm, pm, (float)(w[k] & 0xffffu)) << (8 * k);
+        cv |= aw_round<true, false>(root[k], sv, pr, (float)(w[k] >> 16)) << (8 * k);
+      }
     }
+    aw_put_codes4<FULL>(static_cast<uint8_t*>(m), i, n, svec, cm);
+    aw_put_codes4<FULL>(static_cast<uint8_t*>(v), i, n, svec, cv);
+    if (lane == 0) {
+      L.ms[lo][b0 / AW_BLOCK] = sm;
+      L.vs[lo][b0 / AW_BLOCK] = sv;
+    }
+  };
+  for (int64_t b0 = begin + (int64_t)wave * AW_BLOCK; b0 < end; b0 += AW_THREADS / 64 * AW_BLOCK) {
+    if (vec && svec && b0 + AW_BLOCK <= n) block(AwBool<true>{}, b0);
+    else block(AwBool<false>{}, b0);
   }
 }
 }  // namespace
