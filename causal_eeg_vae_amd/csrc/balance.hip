@@ -8,10 +8,11 @@
 #include "ceeg_internal.h"
 
 namespace {
-constexpr int BL_THREADS = 256;
+constexpr int BL_THREADS = 512;
 constexpr int BL_WAVES = BL_THREADS / 64;
 constexpr int BL_MAX_E = 4096;
-constexpr int BL_MAX_WG = 1024;
+constexpr int BL_MAX_WG = 512;
+constexpr int BL_JOIN = 16;  // columns per workgroup of the join
 
 struct BlRow {  // where the scores of a row and the columns of a lane are
   const void* s;
@@ -54,13 +55,35 @@ __device__ __forceinline__ void bl_load(const BlRow& a, int64_t t, int l, float 
   }
 }
 
+// Over the lane group of a row, the same in each of its lanes: a whole wave joins in registers (row shifts and broadcasts end in lane 63), smaller groups by butterflies.
+__device__ __forceinline__ float bl_max(int lanes, float v) {
+  if (lanes == 64) {
+#define BL_STEP(CTRL, ROWS) v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, ROWS, 0xf, false)))
+    BL_STEP(0x111, 0xf); BL_STEP(0x112, 0xf); BL_STEP(0x114, 0xf); BL_STEP(0x118, 0xf); BL_STEP(0x142, 0xa); BL_STEP(0x143, 0xc);
+#undef BL_STEP
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+  }
+  for (int o = lanes >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+__device__ __forceinline__ float bl_sum(int lanes, float v) {
+  if (lanes == 64) {
+#define BL_STEP(CTRL, ROWS) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, true))
+    BL_STEP(0x111, 0xf); BL_STEP(0x112, 0xf); BL_STEP(0x114, 0xf); BL_STEP(0x118, 0xf); BL_STEP(0x142, 0xa); BL_STEP(0x143, 0xc);
+#undef BL_STEP
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+  }
+  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
 // x -> softmax over the lane group; a row of nothing but -inf has no probability anywhere
 template <int N>
 __device__ __forceinline__ void bl_softmax(int lanes, float (&x)[N]) {
   float top = x[0];
 #pragma unroll
   for (int k = 1; k < N; ++k) top = fmaxf(top, x[k]);
-  for (int o = lanes >> 1; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  top = bl_max(lanes, top);
   const float base = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
 #pragma unroll
@@ -68,7 +91,7 @@ __device__ __forceinline__ void bl_softmax(int lanes, float (&x)[N]) {
     x[k] = __expf(x[k] - base);
     sum += x[k];
   }
-  for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  sum = bl_sum(lanes, sum);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int k = 0; k < N; ++k) x[k] *= inv;
@@ -105,26 +128,36 @@ __global__ __launch_bounds__(BL_THREADS) void balance_rows_kernel(BlRow a, const
   for (int k = 0; k < NV * VEC; ++k) acc[k] = 0.f;
   int rows = 0, bad = 0;
   const int64_t stride = (int64_t)gridDim.x * BL_WAVES * per;
-  for (int64_t t0 = ((int64_t)blockIdx.x * BL_WAVES + wave) * per; t0 < a.T; t0 += stride) {  // the same number of turns for a wave's lanes
-    const int64_t t = t0 + sub;
-    const bool on = t < a.T && (!a.mask || a.mask[t]);
-    float x[NV * VEC];
-    if (on) {
-      bl_load<BF16, VEC, NV>(a, t, l, x);
-    } else {
+  constexpr int R = NV * VEC <= 16 ? 2 : 1;  // rows at a time: the second one's loads and butterflies run in the shadow of the first one's
+  for (int64_t t0 = ((int64_t)blockIdx.x * BL_WAVES + wave) * per; t0 < a.T; t0 += R * stride) {  // the same number of turns for a wave's lanes
+    float x[R][NV * VEC];
+    bool on[R];
 #pragma unroll
-      for (int k = 0; k < NV * VEC; ++k) x[k] = -INFINITY;
-    }
-    bl_softmax(a.lanes, x);
+    for (int r = 0; r < R; ++r) {
+      const int64_t t = t0 + r * stride + sub;
+      on[r] = t < a.T && (!a.mask || a.mask[t]);
+      if (on[r]) {
+        bl_load<BF16, VEC, NV>(a, t, l, x[r]);
+      } else {
 #pragma unroll
-    for (int k = 0; k < NV * VEC; ++k) acc[k] += x[k];
-    if (on) {
-      for (int j = l; j < K; j += a.lanes) {
-        const int64_t e = idx64 ? static_cast<const int64_t*>(idx)[t * K + j] : (int64_t)static_cast<const int32_t*>(idx)[t * K + j];
-        if (e >= 0 && e < a.E) atomicAdd(&s_c[e], 1);
-        else if (e != -1) bad = 1;
+        for (int k = 0; k < NV * VEC; ++k) x[r][k] = -INFINITY;
       }
-      rows += l == 0;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) bl_softmax(a.lanes, x[r]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t t = t0 + r * stride + sub;
+#pragma unroll
+      for (int k = 0; k < NV * VEC; ++k) acc[k] += x[r][k];
+      if (on[r]) {
+        for (int j = l; j < K; j += a.lanes) {
+          const int64_t e = idx64 ? static_cast<const int64_t*>(idx)[t * K + j] : (int64_t)static_cast<const int32_t*>(idx)[t * K + j];
+          if (e >= 0 && e < a.E) atomicAdd(&s_c[e], 1);
+          else if (e != -1) bad = 1;
+        }
+        rows += l == 0;
+      }
     }
   }
   // the lane groups of a wave hold the same columns
@@ -174,24 +207,37 @@ __global__ __launch_bounds__(BL_THREADS) void balance_rows_kernel(BlRow a, const
   if (threadIdx.x == 0) part_n[blockIdx.x] = make_int2(s_n[0], s_n[1]);
 }
 
-// 64 columns per workgroup: P and counts over all workgroups of the row pass; f = counts / (n K); stats = [f (E), n]; dots[wg] = sum f P
+// 16 columns per workgroup: P and counts over all workgroups of the row pass; f = counts / (n K); stats = [f (E), n]; dots[wg] = sum f P.  The partial sums come from other
+// XCDs' memory side, so that latency bounds this: 64 threads a column, 8 loads of each in flight.
 __global__ __launch_bounds__(1024) void balance_join_kernel(const float* __restrict__ part_p, const int32_t* __restrict__ part_c,
                                                             const int2* __restrict__ part_n, int wgs, int E, int K, int64_t* __restrict__ counts,
                                                             float* __restrict__ stats, double* __restrict__ dots) {
-  __shared__ double s_p[16][64];
-  __shared__ long long s_c[16][64];
+  constexpr int ROWS = 1024 / BL_JOIN;
+  __shared__ double s_p[ROWS][BL_JOIN];
+  __shared__ long long s_c[ROWS][BL_JOIN];
   __shared__ long long s_n[16];
   __shared__ int s_bad;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int e = blockIdx.x * 64 + lane;
+  const int col = threadIdx.x % BL_JOIN, row = threadIdx.x / BL_JOIN;
+  const int e = blockIdx.x * BL_JOIN + col;
   if (threadIdx.x == 0) s_bad = 0;
   double p = 0.0;
   long long c = 0, n = 0;
   int bad = 0;
   if (e < E) {
-    for (int b = w; b < wgs; b += 16) {
-      p += (double)part_p[(int64_t)b * E + e];
-      c += part_c[(int64_t)b * E + e];
+    for (int b0 = row; b0 < wgs; b0 += 8 * ROWS) {
+      float vp[8];
+      int vc[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int b = b0 + ROWS * k;
+        vp[k] = b < wgs ? part_p[(int64_t)b * E + e] : 0.f;
+        vc[k] = b < wgs ? part_c[(int64_t)b * E + e] : 0;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        p += (double)vp[k];
+        c += vc[k];
+      }
     }
   }
   for (int b = threadIdx.x; b < wgs; b += 1024) {
@@ -199,31 +245,34 @@ __global__ __launch_bounds__(1024) void balance_join_kernel(const float* __restr
     bad |= part_n[b].y;
   }
   for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-  s_p[w][lane] = p;
-  s_c[w][lane] = c;
-  if (lane == 0) s_n[w] = n;
+  s_p[row][col] = p;
+  s_c[row][col] = c;
+  if ((threadIdx.x & 63) == 0) s_n[threadIdx.x >> 6] = n;
   __syncthreads();
   if (bad) s_bad = 1;  // every writer writes the same
   __syncthreads();
-  if (w == 0) {
+  if (threadIdx.x < 64) {
     p = 0.0; c = 0; n = 0;
-    for (int k = 0; k < 16; ++k) { p += s_p[k][lane]; c += s_c[k][lane]; n += s_n[k]; }
+    for (int k = 0; k < ROWS; ++k) { p += s_p[k][col]; c += s_c[k][col]; }
+    for (int k = 0; k < 16; ++k) n += s_n[k];
     const double rows = n > 0 ? (double)n : 1.0;  // no row that counts: loss and gradient are zero
     const double f = bl_share(c, rows, K, s_bad != 0);
     double d = 0.0;
-    if (e < E) {
+    if (row == 0 && e < E) {
       counts[e] = c;
       stats[e] = (float)f;
       d = f * (p / rows);
     }
-    if (blockIdx.x == 0 && lane == 0) stats[E] = (float)rows;
+    if (blockIdx.x == 0 && threadIdx.x == 0) stats[E] = (float)rows;
     d = ceeg_wave_sum_d(d);
-    if (lane == 0) dots[blockIdx.x] = d;
+    if (threadIdx.x == 0) dots[blockIdx.x] = d;
   }
 }
 
 __global__ void balance_loss_kernel(const double* __restrict__ dots, int n, int E, float* __restrict__ loss) {
-  const double d = ceeg_wave_sum_d((int)threadIdx.x < n ? dots[threadIdx.x] : 0.0);  // E <= 4096: at most 64 parts
+  double d = 0.0;
+  for (int k = threadIdx.x; k < n; k += 64) d += dots[k];
+  d = ceeg_wave_sum_d(d);
   if (threadIdx.x == 0) loss[0] = (float)(d * E);
 }
 
@@ -253,7 +302,7 @@ __global__ __launch_bounds__(BL_THREADS) void balance_grad_kernel(BlRow a, const
       float d = 0.f;
 #pragma unroll
       for (int k = 0; k < NV * VEC; ++k) d = __fmaf_rn(f[k], x[k], d);
-      for (int o = a.lanes >> 1; o > 0; o >>= 1) d += __shfl_xor(d, o, 64);
+      d = bl_sum(a.lanes, d);
 #pragma unroll
       for (int k = 0; k < NV * VEC; ++k) x[k] = scale * x[k] * (f[k] - d);
     } else {
@@ -297,9 +346,9 @@ bool bl_vec(const void* s, int64_t ld, int E, int dtype) {
   return E % per == 0 && ld % per == 0 && ceeg_aligned(s, 16);
 }
 int bl_wgs(int64_t T, int E, int lanes) {
-  // as many workgroups as there are rows for, 1024 at most (four per compute unit), fewer where their partial sums would weigh more than the rows
+  // as many workgroups as there are rows for, 512 at most (16 waves per compute unit), fewer where their partial sums would weigh more than the rows
   int64_t wgs = (T + BL_WAVES * (64 / lanes) - 1) / (BL_WAVES * (64 / lanes));
-  const int64_t cap = E > 1024 ? BL_MAX_WG / 4 : BL_MAX_WG;
+  const int64_t cap = E > 1024 ? BL_MAX_WG / 2 : BL_MAX_WG;
   return (int)(wgs < cap ? wgs : cap);
 }
 int bl_check(const void* s, int64_t ld, int64_t T, int E, int dtype) {
@@ -344,7 +393,7 @@ extern "C" size_t ceeg_balance_ws_bytes(int64_t T, int E) {
   int lanes, nv;
   bl_shape(E, 1, &lanes, &nv);  // one column a piece has the most lanes per row, hence the most workgroups
   const size_t wgs = (size_t)bl_wgs(T, E, lanes);
-  return ceeg_ws_part(wgs * E, 4) + ceeg_ws_part(wgs * E, 4) + ceeg_ws_part(wgs, 8) + ceeg_ws_part(64, 8);
+  return ceeg_ws_part(wgs * E, 4) + ceeg_ws_part(wgs * E, 4) + ceeg_ws_part(wgs, 8) + ceeg_ws_part(BL_MAX_E / BL_JOIN, 8);
 }
 
 extern "C" int ceeg_balance_fwd(const void* scores, int64_t ld, int dtype, const void* idx, int idx_bytes, int64_t T, int E, int K, const uint8_t* mask,
@@ -363,14 +412,14 @@ extern "C" int ceeg_balance_fwd(const void* scores, int64_t ld, int dtype, const
   float* part_p = w.take<float>((size_t)wgs * E);
   int32_t* part_c = w.take<int32_t>((size_t)wgs * E);
   int2* part_n = w.take<int2>(wgs);
-  double* dots = w.take<double>(64);
+  double* dots = w.take<double>(BL_MAX_E / BL_JOIN);
   if (!w.ok) return CEEG_EWORKSPACE;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const size_t lds = (size_t)E * 8;  // 32 KB at most
   BL_DISPATCH(balance_rows_kernel, <<<wgs, BL_THREADS, lds, st>>>(a, idx, idx_bytes == 8, K, part_p, part_c, part_n, BlOut{loss, counts, stats}));
   CEEG_CHECK_LAUNCH();
   if (wgs == 1) return CEEG_OK;
-  const int joins = (E + 63) / 64;
+  const int joins = (E + BL_JOIN - 1) / BL_JOIN;
   balance_join_kernel<<<joins, 1024, 0, st>>>(part_p, part_c, part_n, wgs, E, K, counts, stats, dots);
   CEEG_CHECK_LAUNCH();
   balance_loss_kernel<<<1, 64, 0, st>>>(dots, joins, E, loss);
@@ -388,7 +437,7 @@ extern "C" int ceeg_balance_bwd(const void* scores, int64_t ld, int dtype, int64
   int nv;
   bl_shape(E, vec, &a.lanes, &nv);
   const int64_t units = (T + BL_WAVES * (64 / a.lanes) - 1) / (BL_WAVES * (64 / a.lanes));
-  const unsigned wgs = (unsigned)(units < 2048 ? units : 2048);  // eight per compute unit: every lane reads its f once for many rows
+  const unsigned wgs = (unsigned)(units < 1024 ? units : 1024);  // four per compute unit: every lane reads its f once for many rows
   const hipStream_t st = static_cast<hipStream_t>(stream);
   BL_DISPATCH(balance_grad_kernel, <<<wgs, BL_THREADS, 0, st>>>(a, stats, g, dscores));
   CEEG_CHECK_LAUNCH();

@@ -1,6 +1,6 @@
 """AdamW over many tensors in one launch (ceeg_adamw_step, include/ceeg.h), moments in 32 bits or in 8.  The reference trains with Adam
 (scripts/run.py:56); `Trainer(optimizer="adamw")` takes this one."""
-import ctypes as C
+import array
 import operator
 
 import torch
@@ -52,6 +52,8 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9,
         raise ValueError(f"lists of one length expected, got {n}, {len(grads)}, {len(exp_avgs)} and {len(exp_avg_sqs)}")
     if n == 0:
         return
+    if not isinstance(params[0], torch.Tensor):
+        raise TypeError(f"parameters must be tensors, got {type(params[0]).__name__}")
     dtype, dev = params[0].dtype, params[0].device
     if dtype not in _DTYPES:
         raise TypeError(f"parameters must be float32 or bfloat16, got {dtype}")
@@ -70,16 +72,16 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9,
     state = torch.float8_e4m3fn if held else torch.float32
     every = (("params", params, dtype), ("grads", grads, dtype), ("exp_avgs", ms, state), ("exp_avg_sqs", vs, state))
     T = torch.Tensor
-    for what, tensors, _ in every:
-        if not all(isinstance(t, T) for t in tensors):
-            raise ValueError(f"{what}: tensors expected")
-    sizes = list(map(T.numel, params))   # a call goes through hundreds of small tensors: mapped methods, no loop of attributes
-    at = params[0].get_device()
-    for what, tensors, want in every:
-        if list(map(T.numel, tensors)) != sizes or not all(map(T.is_contiguous, tensors)) or set(map(_dtype_of, tensors)) != {want} or \
-                set(map(T.get_device, tensors)) != {at}:
-            raise ValueError(f"{what}: contiguous {want} tensors of the parameters' sizes on {dev} expected, got " +
-                             ", ".join(f"{t.dtype} {tuple(t.shape)} on {t.device}" for t in tensors[:4]))
+    try:   # a call goes through hundreds of small tensors: mapped methods, no loop of attributes
+        sizes = list(map(T.numel, params))
+        at = params[0].get_device()
+        for what, tensors, want in every:
+            if list(map(T.numel, tensors)) != sizes or not all(map(T.is_contiguous, tensors)) or set(map(_dtype_of, tensors)) != {want} or \
+                    set(map(T.get_device, tensors)) != {at}:
+                raise ValueError(f"{what}: contiguous {want} tensors of the parameters' sizes on {dev} expected, got " +
+                                 ", ".join(f"{t.dtype} {tuple(t.shape)} on {t.device}" for t in tensors[:4]))
+    except TypeError:
+        raise ValueError("params, grads, exp_avgs and exp_avg_sqs: tensors expected") from None
     if held:
         if list(map(T.numel, scales)) != [-(-k // BLOCK) for k in sizes] * 2 or not all(map(T.is_contiguous, scales)) or \
                 set(map(_dtype_of, scales)) != {torch.float32} or set(map(T.get_device, scales)) != {at}:
@@ -88,18 +90,19 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9,
     _lib.require_cuda(params[0])
     pp, mp, vp = _addresses(params), _addresses(ms), _addresses(vs)
     sp = _addresses(scales) if held else []
-    where = [a for a in pp + mp + vp + sp if a]   # an empty tensor has no address
-    if len(set(where)) < len(where):
+    where = pp + mp + vp + sp
+    if len(set(where) - {0}) < len(where) - where.count(0):   # an empty tensor has no address
         raise ValueError("a tensor that the step writes is given twice")
     b1, b2 = betas
     step_t, lr_t = _scalar(step, "step", dev), _scalar(lr, "lr", dev)
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and (step_t is not None or step >= 1)):
         raise ValueError(f"betas in [0, 1), eps >= 0 and step >= 1 expected, got {betas}, {eps} and {step}")
-    array = C.c_void_p * n
+    # host arrays of addresses, alive for the call
+    lists = [array.array("q", sizes)] + [array.array("Q", x) for x in (pp, _addresses(grads), mp, vp, sp[:n], sp[n:])]
+    sizes_at, p_at, g_at, m_at, v_at, ms_at, vs_at = (x.buffer_info()[0] for x in lists)
     with _lib.on(dev):
         _lib.check(_lib.lib().ceeg_adamw_step(
-            n, (C.c_int64 * n)(*sizes), array(*pp), array(*_addresses(grads)), array(*mp), array(*vp),
-            array(*sp[:n]) if held else None, array(*sp[n:]) if held else None, _DTYPES[dtype], 8 if held else 32,
+            n, sizes_at, p_at, g_at, m_at, v_at, ms_at if held else None, vs_at if held else None, _DTYPES[dtype], 8 if held else 32,
             0.0 if lr_t is not None else float(lr), float(b1), float(b2), float(eps), float(weight_decay), 1 if step_t is not None else int(step),
             _lib.ptr(lr_t), _lib.ptr(step_t), int(seed) & (2**64 - 1), _lib.stream()), "ceeg_adamw_step")
 
