@@ -629,16 +629,16 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_dlogits_kernel(CeMat W, CeMa
         for (int k = 0; k < 4; ++k)
           if (t >= N || vb + i * 16 + 4 * q + k >= Vc) g.acc[i][j][k] = 0.f;  // whatever was multiplied there
     }
-    if (t >= Nz) continue;
+    // through LDS (the tiles are done with), so that rows leave in whole lines: token by token, its 16-byte pieces at piece ^ (token mod 16)
+    const int tl = (wn * G::NT + j) * 16 + (lane & 15);
 #pragma unroll
     for (int i = 0; i < G::MT; ++i) {
-      const int v = vb + i * 16 + 4 * q;
-      if (v >= ldv) continue;
+      const int vl = (wm * G::MT + i) * 16 + 4 * q;
       f32x4 x = g.acc[i][j];
 #pragma unroll
       for (int a = 0; a < PL; ++a) {
         const uint2 p = make_uint2(ceeg_f32_to_bf16x2(x[0], x[1]), ceeg_f32_to_bf16x2(x[2], x[3]));
-        *reinterpret_cast<uint2*>(dl + a * plane + (int64_t)t * ldv + v) = p;
+        *reinterpret_cast<uint2*>(lds + a * BN * BM + tl * BM + (((vl >> 3) ^ (tl & (BM / 8 - 1) & 15)) * 8 + (vl & 4))) = p;
         if (a + 1 < PL) {  // what the plane leaves, 2^8 times
           x[0] = (x[0] - __uint_as_float(p.x << 16)) * 256.f;
           x[1] = (x[1] - __uint_as_float(p.x & 0xffff0000u)) * 256.f;
@@ -646,6 +646,18 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_dlogits_kernel(CeMat W, CeMa
           x[3] = (x[3] - __uint_as_float(p.y & 0xffff0000u)) * 256.f;
         }
       }
+    }
+  }
+  __syncthreads();
+  constexpr int PER = BM / 8;
+  static_assert(PL * BN * BM <= G::LDS && BN * PER % G::THREADS == 0, "the tile fits");
+#pragma unroll
+  for (int a = 0; a < PL; ++a) {
+#pragma unroll
+    for (int c = 0; c < BN * PER / G::THREADS; ++c) {
+      const int at = c * G::THREADS + threadIdx.x, tl = at / PER, piece = at % PER, t = n0 + tl, v = m0 + piece * 8;
+      if (t < Nz && v < ldv)
+        *reinterpret_cast<uint4*>(dl + a * plane + (int64_t)t * ldv + v) = *reinterpret_cast<const uint4*>(lds + a * BN * BM + tl * BM + (piece ^ (tl & (PER - 1) & 15)) * 8);
     }
   }
 }
