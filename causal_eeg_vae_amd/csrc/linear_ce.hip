@@ -396,7 +396,7 @@ struct CeTile {
 
 // The tile shapes.  256 x 256 on eight waves reads LDS least per product and fills the chip from 256 tiles up (one workgroup per compute unit); 128 x 128 halves what is lost on
 // smaller grids; 64 x 64 spreads the smallest, which are bound by latency, and keeps more tiles on their way.
-template <int PL, bool TA, bool TB> struct CeBig { using Tile = CeTile<1, 256, 256, 2, 4, 4, false, TA, TB>; };
+template <int PL, bool TA, bool TB> struct CeBig { using Tile = CeTile<1, 256, 256, 2, 4, 4, true, TA, TB>; };
 template <int PL, bool TA, bool TB> struct CeMid { using Tile = CeTile<1, 128, 128, 2, 2, 4, true, TA, TB>; };
 template <bool TA, bool TB> struct CeMid<3, TA, TB> { using Tile = CeTile<3, 128, 128, 4, 2, 3, false, TA, TB>; };
 template <int PL, bool TA, bool TB> struct CeSmall { using Tile = CeTile<1, 64, 64, 2, 2, 8, true, TA, TB>; };
@@ -662,14 +662,30 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_dlogits_kernel(CeMat W, CeMa
   }
 }
 
+// Into how many stretches a sum of k elements is cut for a grid of `tiles`, so that the compute units hold as many workgroups as their LDS allows (`want`), each with
+// 256 elements at least.  dh: few tiles (tokens x H) against a long sum over the vocabulary; its tokens are counted on the device, and fewer of them mean more stretches.
+struct CeCut {
+  int want;        // 0: `most` is the number
+  int most;
+  int64_t room;    // rows of all slots together that there is memory for
+};
+__host__ __device__ __forceinline__ int ce_slots(const CeCut& c, int64_t tiles, int64_t rows, int64_t k) {
+  if (c.want == 0) return c.most;
+  int64_t s = c.want / (tiles > 0 ? tiles : 1);
+  if (s > k / 256) s = k / 256;
+  if (s > c.room / (rows > 0 ? rows : 1)) s = c.room / (rows > 0 ? rows : 1);
+  if (s > 64) s = 64;
+  return (int)(s < 1 ? 1 : s);
+}
+
 // D of a product into fp32 slots [slots][rows][H], each holding a stretch of the sum (k_slot elements): dh += dl W (rows: tokens, A = W, B = dl) or dW = dl^T h (rows:
 // classes, A = h, B = dl).  A slot keeps its sum over the pieces (`add`).
 template <class G, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(G::THREADS, 1) void ce_slots_kernel(CeMat A, CeMat B, const int32_t* __restrict__ n, int by_tokens, int H, int64_t rows, int K, int slots, int add,
+__global__ __launch_bounds__(G::THREADS, 1) void ce_slots_kernel(CeMat A, CeMat B, const int32_t* __restrict__ n, int by_tokens, int H, int64_t rows, int K, int k_all, CeCut cut, int add,
                                                               float* __restrict__ out) {
   __shared__ __align__(16) unsigned short lds[G::LDS];
   const int N = n[0], end = by_tokens ? N : (int)rows;
-  const int tiles_m = (H + BM - 1) / BM, tiles = tiles_m * ((end + BN - 1) / BN), id = ce_xcd(blockIdx.x, tiles * slots);
+  const int tiles_m = (H + BM - 1) / BM, tiles = tiles_m * ((end + BN - 1) / BN), slots = ce_slots(cut, tiles, end, k_all), id = ce_xcd(blockIdx.x, tiles * slots);
   if (id < 0) return;
   const int slot = id / tiles, rest = id - slot * tiles;
   const int m0 = rest % tiles_m * BM, n0 = rest / tiles_m * BN;
@@ -691,7 +707,7 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_slots_kernel(CeMat A, CeMat 
   for (int j = 0; j < G::NT; ++j) {
     const int r = n0 + (wn * G::NT + j) * 16 + (lane & 15);
     if (r >= end) continue;
-    float* const to = out + (slot * rows + r) * H;
+    float* const to = out + ((int64_t)slot * end + r) * H;
 #pragma unroll
     for (int i = 0; i < G::MT; ++i) {
       const int c = m0 + (wm * G::MT + i) * 16 + 4 * q;
@@ -750,15 +766,15 @@ __global__ __launch_bounds__(256) void ce_dw_join_kernel(const float* __restrict
 }
 
 template <bool F32>
-__global__ __launch_bounds__(256) void ce_dh_join_kernel(const float* __restrict__ part, int slots, const int32_t* __restrict__ n, const int32_t* __restrict__ pos, CeScale scale, int64_t T,
-                                                         int H, void* __restrict__ dh) {
+__global__ __launch_bounds__(256) void ce_dh_join_kernel(const float* __restrict__ part, int edge, int k_all, CeCut cut, const int32_t* __restrict__ n, const int32_t* __restrict__ pos,
+                                                         CeScale scale, int H, void* __restrict__ dh) {
   const int64_t t = blockIdx.x;
-  const int j = pos[t];
-  const float s = scale.s(n[0]);
+  const int N = n[0], j = pos[t], slots = ce_slots(cut, (int64_t)((H + edge - 1) / edge) * ((N + edge - 1) / edge), N, k_all);
+  const float s = scale.s(N);
   for (int c = threadIdx.x; c < H; c += 256) {
     float x = 0.f;
     if (j >= 0) {
-      for (int k = 0; k < slots; ++k) x += part[(k * T + j) * H + c];
+      for (int k = 0; k < slots; ++k) x += part[((int64_t)k * N + j) * H + c];
       x *= s;
     }
     if (F32) static_cast<float*>(dh)[t * H + c] = x;
@@ -777,6 +793,9 @@ int ce_edge(int planes, int64_t rows, int64_t cols, int64_t cuts) {
   return 64;
 }
 
+// workgroups that the compute units hold at once
+int ce_want(int planes, int edge) { return planes == 3 || edge == 256 ? 256 : 512; }
+
 struct CePlan {
   int P;
   bool direct;           // W is read where it is
@@ -784,17 +803,9 @@ struct CePlan {
   int64_t piece, ldv;    // columns of a piece of the vocabulary, padded
   int pieces;
   int e_logits, e_dh, e_dw;         // tile edges
-  int dh_slots, dw_slots;           // stretches that the sums are cut into
+  CeCut dh_cut;                     // stretches that the sums are cut into
+  int dw_slots;
 };
-
-// how often a sum of k elements is cut for a grid of `tiles`: until the compute units hold as many workgroups as their LDS allows, 256 elements a stretch at least
-int ce_cuts(int planes, int edge, int64_t tiles, int64_t k) {
-  const int64_t want = planes == 3 || edge == 256 ? 256 : 512;
-  int64_t s = (want + tiles - 1) / tiles;
-  if (s > k / 256) s = k / 256;
-  if (s > 64) s = 64;
-  return (int)(s < 1 ? 1 : s);
-}
 
 CePlan ce_plan(int64_t T, int64_t H, int64_t V, int dtype, bool backward) {
   CePlan c;
@@ -815,10 +826,14 @@ CePlan ce_plan(int64_t T, int64_t H, int64_t V, int dtype, bool backward) {
   c.e_logits = ce_edge(c.P, cols, T, 1);
   const auto tiles = [&](int64_t a, int64_t b, int64_t e) { return ((a + e - 1) / e) * ((b + e - 1) / e); };
   c.e_dh = ce_edge(c.P, H, T, c.ldv / 1024 + 1);
-  c.dh_slots = ce_cuts(c.P, c.e_dh, tiles(H, T, c.e_dh), c.ldv);
+  c.dh_cut = CeCut{ce_want(c.P, c.e_dh), 0, INT64_MAX};
+  c.dh_cut.room = T * ce_slots(c.dh_cut, tiles(H, T, c.e_dh), T, c.ldv);
   c.e_dw = ce_edge(c.P, H, cols, T / 1024 + 1);
-  c.dw_slots = ce_cuts(c.P, c.e_dw, tiles(H, cols, c.e_dw), T);
-  if (tiles(H, cols, c.e_dw) >= 200) c.dw_slots = 1;
+  // a sum over few tokens is short, so that a last round of large tiles that leaves compute units idle weighs more than their better rate (1152 x 768 x 50257:
+  // 591 tiles of 256 in 3 rounds 131 us, 2358 of 128 in 5 half rounds 115 us)
+  const auto fill = [&](int64_t n, int64_t at_once) { return (double)n / (double)up(n, at_once); };
+  if (c.e_dw == 256 && T <= 2048 && fill(tiles(H, cols, 128), 512) > 1.15 * fill(tiles(H, cols, 256), 256)) c.e_dw = 128;
+  c.dw_slots = tiles(H, cols, c.e_dw) >= 200 ? 1 : ce_slots(CeCut{ce_want(c.P, c.e_dw), 0, INT64_MAX}, tiles(H, cols, c.e_dw), 1, T);
   return c;
 }
 
@@ -843,7 +858,7 @@ size_t ce_fwd_bytes(int64_t T, int64_t H, int64_t V, int dtype) {
 size_t ce_bwd_bytes(int64_t T, int64_t H, int64_t V, int dtype) {
   const CePlan c = ce_plan(T, H, V, dtype, true);
   return (c.direct ? ceeg_ws_part((size_t)PAD * c.Kp, 2) : ceeg_ws_part((size_t)c.P * c.piece * c.Kp, 2)) + ceeg_ws_part((size_t)c.P * c.Tp * c.ldv, 2) +
-         ceeg_ws_part((size_t)c.dh_slots * T * H, 4) + (c.dw_slots > 1 ? ceeg_ws_part((size_t)c.dw_slots * c.piece * H, 4) : 0) + ceeg_ws_part(1, 4) + ceeg_ws_part(T, 4);
+         ceeg_ws_part((size_t)c.dh_cut.room * H, 4) + (c.dw_slots > 1 ? ceeg_ws_part((size_t)c.dw_slots * c.piece * H, 4) : 0) + ceeg_ws_part(1, 4) + ceeg_ws_part(T, 4);
 }
 
 void ce_pack(int dtype, const void* src, int64_t ld, int64_t R, int64_t C, int64_t Cp, bool zeros, unsigned short* out, int64_t plane, hipStream_t st) {
@@ -960,7 +975,7 @@ extern "C" int ceeg_linear_ce_bwd(const void* packed, const void* W, int64_t ldw
   unsigned short* wc = c.direct ? nullptr : w.take<unsigned short>((size_t)c.P * c.piece * c.Kp);
   unsigned short* tail = c.direct ? w.take<unsigned short>((size_t)PAD * c.Kp) : nullptr;
   unsigned short* dl = w.take<unsigned short>((size_t)c.P * c.Tp * c.ldv);
-  float* dh_slots = w.take<float>((size_t)c.dh_slots * T * H);
+  float* dh_slots = w.take<float>((size_t)c.dh_cut.room * H);
   float* dw_slots = c.dw_slots > 1 ? w.take<float>((size_t)c.dw_slots * c.piece * H) : nullptr;
   float* top = w.take<float>(1);
   float* r = w.take<float>(T);
@@ -994,9 +1009,9 @@ extern "C" int ceeg_linear_ce_bwd(const void* packed, const void* W, int64_t ldw
         ce_pack(dtype, ce_at(W, (v0 + Wk.k_tail) * ldw, dtype), ldw, Vc % PAD, H, c.Kp, true, tail, 0, st);
         CEEG_CHECK_LAUNCH();
       }
-      const int all = tiles(H, c.e_dh) * tiles(T, c.e_dh);
+      const int all = tiles(H, c.e_dh) * tiles(T, c.e_dh), grid = all > c.dh_cut.want ? all : c.dh_cut.want;  // one stretch of every tile, or as many as are wanted
 #define CE_CALL(PL, E, WM, WN, TILE)                                                                                                                                              \
-  ce_slots_kernel<CE_TILE_OF(TILE), E, E, WM, WN><<<all * c.dh_slots, WM * WN * 64, 0, st>>>(Wk, dlm, n, 1, (int)H, T, (int)ldv, c.dh_slots, p > 0, dh_slots)
+  ce_slots_kernel<CE_TILE_OF(TILE), E, E, WM, WN><<<grid, WM * WN * 64, 0, st>>>(Wk, dlm, n, 1, (int)H, T, (int)ldv, (int)c.ldv, c.dh_cut, p > 0, dh_slots)
       CE_TILES(c.P, c.e_dh, true, false, CE_CALL);
 #undef CE_CALL
       CEEG_CHECK_LAUNCH();
@@ -1007,7 +1022,7 @@ extern "C" int ceeg_linear_ce_bwd(const void* packed, const void* W, int64_t ldw
       void* const to = const_cast<void*>(ce_at(dw, v0 * H, dtype));
       if (c.dw_slots > 1) {
 #define CE_CALL(PL, E, WM, WN, TILE)                                                                                                                                      \
-  ce_slots_kernel<CE_TILE_OF(TILE), E, E, WM, WN><<<all * c.dw_slots, WM * WN * 64, 0, st>>>(hk, dlk, n, 0, (int)H, Vc, 0, c.dw_slots, 0, dw_slots)
+  ce_slots_kernel<CE_TILE_OF(TILE), E, E, WM, WN><<<all * c.dw_slots, WM * WN * 64, 0, st>>>(hk, dlk, n, 0, (int)H, Vc, 0, 0, CeCut{0, c.dw_slots, 0}, 0, dw_slots)
         CE_TILES(c.P, c.e_dw, true, true, CE_CALL);
 #undef CE_CALL
         CEEG_CHECK_LAUNCH();
@@ -1023,8 +1038,8 @@ extern "C" int ceeg_linear_ce_bwd(const void* packed, const void* W, int64_t ldw
     }
   }
   if (dh) {
-    if (dtype == CEEG_F32) ce_dh_join_kernel<true><<<(unsigned)T, 256, 0, st>>>(dh_slots, c.dh_slots, n, pos, scale, T, (int)H, dh);
-    else ce_dh_join_kernel<false><<<(unsigned)T, 256, 0, st>>>(dh_slots, c.dh_slots, n, pos, scale, T, (int)H, dh);
+    if (dtype == CEEG_F32) ce_dh_join_kernel<true><<<(unsigned)T, 256, 0, st>>>(dh_slots, c.e_dh, (int)c.ldv, c.dh_cut, n, pos, scale, (int)H, dh);
+    else ce_dh_join_kernel<false><<<(unsigned)T, 256, 0, st>>>(dh_slots, c.e_dh, (int)c.ldv, c.dh_cut, n, pos, scale, (int)H, dh);
     CEEG_CHECK_LAUNCH();
   }
   return CEEG_OK;
