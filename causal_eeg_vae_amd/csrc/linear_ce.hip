@@ -47,54 +47,60 @@ struct CeTokens {
   float* zeros;
 };
 
-// All of them by one workgroup; `write`: into memory; `places` (LDS): pos, for up to CE_SCAN tokens.  Returns how many count.
+// All of them by one workgroup; `write`: into memory; `places` (LDS): pos, for up to CE_SCAN tokens.  Returns how many count.  4096 tokens a turn: every wave counts in
+// EACH stretches of 64 (loads and stores lane after lane), the 64 counts are summed up by one wave.
 template <int THREADS>
 __device__ __forceinline__ int ce_scan(const CeTokens& a, bool write, int32_t* places) {
-  constexpr int WAVES = THREADS / 64;
-  __shared__ int s_sum[WAVES];
+  constexpr int WAVES = THREADS / 64, EACH = 64 / WAVES;
+  __shared__ int s_sum[65];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int base = 0;
-  for (int64_t t0 = 0; t0 < a.T; t0 += THREADS * 4) {
-    const int64_t t = t0 + 4 * threadIdx.x;
-    int64_t v[4];
-    int mine = 0;
+  for (int64_t t0 = 0; t0 < a.T; t0 += 4096) {
+    int64_t v[EACH];
+    uint64_t on[EACH];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[k] = t + k < a.T ? a.y[t + k] : a.ignore;
-      mine += v[k] != a.ignore;
+    for (int k = 0; k < EACH; ++k) {
+      const int64_t t = t0 + k * THREADS + threadIdx.x;
+      v[k] = a.ignore;
+      if (t0 + k * THREADS < a.T && t < a.T) v[k] = a.y[t];
     }
-    int pre = mine;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(pre, o, 64);
-      if (lane >= o) pre += u;
+    for (int k = 0; k < EACH; ++k) {
+      on[k] = __ballot(v[k] != a.ignore);
+      if (lane == 0) s_sum[k * WAVES + wave] = __popcll(on[k]);
     }
-    if (lane == 63) s_sum[wave] = pre;
     __syncthreads();
-    int before = 0, all = 0;
+    if (wave == 0) {
+      const int mine = s_sum[lane];
+      int pre = mine;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      before += w < wave ? s_sum[w] : 0;
-      all += s_sum[w];
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(pre, o, 64);
+        if (lane >= o) pre += u;
+      }
+      s_sum[lane] = pre - mine;
+      if (lane == 63) s_sum[64] = pre;
     }
-    int j = base + before + pre - mine;
+    __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (t + k >= a.T) continue;
-      const bool on = v[k] != a.ignore;
-      if (places) places[t + k] = on ? j : -1;
+    for (int k = 0; k < EACH; ++k) {
+      const int64_t t = t0 + k * THREADS + threadIdx.x;
+      if (t0 + k * THREADS >= a.T) break;
+      const bool counts = on[k] >> lane & 1;
+      const int j = base + s_sum[k * WAVES + wave] + __popcll(on[k] & ((1ull << lane) - 1));
+      if (t >= a.T) continue;
+      if (places) places[t] = counts ? j : -1;
       if (write) {
-        a.pos[t + k] = on ? j : -1;
-        if (on) {
-          a.rows[j] = (int32_t)(t + k);
+        a.pos[t] = counts ? j : -1;
+        if (counts) {
+          a.rows[j] = (int32_t)t;
           a.yc[j] = v[k] >= 0 && v[k] < a.V ? (int32_t)v[k] : -1;
         } else if (a.zeros) {
-          a.zeros[t + k] = 0.f;
+          a.zeros[t] = 0.f;
         }
       }
-      j += on;
     }
-    base += all;
+    base += s_sum[64];
     __syncthreads();
   }
   if (write && threadIdx.x == 0) a.n[0] = base;
@@ -765,21 +771,36 @@ __global__ __launch_bounds__(256) void ce_dw_join_kernel(const float* __restrict
   else static_cast<unsigned short*>(dw)[i] = ceeg_f32_to_bf16(x);
 }
 
+// the slots of dh joined, four columns a thread, eight slots in flight; rows of tokens that do not count are zero
 template <bool F32>
 __global__ __launch_bounds__(256) void ce_dh_join_kernel(const float* __restrict__ part, int edge, int k_all, CeCut cut, const int32_t* __restrict__ n, const int32_t* __restrict__ pos,
-                                                         CeScale scale, int H, void* __restrict__ dh) {
-  const int64_t t = blockIdx.x;
-  const int N = n[0], j = pos[t], slots = ce_slots(cut, (int64_t)((H + edge - 1) / edge) * ((N + edge - 1) / edge), N, k_all);
-  const float s = scale.s(N);
-  for (int c = threadIdx.x; c < H; c += 256) {
-    float x = 0.f;
-    if (j >= 0) {
-      for (int k = 0; k < slots; ++k) x += part[((int64_t)k * N + j) * H + c];
-      x *= s;
+                                                         CeScale scale, int64_t T, int H, void* __restrict__ dh) {
+  const int per = (H + 3) / 4;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, t = id / per;
+  if (t >= T) return;
+  const int N = n[0], j = pos[t], c = (int)(id - t * per) * 4;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  if (j >= 0) {
+    const int slots = ce_slots(cut, (int64_t)((H + edge - 1) / edge) * ((N + edge - 1) / edge), N, k_all);
+    const float* const from = part + (int64_t)j * H + c;
+    for (int k0 = 0; k0 < slots; k0 += 8) {
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float* const f = from + (int64_t)(k0 + k) * N * H;
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k0 + k >= slots) continue;
+        if ((H & 3) == 0) v[k] = *reinterpret_cast<const float4*>(f);
+        else v[k] = make_float4(f[0], c + 1 < H ? f[1] : 0.f, c + 2 < H ? f[2] : 0.f, c + 3 < H ? f[3] : 0.f);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) { x[0] += v[k].x; x[1] += v[k].y; x[2] += v[k].z; x[3] += v[k].w; }
     }
-    if (F32) static_cast<float*>(dh)[t * H + c] = x;
-    else static_cast<unsigned short*>(dh)[t * H + c] = ceeg_f32_to_bf16(x);
+    const float s = scale.s(N);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] *= s;
   }
+  ce_store4<F32>(dh, t * H + c, H - c, H, x[0], x[1], x[2], x[3]);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -1038,8 +1059,9 @@ extern "C" int ceeg_linear_ce_bwd(const void* packed, const void* W, int64_t ldw
     }
   }
   if (dh) {
-    if (dtype == CEEG_F32) ce_dh_join_kernel<true><<<(unsigned)T, 256, 0, st>>>(dh_slots, c.e_dh, (int)c.ldv, c.dh_cut, n, pos, scale, (int)H, dh);
-    else ce_dh_join_kernel<false><<<(unsigned)T, 256, 0, st>>>(dh_slots, c.e_dh, (int)c.ldv, c.dh_cut, n, pos, scale, (int)H, dh);
+    const unsigned grid = (unsigned)((T * ((H + 3) / 4) + 255) / 256);
+    if (dtype == CEEG_F32) ce_dh_join_kernel<true><<<grid, 256, 0, st>>>(dh_slots, c.e_dh, (int)c.ldv, c.dh_cut, n, pos, scale, T, (int)H, dh);
+    else ce_dh_join_kernel<false><<<grid, 256, 0, st>>>(dh_slots, c.e_dh, (int)c.ldv, c.dh_cut, n, pos, scale, T, (int)H, dh);
     CEEG_CHECK_LAUNCH();
   }
   return CEEG_OK;
