@@ -404,9 +404,9 @@ struct CeTile {
 // smaller grids; 64 x 64 spreads the smallest, which are bound by latency, and keeps more tiles on their way.
 template <int PL, bool TA, bool TB> struct CeBig { using Tile = CeTile<1, 256, 256, 2, 4, 4, true, TA, TB>; };
 template <int PL, bool TA, bool TB> struct CeMid { using Tile = CeTile<1, 128, 128, 2, 2, 4, true, TA, TB>; };
-template <bool TA, bool TB> struct CeMid<3, TA, TB> { using Tile = CeTile<3, 128, 128, 4, 2, 3, false, TA, TB>; };
+template <bool TA, bool TB> struct CeMid<3, TA, TB> { using Tile = CeTile<3, 128, 64, 2, 2, 2, false, TA, TB>; };
 template <int PL, bool TA, bool TB> struct CeSmall { using Tile = CeTile<1, 64, 64, 2, 2, 8, true, TA, TB>; };
-template <bool TA, bool TB> struct CeSmall<3, TA, TB> { using Tile = CeTile<3, 64, 64, 2, 2, 4, false, TA, TB>; };
+template <bool TA, bool TB> struct CeSmall<3, TA, TB> { using Tile = CeTile<3, 64, 64, 2, 2, 3, false, TA, TB>; };
 
 // exp(x - base).  bf16: one fused multiply-add in front of the instruction, whose rounding of base * log2(e) is worth 2^-24 |base| of the result; fp32: the difference first.
 template <int PL>
@@ -430,6 +430,13 @@ __device__ __forceinline__ void ce_store4(void* to, int64_t at, int left, int H,
     if (F32) static_cast<float*>(to)[at + k] = x[k];
     else static_cast<unsigned short*>(to)[at + k] = ceeg_f32_to_bf16(x[k]);
   }
+}
+
+// Edge along n of the tile with this edge along m
+__host__ __device__ __forceinline__ int ce_n(int planes, int edge) { return planes == 3 ? 64 : edge; }
+__host__ __device__ __forceinline__ int64_t ce_tiles(int planes, int edge, int64_t m, int64_t n) {
+  const int en = ce_n(planes, edge);
+  return ((m + edge - 1) / edge) * ((n + en - 1) / en);
 }
 
 // Workgroups go to the eight XCDs in turn: each XCD gets a run of consecutive tiles (-1: none left for this workgroup) ...
@@ -773,7 +780,7 @@ __global__ __launch_bounds__(256) void ce_dw_join_kernel(const float* __restrict
 
 // the slots of dh joined, four columns a thread, eight slots in flight; rows of tokens that do not count are zero
 template <bool F32>
-__global__ __launch_bounds__(256) void ce_dh_join_kernel(const float* __restrict__ part, int edge, int k_all, CeCut cut, const int32_t* __restrict__ n, const int32_t* __restrict__ pos,
+__global__ __launch_bounds__(256) void ce_dh_join_kernel(const float* __restrict__ part, int planes, int edge, int k_all, CeCut cut, const int32_t* __restrict__ n, const int32_t* __restrict__ pos,
                                                          CeScale scale, int64_t T, int H, void* __restrict__ dh) {
   const int per = (H + 3) / 4;
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, t = id / per;
@@ -781,7 +788,7 @@ __global__ __launch_bounds__(256) void ce_dh_join_kernel(const float* __restrict
   const int N = n[0], j = pos[t], c = (int)(id - t * per) * 4;
   float x[4] = {0.f, 0.f, 0.f, 0.f};
   if (j >= 0) {
-    const int slots = ce_slots(cut, (int64_t)((H + edge - 1) / edge) * ((N + edge - 1) / edge), N, k_all);
+    const int slots = ce_slots(cut, ce_tiles(planes, edge, H, N), N, k_all);
     const float* const from = part + (int64_t)j * H + c;
     for (int k0 = 0; k0 < slots; k0 += 8) {
       float4 v[8];
@@ -808,14 +815,14 @@ constexpr int TMIN = 64;  // the smallest tile: what is counted in tiles is size
 
 // Tile edge for a grid of rows x columns (x the ways its sum may be cut): the largest that gives every compute unit a workgroup
 int ce_edge(int planes, int64_t rows, int64_t cols, int64_t cuts) {
-  const auto tiles = [&](int64_t e) { return ((rows + e - 1) / e) * ((cols + e - 1) / e); };
+  const auto tiles = [&](int e) { return ce_tiles(planes, e, rows, cols); };
   if (planes == 1 && tiles(256) * cuts >= 200) return 256;
   if (tiles(128) * cuts >= 200) return 128;
   return 64;
 }
 
 // workgroups that the compute units hold at once
-int ce_want(int planes, int edge) { return planes == 3 || edge == 256 ? 256 : 512; }
+int ce_want(int edge) { return edge == 256 ? 256 : 512; }
 
 struct CePlan {
   int P;
@@ -845,16 +852,16 @@ CePlan ce_plan(int64_t T, int64_t H, int64_t V, int dtype, bool backward) {
   c.ldv = up(c.piece < V ? c.piece : V, PAD);
   const int64_t cols = c.piece < V ? c.piece : V;
   c.e_logits = ce_edge(c.P, cols, T, 1);
-  const auto tiles = [&](int64_t a, int64_t b, int64_t e) { return ((a + e - 1) / e) * ((b + e - 1) / e); };
+  const auto tiles = [&](int64_t m, int64_t n, int e) { return ce_tiles(c.P, e, m, n); };
   c.e_dh = ce_edge(c.P, H, T, c.ldv / 1024 + 1);
-  c.dh_cut = CeCut{ce_want(c.P, c.e_dh), 0, INT64_MAX};
+  c.dh_cut = CeCut{ce_want(c.e_dh), 0, INT64_MAX};
   c.dh_cut.room = T * ce_slots(c.dh_cut, tiles(H, T, c.e_dh), T, c.ldv);
   c.e_dw = ce_edge(c.P, H, cols, T / 1024 + 1);
   // a sum over few tokens is short, so that a last round of large tiles that leaves compute units idle weighs more than their better rate (1152 x 768 x 50257:
   // 591 tiles of 256 in 3 rounds 131 us, 2358 of 128 in 5 half rounds 115 us)
   const auto fill = [&](int64_t n, int64_t at_once) { return (double)n / (double)up(n, at_once); };
   if (c.e_dw == 256 && T <= 2048 && fill(tiles(H, cols, 128), 512) > 1.15 * fill(tiles(H, cols, 256), 256)) c.e_dw = 128;
-  c.dw_slots = tiles(H, cols, c.e_dw) >= 200 ? 1 : ce_slots(CeCut{ce_want(c.P, c.e_dw), 0, INT64_MAX}, tiles(H, cols, c.e_dw), 1, T);
+  c.dw_slots = tiles(H, cols, c.e_dw) >= 200 ? 1 : ce_slots(CeCut{ce_want(c.e_dw), 0, INT64_MAX}, tiles(H, cols, c.e_dw), 1, T);
   return c;
 }
 
@@ -889,17 +896,17 @@ void ce_pack(int dtype, const void* src, int64_t ld, int64_t R, int64_t C, int64
 }
 inline const void* ce_at(const void* p, int64_t n, int dtype) { return static_cast<const char*>(p) + n * (dtype == CEEG_F32 ? 4 : 2); }
 
-// CALL with (tile, edge in classes, edge in tokens, waves in each): the planes and the edge chosen
-#define CE_TILES(PLANES, EDGE, TA, TB, CALL)                                    \
-  do {                                                                          \
-    if ((PLANES) == 3) {                                                        \
-      if ((EDGE) == 128) { CALL(3, 128, 4, 2, (CeMid<3, TA, TB>::Tile)); }      \
-      else { CALL(3, 64, 2, 2, (CeSmall<3, TA, TB>::Tile)); }                   \
-    } else {                                                                    \
-      if ((EDGE) == 256) { CALL(1, 256, 2, 4, (CeBig<1, TA, TB>::Tile)); }      \
-      else if ((EDGE) == 128) { CALL(1, 128, 2, 2, (CeMid<1, TA, TB>::Tile)); } \
-      else { CALL(1, 64, 2, 2, (CeSmall<1, TA, TB>::Tile)); }                   \
-    }                                                                           \
+// CALL with (planes, edges along m and n, waves along each, tile type) of the edge chosen
+#define CE_TILES(PLANES, EDGE, TA, TB, CALL)                                         \
+  do {                                                                               \
+    if ((PLANES) == 3) {                                                             \
+      if ((EDGE) == 128) { CALL(3, 128, 64, 2, 2, (CeMid<3, TA, TB>::Tile)); }       \
+      else { CALL(3, 64, 64, 2, 2, (CeSmall<3, TA, TB>::Tile)); }                    \
+    } else {                                                                         \
+      if ((EDGE) == 256) { CALL(1, 256, 256, 2, 4, (CeBig<1, TA, TB>::Tile)); }      \
+      else if ((EDGE) == 128) { CALL(1, 128, 128, 2, 2, (CeMid<1, TA, TB>::Tile)); } \
+      else { CALL(1, 64, 64, 2, 2, (CeSmall<1, TA, TB>::Tile)); }                    \
+    }                                                                                \
   } while (0)
 template <class> struct CeArg;
 template <class X> struct CeArg<void(X)> { using type = X; };
@@ -951,7 +958,6 @@ extern "C" int ceeg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int
     else ce_prepare_kernel<false, false><<<grid, 256, 0, st>>>(tk, h, ldh, (int)H, (int)c.Kp, each, hc, c.Tp * c.Kp);
   }
   CEEG_CHECK_LAUNCH();
-  const int e = c.e_logits, tiles_n = (int)((T + e - 1) / e);
   const CeMat Bm{hc, c.Kp, c.Tp * c.Kp, 0, nullptr, INT_MAX};
   for (int p = 0; p < c.pieces; ++p) {
     const int64_t v0 = p * c.piece, Vc = V - v0 < c.piece ? V - v0 : c.piece;
@@ -961,10 +967,10 @@ extern "C" int ceeg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int
       CEEG_CHECK_LAUNCH();
       A = CeMat{wc, c.Kp, c.piece * c.Kp, (int)Vc, nullptr, INT_MAX};
     }
-    const int tiles_m = (int)((Vc + e - 1) / e);
-#define CE_CALL(PL, E, WM, WN, TILE) \
-  ce_stats_kernel<CE_TILE_OF(TILE), PL, E, E, WM, WN><<<tiles_m * tiles_n, WM * WN * 64, 0, st>>>(A, Bm, n, yc, (int)v0, (int)c.Kp, (int)(v0 / E), parts, part, at_y)
-    CE_TILES(c.P, e, false, false, CE_CALL);
+    const unsigned grid = (unsigned)ce_tiles(c.P, c.e_logits, Vc, T);
+#define CE_CALL(PL, BM, BN, WM, WN, TILE) \
+  ce_stats_kernel<CE_TILE_OF(TILE), PL, BM, BN, WM, WN><<<grid, WM * WN * 64, 0, st>>>(A, Bm, n, yc, (int)v0, (int)c.Kp, (int)(v0 / BM), parts, part, at_y)
+    CE_TILES(c.P, c.e_logits, false, false, CE_CALL);
 #undef CE_CALL
     CEEG_CHECK_LAUNCH();
   }
@@ -1008,7 +1014,6 @@ extern "C" int ceeg_linear_ce_bwd(const void* packed, const void* W, int64_t ldw
     ce_scale_kernel<<<1, 1024, 0, st>>>(n, rows, g, top, r);
     CEEG_CHECK_LAUNCH();
   }
-  const auto tiles = [](int64_t x, int e) { return (int)((x + e - 1) / e); };
   const CeMat hm{hc, c.Kp, c.Tp * c.Kp, 0, nullptr, INT_MAX}, hk{hc, c.Kp, c.Tp * c.Kp, (int)c.Kp, nullptr, INT_MAX};
   for (int p = 0; p < c.pieces; ++p) {
     const int64_t v0 = p * c.piece, Vc = V - v0 < c.piece ? V - v0 : c.piece, ldv = up(Vc, PAD), plane = c.Tp * c.ldv;
@@ -1018,9 +1023,9 @@ extern "C" int ceeg_linear_ce_bwd(const void* packed, const void* W, int64_t ldw
       CEEG_CHECK_LAUNCH();
       A = CeMat{wc, c.Kp, c.piece * c.Kp, (int)Vc, nullptr, INT_MAX};
     }
-    const int tiles_t = tiles(T, c.e_logits), tiles_v = tiles(ldv, c.e_logits);
-#define CE_CALL(PL, E, WM, WN, TILE)                                                                                                                                     \
-  ce_dlogits_kernel<CE_TILE_OF(TILE), PL, E, E, WM, WN><<<tiles_v * tiles_t, WM * WN * 64, 0, st>>>(A, hm, n, yc, lse, scale, (int)v0, (int)ldv, plane, (int)c.Kp, dl)
+    const unsigned grid_l = (unsigned)ce_tiles(c.P, c.e_logits, ldv, T);
+#define CE_CALL(PL, BM, BN, WM, WN, TILE)                                                                                                                                     \
+  ce_dlogits_kernel<CE_TILE_OF(TILE), PL, BM, BN, WM, WN><<<grid_l, WM * WN * 64, 0, st>>>(A, hm, n, yc, lse, scale, (int)v0, (int)ldv, plane, (int)c.Kp, dl)
     CE_TILES(c.P, c.e_logits, false, false, CE_CALL);
 #undef CE_CALL
     CEEG_CHECK_LAUNCH();
@@ -1030,20 +1035,20 @@ extern "C" int ceeg_linear_ce_bwd(const void* packed, const void* W, int64_t ldw
         ce_pack(dtype, ce_at(W, (v0 + Wk.k_tail) * ldw, dtype), ldw, Vc % PAD, H, c.Kp, true, tail, 0, st);
         CEEG_CHECK_LAUNCH();
       }
-      const int all = tiles(H, c.e_dh) * tiles(T, c.e_dh), grid = all > c.dh_cut.want ? all : c.dh_cut.want;  // one stretch of every tile, or as many as are wanted
-#define CE_CALL(PL, E, WM, WN, TILE)                                                                                                                                              \
-  ce_slots_kernel<CE_TILE_OF(TILE), E, E, WM, WN><<<grid, WM * WN * 64, 0, st>>>(Wk, dlm, n, 1, (int)H, T, (int)ldv, (int)c.ldv, c.dh_cut, p > 0, dh_slots)
+      const int all = (int)ce_tiles(c.P, c.e_dh, H, T), grid = all > c.dh_cut.want ? all : c.dh_cut.want;  // one stretch of every tile, or as many as are wanted
+#define CE_CALL(PL, BM, BN, WM, WN, TILE)                                                                                                                                              \
+  ce_slots_kernel<CE_TILE_OF(TILE), BM, BN, WM, WN><<<grid, WM * WN * 64, 0, st>>>(Wk, dlm, n, 1, (int)H, T, (int)ldv, (int)c.ldv, c.dh_cut, p > 0, dh_slots)
       CE_TILES(c.P, c.e_dh, true, false, CE_CALL);
 #undef CE_CALL
       CEEG_CHECK_LAUNCH();
     }
     if (dw) {
       const CeMat dlk{dl, ldv, plane, (int)ldv, nullptr, INT_MAX};
-      const int all = tiles(H, c.e_dw) * tiles(Vc, c.e_dw);
+      const int all = (int)ce_tiles(c.P, c.e_dw, H, Vc);
       void* const to = const_cast<void*>(ce_at(dw, v0 * H, dtype));
       if (c.dw_slots > 1) {
-#define CE_CALL(PL, E, WM, WN, TILE)                                                                                                                                      \
-  ce_slots_kernel<CE_TILE_OF(TILE), E, E, WM, WN><<<all * c.dw_slots, WM * WN * 64, 0, st>>>(hk, dlk, n, 0, (int)H, Vc, 0, 0, CeCut{0, c.dw_slots, 0}, 0, dw_slots)
+#define CE_CALL(PL, BM, BN, WM, WN, TILE)                                                                                                                                      \
+  ce_slots_kernel<CE_TILE_OF(TILE), BM, BN, WM, WN><<<all * c.dw_slots, WM * WN * 64, 0, st>>>(hk, dlk, n, 0, (int)H, Vc, 0, 0, CeCut{0, c.dw_slots, 0}, 0, dw_slots)
         CE_TILES(c.P, c.e_dw, true, true, CE_CALL);
 #undef CE_CALL
         CEEG_CHECK_LAUNCH();
@@ -1051,7 +1056,7 @@ extern "C" int ceeg_linear_ce_bwd(const void* packed, const void* W, int64_t ldw
         if (dtype == CEEG_F32) ce_dw_join_kernel<true><<<grid, 256, 0, st>>>(dw_slots, c.dw_slots, n, scale, Vc * H, to);
         else ce_dw_join_kernel<false><<<grid, 256, 0, st>>>(dw_slots, c.dw_slots, n, scale, Vc * H, to);
       } else {
-#define CE_CALL(PL, E, WM, WN, TILE) ce_dw_kernel<CE_TILE_OF(TILE), PL == 3, E, E, WM, WN><<<all, WM * WN * 64, 0, st>>>(hk, dlk, n, scale, (int)H, (int)Vc, to)
+#define CE_CALL(PL, BM, BN, WM, WN, TILE) ce_dw_kernel<CE_TILE_OF(TILE), PL == 3, BM, BN, WM, WN><<<all, WM * WN * 64, 0, st>>>(hk, dlk, n, scale, (int)H, (int)Vc, to)
         CE_TILES(c.P, c.e_dw, true, true, CE_CALL);
 #undef CE_CALL
       }
@@ -1060,8 +1065,8 @@ extern "C" int ceeg_linear_ce_bwd(const void* packed, const void* W, int64_t ldw
   }
   if (dh) {
     const unsigned grid = (unsigned)((T * ((H + 3) / 4) + 255) / 256);
-    if (dtype == CEEG_F32) ce_dh_join_kernel<true><<<grid, 256, 0, st>>>(dh_slots, c.e_dh, (int)c.ldv, c.dh_cut, n, pos, scale, T, (int)H, dh);
-    else ce_dh_join_kernel<false><<<grid, 256, 0, st>>>(dh_slots, c.e_dh, (int)c.ldv, c.dh_cut, n, pos, scale, T, (int)H, dh);
+    if (dtype == CEEG_F32) ce_dh_join_kernel<true><<<grid, 256, 0, st>>>(dh_slots, c.P, c.e_dh, (int)c.ldv, c.dh_cut, n, pos, scale, T, (int)H, dh);
+    else ce_dh_join_kernel<false><<<grid, 256, 0, st>>>(dh_slots, c.P, c.e_dh, (int)c.ldv, c.dh_cut, n, pos, scale, T, (int)H, dh);
     CEEG_CHECK_LAUNCH();
   }
   return CEEG_OK;
