@@ -811,8 +811,6 @@ __global__ __launch_bounds__(256) void ce_dh_join_kernel(const float* __restrict
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-constexpr int TMIN = 64;  // the smallest tile: what is counted in tiles is sized for it
-
 // Tile edge for a grid of rows x columns (x the ways its sum may be cut): the largest that gives every compute unit a workgroup
 int ce_edge(int planes, int64_t rows, int64_t cols, int64_t cuts) {
   const auto tiles = [&](int e) { return ce_tiles(planes, e, rows, cols); };
@@ -880,7 +878,7 @@ int ce_check(const void* h, int64_t ldh, const void* W, int64_t ldw, int64_t T, 
 size_t ce_packed_bytes(const CePlan& c) { return ceeg_ws_part((size_t)c.P * c.Tp * c.Kp, 2); }
 size_t ce_fwd_bytes(int64_t T, int64_t H, int64_t V, int dtype) {
   const CePlan c = ce_plan(T, H, V, dtype, false);
-  const size_t parts = (size_t)(V + TMIN - 1) / TMIN;
+  const size_t parts = (size_t)(V + c.e_logits - 1) / c.e_logits;
   return (c.direct ? 0 : ceeg_ws_part((size_t)c.P * c.piece * c.Kp, 2)) + ceeg_ws_part((size_t)T * parts, 8) + 2 * ceeg_ws_part(T, 4);
 }
 size_t ce_bwd_bytes(int64_t T, int64_t H, int64_t V, int dtype) {

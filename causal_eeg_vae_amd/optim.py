@@ -97,6 +97,8 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9,
     step_t, lr_t = _scalar(step, "step", dev), _scalar(lr, "lr", dev)
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and (step_t is not None or step >= 1)):
         raise ValueError(f"betas in [0, 1), eps >= 0 and step >= 1 expected, got {betas}, {eps} and {step}")
+    if step_t is None and torch.cuda.is_current_stream_capturing():
+        raise ValueError("a captured step needs its number as a tensor on the device: an int would be the same at every replay")
     # host arrays of addresses, alive for the call
     lists = [array.array("q", sizes)] + [array.array("Q", x) for x in (pp, _addresses(grads), mp, vp, sp[:n], sp[n:])]
     sizes_at, p_at, g_at, m_at, v_at, ms_at, vs_at = (x.buffer_info()[0] for x in lists)
@@ -155,6 +157,8 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 st = self.state[p]
                 if not st:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("AdamW: take a step before capturing one: moments made inside a graph would start anew at every replay")
                     st.update(self._new_state(p, group))
                 lists.setdefault((p.dtype, p.device, isinstance(st["exp_avg"], tuple)), []).append(p)
             if not lists:

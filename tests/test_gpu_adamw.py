@@ -312,6 +312,37 @@ def test_step_captured_into_a_graph(bits):
             assert torch.equal(x, y), k
 
 
+def test_captures_that_would_replay_wrongly_are_refused():
+    from causal_eeg_vae_amd import AdamW, adamw_step_
+    p = [torch.ones(10, device="cuda")]
+    x = [torch.zeros(10, device="cuda") for _ in range(3)]
+    model = _model()
+    for q in model.parameters():
+        q.grad = torch.zeros_like(q)
+    opt = AdamW(model.parameters(), capturable=True)
+    for error, call in ((ValueError, lambda: adamw_step_(p, x[:1], x[1:2], x[2:], step=3)), (RuntimeError, opt.step)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            p[0].mul_(1.0)
+            with pytest.raises(error):
+                call()
+    assert torch.equal(p[0], torch.ones(10, device="cuda"))
+
+
+def test_on_another_stream():
+    from causal_eeg_vae_amd import adamw_step_
+    a, b = _tensors([70001, 300], torch.float32, seed=4), _tensors([70001, 300], torch.float32, seed=4)
+    adamw_step_(*a, **HYPER)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        b[1][0].mul_(1.0)        # the step follows what its own stream holds
+        adamw_step_(*b, **HYPER)
+    s.synchronize()
+    for x, y in zip(a, b):
+        assert all(torch.equal(s, t) for s, t in zip(x, y))
+
+
 def test_capturable_equals_plain():
     """The count on the device and the count on the host give the same stream of random numbers; the factors differ by a rounding."""
     from causal_eeg_vae_amd import AdamW
