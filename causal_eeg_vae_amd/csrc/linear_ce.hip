@@ -520,19 +520,39 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_stats_kernel(CeMat W, CeMat 
   }
 }
 
-// A wave joins the pieces' maxima and sums of token j
-__device__ __forceinline__ float ce_join(const float2* __restrict__ part, int64_t j, int parts, int lane) {
-  float top = -INFINITY;
-  for (int c = lane; c < parts; c += 64) top = fmaxf(top, part[j * parts + c].x);
+// A wave joins the pieces' maxima and sums of R tokens j, j + step, ... (below N): one pass, the loads of eight pieces of every token in flight
+template <int R>
+__device__ __forceinline__ void ce_join(const float2* __restrict__ part, int64_t j, int64_t step, int64_t N, int parts, int lane, float (&lse)[R]) {
+  float top[R], sum[R];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-  const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  for (int c = lane; c < parts; c += 64) {
-    const float2 u = part[j * parts + c];
-    sum += u.y * __expf(u.x - base);
+  for (int r = 0; r < R; ++r) { top[r] = -INFINITY; sum[r] = 0.f; }
+  for (int c0 = lane; c0 < parts; c0 += 8 / R * 64) {
+    float2 u[R][8 / R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int k = 0; k < 8 / R; ++k)
+        u[r][k] = j + r * step < N && c0 + 64 * k < parts ? part[(j + r * step) * parts + c0 + 64 * k] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float t = top[r];
+#pragma unroll
+      for (int k = 0; k < 8 / R; ++k) t = fmaxf(t, u[r][k].x);
+      const float base = t == -INFINITY ? 0.f : t;
+      sum[r] *= __expf(top[r] - base);
+#pragma unroll
+      for (int k = 0; k < 8 / R; ++k) sum[r] += u[r][k].y * __expf(u[r][k].x - base);
+      top[r] = t;
+    }
   }
-  return base + logf(ceeg_wave_sum(sum));
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float t = top[r];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o, 64));
+    const float base = t == -INFINITY ? 0.f : t;
+    lse[r] = base + logf(ceeg_wave_sum(sum[r] * __expf(top[r] - base)));
+  }
 }
 // a class outside [0, V) cannot raise an error from here: its loss is NaN
 __device__ __forceinline__ float ce_row_loss(float lse, const float* __restrict__ at_y, const int32_t* __restrict__ yc, int64_t j) {
@@ -545,10 +565,11 @@ __global__ __launch_bounds__(256) void ce_lse_kernel(const int32_t* __restrict__
   const int lane = threadIdx.x & 63;
   const int64_t j = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (j >= n[0]) return;
-  const float l = ce_join(part, j, parts, lane);
+  float l[1];
+  ce_join<1>(part, j, 1, n[0], parts, lane, l);
   if (lane == 0) {
-    lse[j] = l;
-    rowloss[rows ? rows[j] : j] = ce_row_loss(l, at_y, yc, j);
+    lse[j] = l[0];
+    rowloss[rows ? rows[j] : j] = ce_row_loss(l[0], at_y, yc, j);
   }
 }
 
@@ -560,11 +581,15 @@ __global__ __launch_bounds__(1024) void ce_loss_kernel(const int32_t* __restrict
   const int N = n[0], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   double v = 0.0;
   if (JOIN) {
-    for (int j = wave; j < N; j += 16) {
-      const float l = ce_join(part, j, parts, lane);
-      if (lane == 0) {
-        lse[j] = l;
-        v += (double)ce_row_loss(l, at_y, yc, j);
+    for (int j = wave; j < N; j += 128) {
+      float l[8];
+      ce_join<8>(part, j, 16, N, parts, lane, l);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        if (lane == r && j + 16 * r < N) {
+          lse[j + 16 * r] = l[r];
+          v += (double)ce_row_loss(l[r], at_y, yc, j + 16 * r);
+        }
       }
     }
   } else {

@@ -18,7 +18,7 @@ def _dtype(t, what):
 
 def _same_device(*tensors):
     _lib.require_cuda(*tensors)
-    if len({t.device for t in tensors if t is not None}) > 1:
+    if len({t.get_device() for t in tensors if t is not None}) > 1:
         raise ValueError(f"all tensors must be on one device, got {[str(t.device) for t in tensors if t is not None]}")
 
 
@@ -37,34 +37,37 @@ class _LinearCrossEntropy(torch.autograd.Function):
         ldh, ldw = max(hidden.stride(0), H), H if weight.is_contiguous() else weight.stride(0)
         with _lib.on(dev):
             loss = torch.empty(T if reduction == 0 else 1, dtype=torch.float32, device=dev)
-            lse = torch.empty(T, dtype=torch.float32, device=dev)
-            tokens = torch.empty(3 * T + 1, dtype=torch.int32, device=dev)
-            packed = _lib.workspace(L.ceeg_linear_ce_packed_bytes(T, H, dtype), dev)
+            # one buffer for what the backward takes back: the packed rows, lse [T], tokens [3 T + 1]
+            rows = L.ceeg_linear_ce_packed_bytes(T, H, dtype)
+            kept = _lib.workspace(rows + 16 * T + 4, dev)
+            packed = kept.data_ptr()
+            lse, tokens = packed + rows, packed + rows + 4 * T
             ws = _lib.workspace(L.ceeg_linear_ce_fwd_ws_bytes(T, H, V, dtype), dev)
             with _lib.timed("linear_ce_fwd"):
                 _lib.check(L.ceeg_linear_ce_fwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, target.data_ptr(), T, H, V, dtype, ignore_index, reduction,
-                                                loss.data_ptr(), lse.data_ptr(), tokens.data_ptr(), packed.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream()),
+                                                loss.data_ptr(), lse, tokens, packed, ws.data_ptr(), ws.numel(), _lib.stream()),
                            "ceeg_linear_ce_fwd")
-        ctx.save_for_backward(packed, weight, lse, tokens)
-        ctx.sizes = T, H, V, ldw, dtype, reduction, hidden.dtype
+        ctx.save_for_backward(kept, weight)
+        ctx.sizes = T, H, V, ldw, dtype, reduction, rows
         return loss if reduction == 0 else loss[0]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        packed, weight, lse, tokens = ctx.saved_tensors
-        T, H, V, ldw, dtype, reduction, hidden_dtype = ctx.sizes
+        kept, weight = ctx.saved_tensors
+        T, H, V, ldw, dtype, reduction, rows = ctx.sizes
         L = _lib.lib()
         dev = weight.device
         need_h, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         with _lib.on(dev):
             g = g.to(torch.float32).contiguous()
-            dh = torch.empty(T, H, dtype=hidden_dtype, device=dev) if need_h else None
+            packed = kept.data_ptr()
+            dh = torch.empty(T, H, dtype=weight.dtype, device=dev) if need_h else None
             dw = torch.empty(V, H, dtype=weight.dtype, device=dev) if need_w else None
             ws = _lib.workspace(L.ceeg_linear_ce_bwd_ws_bytes(T, H, V, dtype), dev)
             with _lib.timed("linear_ce_bwd"):
-                _lib.check(L.ceeg_linear_ce_bwd(packed.data_ptr(), weight.data_ptr(), ldw, T, H, V, dtype, reduction, g.data_ptr(), lse.data_ptr(),
-                                                tokens.data_ptr(), _lib.ptr(dh), _lib.ptr(dw), ws.data_ptr(), ws.numel(), _lib.stream()),
+                _lib.check(L.ceeg_linear_ce_bwd(packed, weight.data_ptr(), ldw, T, H, V, dtype, reduction, g.data_ptr(), packed + rows,
+                                                packed + rows + 4 * T, _lib.ptr(dh), _lib.ptr(dw), ws.data_ptr(), ws.numel(), _lib.stream()),
                            "ceeg_linear_ce_bwd")
         return dh, dw, None, None, None
 
