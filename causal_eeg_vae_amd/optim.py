@@ -107,6 +107,7 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9,
             n, sizes_at, p_at, g_at, m_at, v_at, ms_at if held else None, vs_at if held else None, _DTYPES[dtype], 8 if held else 32,
             0.0 if lr_t is not None else float(lr), float(b1), float(b2), float(eps), float(weight_decay), 1 if step_t is not None else int(step),
             _lib.ptr(lr_t), _lib.ptr(step_t), int(seed) & (2**64 - 1), _lib.stream()), "ceeg_adamw_step")
+    torch.autograd.graph.increment_version(params)   # a graph that saved a parameter notices
 
 
 class AdamW(torch.optim.Optimizer):

@@ -329,6 +329,16 @@ def test_captures_that_would_replay_wrongly_are_refused():
     assert torch.equal(p[0], torch.ones(10, device="cuda"))
 
 
+def test_a_graph_that_saved_a_parameter_notices():
+    from causal_eeg_vae_amd import adamw_step_
+    w = torch.ones(8, device="cuda", requires_grad=True)
+    loss = (w * w).sum()
+    x = [torch.zeros(8, device="cuda") for _ in range(3)]
+    adamw_step_([w], x[:1], x[1:2], x[2:], step=1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 def test_on_another_stream():
     from causal_eeg_vae_amd import adamw_step_
     a, b = _tensors([70001, 300], torch.float32, seed=4), _tensors([70001, 300], torch.float32, seed=4)
