@@ -157,7 +157,8 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ s
 }
 
 // The hidden states of the tokens that count, packed; `each` tokens per workgroup, the last workgroup adds the zero rows.  SCAN: up to CE_SCAN tokens, whose places every
-// workgroup finds for itself (a few KB from L2) - one launch instead of two; otherwise ce_tokens_kernel has found them.
+// workgroup finds for itself (a few KB from L2) - one launch instead of two; otherwise ce_tokens_kernel has found them.  V = H = 256 forward: 64 tokens 16.3 us, 17.4
+// with two launches; 4096 20.4 and 20.3; 16384 44.7 and 37.4.
 template <bool F32, bool SCAN>
 __global__ __launch_bounds__(256) void ce_prepare_kernel(CeTokens a, const void* __restrict__ h, int64_t ld, int H, int Kp, int each, unsigned short* __restrict__ out, int64_t plane) {
   __shared__ int32_t s_pos[SCAN ? CE_SCAN : 1];
@@ -520,39 +521,27 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_stats_kernel(CeMat W, CeMat 
   }
 }
 
-// A wave joins the pieces' maxima and sums of R tokens j, j + step, ... (below N): one pass, the loads of eight pieces of every token in flight
-template <int R>
-__device__ __forceinline__ void ce_join(const float2* __restrict__ part, int64_t j, int64_t step, int64_t N, int parts, int lane, float (&lse)[R]) {
-  float top[R], sum[R];
+// A wave joins the maxima and sums that the tiles left of token j: one pass, eight loads a lane in flight
+__device__ __forceinline__ float ce_join(const float2* __restrict__ part, int64_t j, int parts, int lane) {
+  float top = -INFINITY, sum = 0.f;
+  for (int c0 = lane; c0 < parts; c0 += 8 * 64) {
+    float2 u[8];
 #pragma unroll
-  for (int r = 0; r < R; ++r) { top[r] = -INFINITY; sum[r] = 0.f; }
-  for (int c0 = lane; c0 < parts; c0 += 8 / R * 64) {
-    float2 u[R][8 / R];
+    for (int k = 0; k < 8; ++k) u[k] = c0 + 64 * k < parts ? part[j * parts + c0 + 64 * k] : make_float2(-INFINITY, 0.f);
+    float t = top;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int k = 0; k < 8 / R; ++k)
-        u[r][k] = j + r * step < N && c0 + 64 * k < parts ? part[(j + r * step) * parts + c0 + 64 * k] : make_float2(-INFINITY, 0.f);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float t = top[r];
-#pragma unroll
-      for (int k = 0; k < 8 / R; ++k) t = fmaxf(t, u[r][k].x);
-      const float base = t == -INFINITY ? 0.f : t;
-      sum[r] *= __expf(top[r] - base);
-#pragma unroll
-      for (int k = 0; k < 8 / R; ++k) sum[r] += u[r][k].y * __expf(u[r][k].x - base);
-      top[r] = t;
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    float t = top[r];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o, 64));
+    for (int k = 0; k < 8; ++k) t = fmaxf(t, u[k].x);
     const float base = t == -INFINITY ? 0.f : t;
-    lse[r] = base + logf(ceeg_wave_sum(sum[r] * __expf(top[r] - base)));
+    sum *= __expf(top - base);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += u[k].y * __expf(u[k].x - base);
+    top = t;
   }
+  float t = top;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o, 64));
+  const float base = t == -INFINITY ? 0.f : t;
+  return base + logf(ceeg_wave_sum(sum * __expf(top - base)));
 }
 // a class outside [0, V) cannot raise an error from here: its loss is NaN
 __device__ __forceinline__ float ce_row_loss(float lse, const float* __restrict__ at_y, const int32_t* __restrict__ yc, int64_t j) {
@@ -565,36 +554,20 @@ __global__ __launch_bounds__(256) void ce_lse_kernel(const int32_t* __restrict__
   const int lane = threadIdx.x & 63;
   const int64_t j = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (j >= n[0]) return;
-  float l[1];
-  ce_join<1>(part, j, 1, n[0], parts, lane, l);
+  const float l = ce_join(part, j, parts, lane);
   if (lane == 0) {
-    lse[j] = l[0];
-    rowloss[rows ? rows[j] : j] = ce_row_loss(l[0], at_y, yc, j);
+    lse[j] = l;
+    rowloss[rows ? rows[j] : j] = ce_row_loss(l, at_y, yc, j);
   }
 }
 
-// Mean over the tokens that count (0 where none does) or sum, one workgroup.  JOIN: few tokens, whose lse it finds on the way; otherwise their losses are there.
-template <bool JOIN>
-__global__ __launch_bounds__(1024) void ce_loss_kernel(const int32_t* __restrict__ n, const float2* __restrict__ part, int parts, const float* __restrict__ at_y,
-                                                       const int32_t* __restrict__ yc, const float* __restrict__ rowloss, int reduction, float* __restrict__ lse, float* __restrict__ loss) {
+// Mean over the tokens that count (0 where none does) or sum, one workgroup.  A launch of its own also for few tokens: one workgroup that finds their lse on the way takes
+// longer than a wave each (32 tokens of 256 classes 19.0 us instead of 16.7 for the whole loss, 1 of 50257 21.3 instead of 18.4).
+__global__ __launch_bounds__(1024) void ce_loss_kernel(const int32_t* __restrict__ n, const float* __restrict__ rowloss, int reduction, float* __restrict__ loss) {
   __shared__ double s[16];
   const int N = n[0], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   double v = 0.0;
-  if (JOIN) {
-    for (int j = wave; j < N; j += 128) {
-      float l[8];
-      ce_join<8>(part, j, 16, N, parts, lane, l);
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        if (lane == r && j + 16 * r < N) {
-          lse[j + 16 * r] = l[r];
-          v += (double)ce_row_loss(l[r], at_y, yc, j + 16 * r);
-        }
-      }
-    }
-  } else {
-    for (int j = threadIdx.x; j < N; j += 1024) v += (double)rowloss[j];
-  }
+  for (int j = threadIdx.x; j < N; j += 1024) v += (double)rowloss[j];
   v = ceeg_wave_sum_d(v);
   if (lane == 0) s[wave] = v;
   __syncthreads();
@@ -836,7 +809,9 @@ __global__ __launch_bounds__(256) void ce_dh_join_kernel(const float* __restrict
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-// Tile edge for a grid of rows x columns (x the ways its sum may be cut): the largest that gives every compute unit a workgroup
+// Tile edge for a grid of rows x columns (x the ways its sum may be cut): the largest that gives (nearly) every compute unit a workgroup.  Forward, H = 512, 256 tiles of
+// that edge: 256 x 256 32.6 us, 128 x 128 39.1 (T = 1024, V = 16384); 128 x 128 23.0 us, 64 x 64 25.3 (V = 4096).  With 128 tiles of it: 256 x 256
+// 31.1 us, 128 x 128 27.2 (V = 8192); 128 x 128 20.2 us, 64 x 64 18.0 (H = 256, V = 2048).
 int ce_edge(int planes, int64_t rows, int64_t cols, int64_t cuts) {
   const auto tiles = [&](int e) { return ce_tiles(planes, e, rows, cols); };
   if (planes == 1 && tiles(256) * cuts >= 200) return 256;
@@ -997,16 +972,10 @@ extern "C" int ceeg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int
 #undef CE_CALL
     CEEG_CHECK_LAUNCH();
   }
-  // few tokens and pieces: one workgroup finds lse and loss (a launch less); more: a wave a token first
-  if (reduction != 0 && T * parts <= 32768) {
-    ce_loss_kernel<true><<<1, 1024, 0, st>>>(n, part, parts, at_y, yc, nullptr, reduction, lse, loss);
-    CEEG_CHECK_LAUNCH();
-    return CEEG_OK;
-  }
   ce_lse_kernel<<<(unsigned)((T + 3) / 4), 256, 0, st>>>(n, part, parts, at_y, yc, reduction == 0 ? rows : nullptr, lse, reduction == 0 ? loss : rowloss);
   CEEG_CHECK_LAUNCH();
   if (reduction != 0) {
-    ce_loss_kernel<false><<<1, 1024, 0, st>>>(n, nullptr, 0, nullptr, nullptr, rowloss, reduction, nullptr, loss);
+    ce_loss_kernel<<<1, 1024, 0, st>>>(n, rowloss, reduction, loss);
     CEEG_CHECK_LAUNCH();
   }
   return CEEG_OK;
