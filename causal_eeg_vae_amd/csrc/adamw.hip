@@ -128,6 +128,18 @@ __device__ __forceinline__ float aw_wave_max(int x) {  // bits of values >= 0: t
 #undef AW_MAX
   return __int_as_float(__builtin_amdgcn_readlane(x, 63));
 }
+// b^t by squaring: t 2^-53 of itself off at most, and so 1 - b^t >= (1 - b) t b^t no more than 2^-53 / (1 - b) of itself
+__device__ __forceinline__ double aw_power(double b, uint32_t t) {
+  double r = 1.0;
+  for (; t; t >>= 1, b *= b)
+    if (t & 1u) r *= b;
+  return r;
+}
+// 1 / b for b and 1 / b of ordinary size (a block's scale lies between 2^-109 and 2^120), nearly rounded: one Newton step behind the instruction
+__device__ __forceinline__ float aw_reciprocal(float b) {
+  const float r = __builtin_amdgcn_rcpf(b);
+  return __fmaf_rn(__fmaf_rn(-b, r, 1.f), r, r);
+}
 // a / b, correctly rounded, from the (nearly) rounded reciprocal r of b: a quotient within a unit and one exact remainder
 __device__ __forceinline__ float aw_quotient(float a, float b, float r) {
   const float q = a * r;
@@ -146,8 +158,7 @@ __device__ __forceinline__ uint32_t aw_round(float x, float scale, float per_sca
   uint32_t c = small ? (uint32_t)below : (u >> 20) - (120u << 3);
   if (SECOND) {
     const float l2 = small ? below + below : (float)(16u + 2u * (c & 7u)), d = l2 + 1.f;
-    const float r0 = __builtin_amdgcn_rcpf(d), r = __fmaf_rn(__fmaf_rn(-d, r0, 1.f), r0, r0);
-    share = aw_quotient(share * (l2 + share), d, r);
+    share = aw_quotient(share * (l2 + share), d, aw_reciprocal(d));
   }
   c += share * 65536.f + rnd >= 65536.f;
   if (SECOND && c == 0u && y > 0.f) c = 1u;
@@ -170,17 +181,27 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_kernel(AwList L, AwHyper h) 
   const int64_t end = begin + h.per_wg < n ? begin + h.per_wg : n;
   float step_size = h.step_size, inv_sqrt_c2 = h.inv_sqrt_c2, decay = h.decay;
   uint64_t seed = h.seed;
-  if (h.step_dev || h.lr_dev) {
-    const double lr = h.lr_dev ? (double)h.lr_dev[0] : h.lrd;
-    decay = (float)(1.0 - lr * h.wdd);
-    if (h.step_dev) {
-      const double t = (double)h.step_dev[0];
-      step_size = (float)(lr / (1.0 - pow(h.b1d, t)));
-      inv_sqrt_c2 = (float)(1.0 / sqrt(1.0 - pow(h.b2d, t)));
-      seed += (uint64_t)(int64_t)t * 0x9E3779B97F4A7C15ull;  // a replayed launch draws other numbers every step
-    } else {
-      step_size = (float)(lr * h.b1d);  // the host put 1 / (1 - b1^t) there
+  if (h.step_dev || h.lr_dev) {  // one wave finds the factors: in 64 bits they cost as much as half a block of elements
+    __shared__ float s_factor[3];
+    if (wave == 0) {
+      const double lr = h.lr_dev ? (double)h.lr_dev[0] : h.lrd;
+      float size = (float)(lr * h.b1d), inv = inv_sqrt_c2;  // without step_dev: the host put 1 / (1 - b1^t) there
+      if (h.step_dev) {
+        const uint32_t t = (uint32_t)h.step_dev[0];  // whole, and below 2^24 where it can still be counted up
+        size = (float)(lr / (1.0 - aw_power(h.b1d, t)));
+        inv = (float)(1.0 / sqrt(1.0 - aw_power(h.b2d, t)));
+      }
+      if (lane == 0) {
+        s_factor[0] = size;
+        s_factor[1] = inv;
+        s_factor[2] = (float)(1.0 - lr * h.wdd);
+      }
     }
+    __syncthreads();
+    step_size = s_factor[0];
+    inv_sqrt_c2 = s_factor[1];
+    decay = s_factor[2];
+    if (h.step_dev) seed += (uint64_t)(int64_t)h.step_dev[0] * 0x9E3779B97F4A7C15ull;  // a replayed launch draws other numbers every step
   }
   void* const p = L.p[lo];
   const void* const g = L.g[lo];
@@ -247,7 +268,7 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_kernel(AwList L, AwHyper h) 
       tv = aw_wave_max(bv);
     }
     const float sm = tm < AW_TINY ? 0.f : tm * AW_PER_TOP, sv = tv < AW_TINY ? 0.f : tv * AW_PER_TOP;
-    const float pm = sm > 0.f ? 1.f / sm : 0.f, pr = sv > 0.f ? 1.f / sv : 0.f;
+    const float pm = sm > 0.f ? aw_reciprocal(sm) : 0.f, pr = sv > 0.f ? aw_reciprocal(sv) : 0.f;
     const uint64_t quad = (uint64_t)i >> 2;
     const uint4 r = aw_philox(seed, (uint32_t)quad, (uint32_t)(quad >> 32), CEEG_TAG_ADAMW, h.ordinal + lo);
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
@@ -307,10 +328,9 @@ extern "C" int ceeg_adamw_step(int tensors, const int64_t* numel, void* const* p
   h.b1d = step_dev ? beta1 : 1.0 / c1; h.b2d = beta2; h.lrd = lr; h.wdd = weight_decay;
   h.step_dev = step_dev; h.lr_dev = lr_dev;
   h.seed = seed;
-  // Elements per workgroup.  One block per wave spreads a small list over as many compute units as there are (64 K elements of 32 / 8 bits: 4.5 / 5.7 us, 5.9 / 9.8 with
-  // 4096); four amortise the workgroup's start once that gives every compute unit one (4 M: 21.3 / 23.5 us instead of 22.7 / 30.0), eight are
-  // better still for the longer start of 8 bits in large lists (64 M: 241 us instead of 256, 393 with 1024; 32 bits 362 instead of 357).
-  h.per_wg = total < (int64_t)1 << 20 ? 1024 : state_bits == 8 && total >= (int64_t)1 << 24 ? 8192 : 4096;
+  // Elements per workgroup.  One block per wave fills the compute units soonest and balances them best (32 bits, 148 tensors of 66 M together: 354 us, 377 with 4096; 8 bits,
+  // 1 M: 8.0 us instead of 9.8).  The longer start of 8 bits is worth four blocks a wave from 4 M on (148 tensors of 66 M: 244 us instead of 267, 250 with 8192).
+  h.per_wg = state_bits == 8 && total >= (int64_t)1 << 22 ? 4096 : 1024;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   for (int t = 0; t < tensors;) {
     AwList L;
