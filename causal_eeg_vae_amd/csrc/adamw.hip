@@ -7,6 +7,8 @@
 // 16 random bits of Philox per value.  sqrt(v) > 0 never becomes 0: a denominator that vanishes while m does not would blow the next step up.
 // Bound: HBM bytes (fp32 28 per element; 8 bits 16 with fp32 parameters, 10 with bf16).  A wave takes one block of 256 elements, 4 per lane - 16-byte loads, the
 // block's maximum by one butterfly, one Philox call per lane for its four elements - so the 8-bit form needs no LDS and no barrier.
+// Measured, 66 M elements in 148 tensors: 32 bits 347 us (5.3 TB/s); 8 bits 244 us (4.3 TB/s: vector instructions, about 140 an element, are as long as the bytes), with 50 M
+// bf16 parameters 156 us (3.2 TB/s).
 // The tensors' pointers travel in the kernel arguments: no table in device memory, nothing to copy or to keep alive.
 #include <math.h>
 #include "ceeg_internal.h"
