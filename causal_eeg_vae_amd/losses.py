@@ -31,7 +31,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         dev = hidden.device
         if hidden.stride(1) != 1 or (T > 1 and hidden.stride(0) < H):
             hidden = hidden.contiguous()
-        if weight.stride(1) != 1 or (V > 1 and weight.stride(0) < H) or (dtype == _lib.CEEG_BF16 and (weight.data_ptr() % 16 or not weight.is_contiguous())):
+        if weight.stride(1) != 1 or (V > 1 and not H <= weight.stride(0) <= 1 << 22) or (dtype == _lib.CEEG_BF16 and (weight.data_ptr() % 16 or not weight.is_contiguous())):
             weight = weight.clone(memory_format=torch.contiguous_format)
         target = target.contiguous()
         ldh, ldw = max(hidden.stride(0), H), H if weight.is_contiguous() else weight.stride(0)
@@ -94,8 +94,8 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
         raise ValueError(f"weight must have a class and a column at least, got {tuple(weight.shape)}")
     _same_device(hidden, weight, target)
     if target.numel() == 0:  # no token: nothing to launch, the gradients are zero
-        none = (hidden.float().sum() + weight.float().sum()) * 0.0
-        return none if reduction != "none" else hidden.float().sum(-1) * 0.0
+        none = hidden.float().sum(-1) + weight[:0].float().sum()
+        return none if reduction == "none" else none.sum()
     loss = _LinearCrossEntropy.apply(hidden.reshape(-1, hidden.shape[-1]), weight, target.reshape(-1), int(ignore_index), _REDUCTIONS[reduction])
     return loss.view(target.shape) if reduction == "none" else loss
 

@@ -280,3 +280,22 @@ def test_no_token_at_all():
         dh, dw = torch.autograd.grad(loss, (h, w))
         assert float(loss) == 0 and dh.shape == h.shape and dw.shape == w.shape and not bool(dw.any())
     assert linear_cross_entropy(h, w, y, reduction="none").shape == (0,)
+
+
+def test_no_token_and_a_weight_that_is_not_finite():
+    from causal_eeg_vae_amd import linear_cross_entropy
+    h = torch.zeros(2, 0, 64, device="cuda", requires_grad=True)
+    w = torch.full((10, 64), float("nan"), device="cuda", requires_grad=True)
+    y = torch.zeros(2, 0, dtype=torch.int64, device="cuda")
+    for reduction in ("mean", "sum", "none"):
+        loss = linear_cross_entropy(h, w, y, reduction=reduction)
+        dh, dw = torch.autograd.grad(loss.sum(), (h, w))
+        assert loss.shape == (y.shape if reduction == "none" else ()) and not bool(loss.sum()) and dh.shape == h.shape and not bool(dw.any())
+
+
+def test_a_weight_of_very_distant_rows():
+    h, w, y = _inputs(5, 8, 3, torch.float32)
+    far = torch.zeros(3, (1 << 22) + 9, device="cuda")
+    far[:, :8] = w
+    for x, z in zip(_run(h, far[:, :8], y), _run(h, w, y)):
+        assert torch.equal(x, z)
