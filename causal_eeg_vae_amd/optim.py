@@ -114,8 +114,8 @@ class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update with one launch for (up to 56) tensors, and, with state_bits=8, moments of one byte an element (+ 4 per 256):
     an optimizer state of a quarter of the size.  Tensors of fewer than `min_8bit_size` elements keep theirs in 32 bits.
 
-    capturable=True keeps the step count on the device, so that `step()` can be captured into a graph and replayed; lr may then be a float32
-    tensor on the device too.  Parameters: float32 or bfloat16 on the GPU, contiguous, gradients of the same type."""
+    capturable=True keeps the step counts on the device, so that `step()` can be captured into a graph and replayed (with gradients of the same
+    parameters every time; the first step, which makes the moments, is taken before); lr may then be a float32 tensor on the device too.  Parameters: float32 or bfloat16 on the GPU, contiguous, gradients of the same type."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, min_8bit_size=4096, seed=0, capturable=False):
         if state_bits not in (8, 32):
@@ -134,15 +134,44 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, with the moments in the types that they were saved in (torch casts them to the parameter's)."""
+        if not all("state_bits" in saved for saved in state_dict["param_groups"]):
+            raise ValueError("the state of another optimizer")
         super().load_state_dict(state_dict)
         kept = lambda x, dev: tuple(t.detach().to(dev, copy=True) for t in x) if isinstance(x, tuple) else x.detach().to(dev, copy=True)  # noqa: E731
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            counts = {}  # parameters that have taken as many steps share their count again
             for p, i in zip(group["params"], saved["params"]):
                 if i in state_dict["state"]:
-                    self.state[p] = {k: kept(x, p.device) for k, x in state_dict["state"][i].items()}
-            if isinstance(group.get("step"), torch.Tensor) or (group["capturable"] and "step" in group):
-                count = float(group["step"])
-                group["step"] = torch.full((), count, dtype=torch.float32, device=group["params"][0].device) if group["capturable"] else int(count)
+                    held = state_dict["state"][i]
+                    st = {k: kept(x, p.device) for k, x in held.items() if k != "step"}
+                    n = int(held["step"])
+                    if group["capturable"]:
+                        if (n, p.device) not in counts:
+                            counts[n, p.device] = torch.full((), n, dtype=torch.float32, device=p.device)
+                        n = counts[n, p.device]
+                    st["step"] = n
+                    self.state[p] = st
+
+    def _count(self, group, taking):
+        """One step more for the parameters in `taking`; on the device one count serves all that have taken the same steps."""
+        if not group["capturable"]:
+            for p in taking:
+                self.state[p]["step"] += 1
+            return
+        now, counts = set(taking), {}
+        for p in group["params"]:
+            st = self.state.get(p)
+            if st:
+                counts.setdefault(id(st["step"]), (st["step"], [], []))[1 if p in now else 2].append(p)
+        for count, with_grad, without in counts.values():
+            if with_grad and without:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("AdamW: a captured step must take the parameters of the step before it")
+                count = count.clone()
+                for p in with_grad:
+                    self.state[p]["step"] = count
+            if with_grad:
+                count += 1
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -152,32 +181,29 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         ordinal = 0
         for group in self.param_groups:
-            lists = {}  # one call takes tensors of one type, one device and one form of state
-            for p in group["params"]:
-                if p.grad is None:
-                    continue
+            taking = [p for p in group["params"] if p.grad is not None]
+            fresh = {}
+            for p in taking:
                 st = self.state[p]
                 if not st:
                     if p.is_cuda and torch.cuda.is_current_stream_capturing():
                         raise RuntimeError("AdamW: take a step before capturing one: moments made inside a graph would start anew at every replay")
                     st.update(self._new_state(p, group))
-                lists.setdefault((p.dtype, p.device, isinstance(st["exp_avg"], tuple)), []).append(p)
-            if not lists:
-                continue
-            if group["capturable"]:
-                if len({dev for _, dev, _ in lists}) > 1:
-                    raise ValueError("capturable: a group's parameters must be on one device")
-                if not isinstance(group.get("step"), torch.Tensor):
-                    group["step"] = torch.full((), float(group.get("step", 0)), dtype=torch.float32, device=next(iter(lists))[1])
-                group["step"] += 1
-            else:
-                group["step"] = group.get("step", 0) + 1
+                    if group["capturable"] and p.device not in fresh:
+                        fresh[p.device] = torch.zeros((), dtype=torch.float32, device=p.device)
+                    st["step"] = fresh[p.device] if group["capturable"] else 0
+            self._count(group, taking)
+            lists = {}  # one call takes tensors of one type, one device, one form of state and one number of steps
+            for p in taking:
+                st = self.state[p]
+                lists.setdefault((p.dtype, p.device, isinstance(st["exp_avg"], tuple), id(st["step"]) if group["capturable"] else st["step"]), []).append(p)
             for ps in lists.values():
+                step = self.state[ps[0]]["step"]
                 seed = group["seed"] + (ordinal << 32)  # another stream for every list
                 ordinal += 1
                 if not group["capturable"]:
-                    seed += group["step"] * _SPREAD
+                    seed += step * _SPREAD
                 adamw_step_(ps, [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in ps], [self.state[p]["exp_avg"] for p in ps],
-                            [self.state[p]["exp_avg_sq"] for p in ps], group["step"], lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                            [self.state[p]["exp_avg_sq"] for p in ps], step, lr=group["lr"], betas=group["betas"], eps=group["eps"],
                             weight_decay=group["weight_decay"], seed=seed)
         return loss

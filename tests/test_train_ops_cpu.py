@@ -143,6 +143,8 @@ def test_adamw_class_refuses():
     with pytest.raises(ValueError):
         Trainer(torch.nn.Linear(2, 2), optimizer="sgd")
     AdamW(p).step()                                    # no gradient: nothing to do
+    with pytest.raises(ValueError):
+        AdamW(p).load_state_dict(torch.optim.AdamW(p).state_dict())
 
 
 def test_block_state_values():
