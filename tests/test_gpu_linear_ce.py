@@ -93,6 +93,15 @@ def test_every_tile_shape(T, H, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("T,H,V", [(3, 32768, 5), (70000, 5, 3), (2, 16, 1200000)])
+def test_one_long_side(T, H, V, dtype):
+    """The widest rows there may be, many tokens of few classes, more classes than a piece holds."""
+    h, w, y = _inputs(T, H, V, dtype)
+    loss, dh, dw, g = _run(h, w, y)
+    _check(h, w, y, loss, dh, dw, "mean", g)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
 def test_reductions_and_upstream_gradients(reduction, dtype):
     h, w, y = _inputs(200, 72, 777, dtype, seed=3)
