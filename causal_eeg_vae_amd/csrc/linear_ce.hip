@@ -162,28 +162,32 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ s
 // The hidden states of the tokens that count, packed; `each` tokens per workgroup, the last workgroup adds the zero rows.  SCAN: up to CE_SCAN tokens, whose places every
 // workgroup finds for itself (a few KB from L2) - one launch instead of two; otherwise ce_tokens_kernel has found them.  V = H = 256 forward: 64 tokens 16.3 us, 17.4
 // with two launches; 4096 20.4 and 20.3; 16384 44.7 and 37.4.
-template <bool F32, bool SCAN>
-__global__ __launch_bounds__(256) void ce_prepare_kernel(CeTokens a, const void* __restrict__ h, int64_t ld, int H, int Kp, int each, unsigned short* __restrict__ out, int64_t plane) {
-  __shared__ int32_t s_pos[SCAN ? CE_SCAN : 1];
+template <bool F32, int SCAN>
+__device__ __forceinline__ void ce_prepare(const CeTokens& a, const void* __restrict__ h, int64_t ld, int H, int Kp, int each, int block, int blocks, unsigned short* __restrict__ out, int64_t plane) {
+  __shared__ int32_t s_pos[SCAN ? SCAN : 1];
   int n;
   if (SCAN) {
-    n = ce_scan<256>(a, blockIdx.x == 0, s_pos);
+    n = ce_scan<256>(a, block == 0, s_pos);
     __syncthreads();
   } else {
     n = a.n[0];
   }
   const int per = Kp / 8;
-  const int64_t t0 = (int64_t)blockIdx.x * each;
+  const int64_t t0 = (int64_t)block * each;
   for (int i = threadIdx.x; i < each * per; i += 256) {
     const int64_t t = t0 + i / per;
     if (t >= a.T) break;
     const int j = SCAN ? s_pos[t] : a.pos[t], c = i % per * 8;
     if (j >= 0) ce_pack8<F32>(static_cast<const char*>(h) + t * ld * (F32 ? 4 : 2), c, H, out + (int64_t)j * Kp + c, plane);
   }
-  if (blockIdx.x == gridDim.x - 1) {
+  if (block == blocks - 1) {
     const int rows = (int)up(n, PAD) - n;
     for (int i = threadIdx.x; i < rows * per; i += 256) ce_pack8<F32>(nullptr, i % per * 8, H, out + (int64_t)(n + i / per) * Kp + i % per * 8, plane);
   }
+}
+template <bool F32, bool SCAN>
+__global__ __launch_bounds__(256) void ce_prepare_kernel(CeTokens a, const void* __restrict__ h, int64_t ld, int H, int Kp, int each, unsigned short* __restrict__ out, int64_t plane) {
+  ce_prepare<F32, SCAN ? CE_SCAN : 0>(a, h, ld, H, Kp, each, blockIdx.x, gridDim.x, out, plane);
 }
 
 // ------------------------------------------------------------------------------------------------ products
@@ -524,13 +528,13 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_stats_kernel(CeMat W, CeMat 
   }
 }
 
-// A wave joins the maxima and sums that the tiles left of token j: one pass, eight loads a lane in flight
-__device__ __forceinline__ float ce_join(const float2* __restrict__ part, int64_t j, int parts, int lane) {
+// A wave joins the maxima and sums c, c + step, ... (c: its first, plus the lane) that the tiles left of a token: one pass, eight loads a lane in flight
+__device__ __forceinline__ float2 ce_join(const float2* __restrict__ part, int c, int step, int parts) {
   float top = -INFINITY, sum = 0.f;
-  for (int c0 = lane; c0 < parts; c0 += 8 * 64) {
+  for (int64_t c0 = c; c0 < parts; c0 += 8 * (int64_t)step) {
     float2 u[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) u[k] = c0 + 64 * k < parts ? part[j * parts + c0 + 64 * k] : make_float2(-INFINITY, 0.f);
+    for (int k = 0; k < 8; ++k) u[k] = c0 + (int64_t)step * k < parts ? part[c0 + (int64_t)step * k] : make_float2(-INFINITY, 0.f);
     float t = top;
 #pragma unroll
     for (int k = 0; k < 8; ++k) t = fmaxf(t, u[k].x);
@@ -544,8 +548,9 @@ __device__ __forceinline__ float ce_join(const float2* __restrict__ part, int64_
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o, 64));
   const float base = t == -INFINITY ? 0.f : t;
-  return base + logf(ceeg_wave_sum(sum * __expf(top - base)));
+  return make_float2(t, ceeg_wave_sum(sum * __expf(top - base)));
 }
+__device__ __forceinline__ float ce_lse(float2 v) { return (v.x == -INFINITY ? 0.f : v.x) + logf(v.y); }
 // a class outside [0, V) cannot raise an error from here: its loss is NaN
 __device__ __forceinline__ float ce_row_loss(float lse, const float* __restrict__ at_y, const int32_t* __restrict__ yc, int64_t j) {
   return yc[j] >= 0 ? lse - at_y[j] : __uint_as_float(0x7fc00000u);
@@ -557,7 +562,7 @@ __global__ __launch_bounds__(256) void ce_lse_kernel(const int32_t* __restrict__
   const int lane = threadIdx.x & 63;
   const int64_t j = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (j >= n[0]) return;
-  const float l = ce_join(part, j, parts, lane);
+  const float l = ce_lse(ce_join(part + j * parts, lane, 64, parts));
   if (lane == 0) {
     lse[j] = l;
     rowloss[rows ? rows[j] : j] = ce_row_loss(l, at_y, yc, j);
@@ -579,6 +584,166 @@ __global__ __launch_bounds__(1024) void ce_loss_kernel(const int32_t* __restrict
     for (int k = 0; k < 16; ++k) v += s[k];
     loss[0] = (float)(reduction == 1 ? v / (N > 0 ? N : 1) : v);
   }
+}
+
+// ------------------------------------------------------------------------------------------------ few tokens
+// The statistics of up to R tokens against W read once as it is (no planes, no padding, fp32 multiply-adds): bound by W's bytes.  16 lanes take four rows of W, a wave sixteen, a
+// workgroup FEW of them; the hidden rows are in LDS in fp32, read once for the four rows.  A last workgroup does what ce_prepare_kernel does meanwhile.
+constexpr int CE_FEW = 64;             // classes of a workgroup
+constexpr int CE_FEW_TOKENS = 8;
+constexpr int CE_FEW_LDS = 48 * 1024;  // bytes of hidden rows
+
+template <bool F32, int R, bool WIDE>
+__global__ __launch_bounds__(256, R == 1 ? 4 : R == 2 ? 3 : 2) void ce_few_kernel(CeTokens a, const void* __restrict__ h, int64_t ldh, const void* __restrict__ W, int64_t ldw, int H, int Kp, int parts,
+                                                        float2* __restrict__ part, float* __restrict__ at_y, unsigned short* __restrict__ packed, int64_t plane) {
+  constexpr int VEC = F32 ? 4 : 8, U = 4;
+  extern __shared__ __align__(16) float s_h[];  // [R][Hv]
+  __shared__ float2 s_wave[4][R];
+  const int blocks = (int)gridDim.x - 1;
+  if ((int)blockIdx.x == blocks) {
+    ce_prepare<F32, CE_FEW_TOKENS>(a, h, ldh, H, Kp, CE_FEW_TOKENS, 0, 1, packed, plane);
+    return;
+  }
+  const int Hv = (int)up(H, 32 * VEC), passes = Hv / (16 * VEC), lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4, l = lane & 15;
+  const int64_t y = lane < a.T ? a.y[lane] : a.ignore;  // T <= R
+  // 16 bytes of each of the four rows, zeros behind H.  WIDE: all of W in pieces of 16 bytes on such addresses
+  const auto load = [&](uint4 (&w)[U], int b, int pass) {
+    const int c = (pass * 16 + l) * VEC;
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = make_uint4(0u, 0u, 0u, 0u);
+    if (c >= H || b >= parts) return;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      int64_t v = (int64_t)b * CE_FEW + wave * 16 + group * U + u;
+      if (v >= a.V) v = a.V - 1;  // what it gives is not looked at
+      const char* const q = static_cast<const char*>(W) + (v * ldw + c) * (F32 ? 4 : 2);
+      if (WIDE) {
+        w[u] = *reinterpret_cast<const uint4*>(q);
+      } else {
+        uint32_t x[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          if (c + k >= H) continue;
+          if (F32) x[k % 4] = reinterpret_cast<const uint32_t*>(q)[k];
+          else x[k / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(q)[k] << (16 * (k & 1));
+        }
+        w[u] = make_uint4(x[0], x[1], x[2], x[3]);
+      }
+    }
+  };
+  uint4 w0[U], w1[U];  // two passes on their way
+  load(w0, blockIdx.x, 0);
+  load(w1, blockIdx.x, 1);
+  uint64_t left = __ballot(y != a.ignore);
+  const int N = __popcll(left);
+  int cls[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int t = left ? __ffsll((unsigned long long)left) - 1 : 0;
+    left &= left - 1;
+    const int64_t own = __shfl(y, t, 64);
+    cls[r] = r < N && own >= 0 && own < a.V ? (int)own : -1;
+    for (int c = threadIdx.x; c < Hv; c += 256) {
+      float x = 0.f;
+      if (r < N && c < H) x = F32 ? static_cast<const float*>(h)[t * ldh + c] : ceeg_bf16_to_f32(static_cast<const unsigned short*>(h)[t * ldh + c]);
+      s_h[r * Hv + c] = x;
+    }
+  }
+  __syncthreads();
+  for (int b = blockIdx.x; b < parts; b += blocks) {
+    float acc[U][R];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < R; ++r) acc[u][r] = 0.f;
+    const auto step = [&](uint4 (&w)[U], int pass) {  // multiplies a pass and asks for the one after the next
+      float f[U][VEC];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t x[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) f[u][k] = __uint_as_float(F32 ? x[k % 4] : k & 1 ? x[k / 2] & 0xffff0000u : x[k / 2] << 16);
+      }
+      const bool more = pass + 2 < passes;
+      load(w, more ? b : b + blocks, more ? pass + 2 : pass + 2 - passes);
+      const float* const x = s_h + (pass * 16 + l) * VEC;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int k = 0; k < VEC; k += 4) {
+          const float4 z = *reinterpret_cast<const float4*>(x + r * Hv + k);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            acc[u][r] = __fmaf_rn(f[u][k + 3], z.w, __fmaf_rn(f[u][k + 2], z.z, __fmaf_rn(f[u][k + 1], z.y, __fmaf_rn(f[u][k], z.x, acc[u][r]))));
+        }
+      }
+    };
+    for (int pass = 0; pass < passes; pass += 2) {
+      step(w0, pass);
+      step(w1, pass + 1);
+    }
+    const int64_t v0 = (int64_t)b * CE_FEW + wave * 16 + group * U;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) acc[u][r] += __shfl_xor(acc[u][r], o, 64);
+        if (v0 + u >= a.V) acc[u][r] = -INFINITY;
+        else if (l == 0 && cls[r] == v0 + u) at_y[r] = acc[u][r];
+        top = fmaxf(top, acc[u][r]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) sum += ce_exp<F32 ? 3 : 1>(acc[u][r], base);
+      sum += __shfl_xor(sum, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      if (lane == 0) s_wave[wave][r] = make_float2(top, sum);
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < N) {
+      float2 v = s_wave[0][threadIdx.x];
+      for (int k = 1; k < 4; ++k) {
+        const float2 o = s_wave[k][threadIdx.x];
+        const float top = fmaxf(v.x, o.x), base = top == -INFINITY ? 0.f : top;
+        v = make_float2(top, v.y * __expf(v.x - base) + o.y * __expf(o.x - base));
+      }
+      part[(int64_t)threadIdx.x * parts + b] = v;
+    }
+    __syncthreads();
+  }
+}
+
+// lse and loss of up to R tokens by one workgroup, 16 / R waves a token
+template <int R>
+__global__ __launch_bounds__(1024) void ce_few_loss_kernel(const int32_t* __restrict__ n, const float2* __restrict__ part, int parts, const float* __restrict__ at_y,
+                                                           const int32_t* __restrict__ yc, const int32_t* __restrict__ rows, int reduction, float* __restrict__ lse, float* __restrict__ loss) {
+  constexpr int EACH = 16 / R;
+  __shared__ float2 s[16];
+  const int N = n[0], lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = wave / EACH;
+  float2 v = make_float2(-INFINITY, 0.f);
+  if (mine < N) v = ce_join(part + (int64_t)mine * parts, wave % EACH * 64 + lane, EACH * 64, parts);
+  if (lane == 0) s[wave] = v;
+  __syncthreads();
+  if (wave != 0) return;
+  double d = 0.0;
+  if (lane < N) {
+    float top = -INFINITY, sum = 0.f;
+    for (int k = 0; k < EACH; ++k) top = fmaxf(top, s[lane * EACH + k].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    for (int k = 0; k < EACH; ++k) sum += s[lane * EACH + k].y * __expf(s[lane * EACH + k].x - base);
+    const float z = ce_lse(make_float2(top, sum)), x = ce_row_loss(z, at_y, yc, lane);
+    lse[lane] = z;
+    if (reduction == 0) loss[rows[lane]] = x;
+    d = (double)x;
+  }
+  if (reduction == 0) return;
+  d = ceeg_wave_sum_d(d);
+  if (lane == 0) loss[0] = (float)(reduction == 1 ? d / (N > 0 ? N : 1) : d);
 }
 
 // What comes back for token j is s r_j.  Mean and sum: r = 1, so that rounding r (p - [v = y]) to bf16 does not round the common factor too.
@@ -834,7 +999,17 @@ struct CePlan {
   int e_logits, e_dh, e_dw;         // tile edges
   CeCut dh_cut;                     // stretches that the sums are cut into
   int dw_slots;
+  int few;                          // tokens that ce_few_kernel takes (a power of two), 0: the tiles
 };
+
+// Up to eight tokens in fp32, two in bf16: the tiles' time hardly depends on how few there are, as they first make planes of W (fp32) or pad it (bf16 of an H that is no multiple
+// of 64).  768 x 50257: fp32 1 token 30 us, tiles 134; 8 tokens 48 and 139; bf16 1 token 19.2 and 28.5, 4 tokens 28.6 and 29.2, 8 tokens 41 and 30.
+size_t ce_few_lds(int few, int64_t H, int dtype) { return (size_t)few * up(H, dtype == CEEG_F32 ? 128 : 256) * 4; }
+int ce_few(int64_t T, int64_t H, int dtype) {
+  if (T > (dtype == CEEG_F32 ? CE_FEW_TOKENS : 2)) return 0;
+  const int r = T > 4 ? 8 : T > 2 ? 4 : (int)T;
+  return ce_few_lds(r, H, dtype) <= CE_FEW_LDS ? r : 0;
+}
 
 CePlan ce_plan(int64_t T, int64_t H, int64_t V, int dtype, bool backward) {
   CePlan c;
@@ -853,6 +1028,8 @@ CePlan ce_plan(int64_t T, int64_t H, int64_t V, int dtype, bool backward) {
   c.ldv = up(c.piece < V ? c.piece : V, PAD);
   const int64_t cols = c.piece < V ? c.piece : V;
   c.e_logits = ce_edge(c.P, cols, T, 1);
+  c.few = backward ? 0 : ce_few(T, H, dtype);
+  if (c.few) c.e_logits = CE_FEW;
   const auto tiles = [&](int64_t m, int64_t n, int e) { return ce_tiles(c.P, e, m, n); };
   c.e_dh = ce_edge(c.P, H, T, c.ldv / 1024 + 1);
   c.dh_cut = CeCut{ce_want(c.e_dh), 0, INT64_MAX};
@@ -882,7 +1059,7 @@ size_t ce_packed_bytes(const CePlan& c) { return ceeg_ws_part((size_t)c.P * c.Tp
 size_t ce_fwd_bytes(int64_t T, int64_t H, int64_t V, int dtype) {
   const CePlan c = ce_plan(T, H, V, dtype, false);
   const size_t parts = (size_t)(V + c.e_logits - 1) / c.e_logits;
-  return (c.direct ? 0 : ceeg_ws_part((size_t)c.P * c.piece * c.Kp, 2)) + ceeg_ws_part((size_t)T * parts, 8) + 2 * ceeg_ws_part(T, 4);
+  return (c.direct || c.few ? 0 : ceeg_ws_part((size_t)c.P * c.piece * c.Kp, 2)) + ceeg_ws_part((size_t)T * parts, 8) + 2 * ceeg_ws_part(T, 4);
 }
 size_t ce_bwd_bytes(int64_t T, int64_t H, int64_t V, int dtype) {
   const CePlan c = ce_plan(T, H, V, dtype, true);
@@ -936,7 +1113,7 @@ extern "C" int ceeg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int
   const int parts = (int)((V + c.e_logits - 1) / c.e_logits);
   CeegWs w(ws, ws_bytes);
   unsigned short* const hc = static_cast<unsigned short*>(packed);
-  unsigned short* wc = c.direct ? nullptr : w.take<unsigned short>((size_t)c.P * c.piece * c.Kp);
+  unsigned short* wc = c.direct || c.few ? nullptr : w.take<unsigned short>((size_t)c.P * c.piece * c.Kp);
   float2* part = w.take<float2>((size_t)T * parts);
   float* at_y = w.take<float>(T);
   float* rowloss = w.take<float>(T);
@@ -944,6 +1121,31 @@ extern "C" int ceeg_linear_ce_fwd(const void* h, int64_t ldh, const void* W, int
   int32_t *n = tokens, *rows = tokens + 1, *pos = rows + T, *yc = pos + T;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const CeTokens tk{y, T, V, ignore_index, n, rows, pos, yc, reduction == 0 ? loss : nullptr};
+  if (c.few) {
+    const size_t lds = ce_few_lds(c.few, H, dtype);
+    const bool wide = ceeg_aligned(W, 16) && (dtype == CEEG_F32 ? (H | ldw) % 4 == 0 : (H | ldw) % 8 == 0);
+    const int resident = 256 * (c.few == 1 ? 4 : c.few == 2 ? 3 : 2);
+    const unsigned grid = (unsigned)(parts < resident ? parts : resident) + 1;  // what is resident at once, and the one that prepares
+#define CE_CALL(F32, R)                                                                                                                                                 \
+  do {                                                                                                                                                                  \
+    if (wide) ce_few_kernel<F32, R, true><<<grid, 256, lds, st>>>(tk, h, ldh, W, ldw, (int)H, (int)c.Kp, parts, part, at_y, hc, c.Tp * c.Kp);                        \
+    else ce_few_kernel<F32, R, false><<<grid, 256, lds, st>>>(tk, h, ldh, W, ldw, (int)H, (int)c.Kp, parts, part, at_y, hc, c.Tp * c.Kp);                            \
+    CEEG_CHECK_LAUNCH();                                                                                                                                                \
+    ce_few_loss_kernel<R><<<1, 1024, 0, st>>>(n, part, parts, at_y, yc, rows, reduction, lse, loss);                                                                    \
+  } while (0)
+    if (dtype == CEEG_F32) {
+      if (c.few == 1) CE_CALL(true, 1);
+      else if (c.few == 2) CE_CALL(true, 2);
+      else if (c.few == 4) CE_CALL(true, 4);
+      else CE_CALL(true, 8);
+    } else {
+      if (c.few == 1) CE_CALL(false, 1);
+      else CE_CALL(false, 2);
+    }
+#undef CE_CALL
+    CEEG_CHECK_LAUNCH();
+    return CEEG_OK;
+  }
   const bool scan = T <= CE_SCAN;
   if (!scan) {
     ce_tokens_kernel<<<1, 1024, 0, st>>>(tk);

@@ -22,34 +22,39 @@ def _same_device(*tensors):
         raise ValueError(f"all tensors must be on one device, got {[str(t.device) for t in tensors if t is not None]}")
 
 
+def _linear_ce(hidden, weight, target, ignore_index, reduction):
+    """The loss, and what the backward takes back."""
+    L = _lib.lib()
+    dtype = _dtype(hidden, "hidden")
+    (T, H), V = hidden.shape, weight.shape[0]
+    dev = hidden.device
+    if hidden.stride(1) != 1 or (T > 1 and hidden.stride(0) < H):
+        hidden = hidden.contiguous()
+    if weight.stride(1) != 1 or (V > 1 and not H <= weight.stride(0) <= 1 << 22) or (dtype == _lib.CEEG_BF16 and (weight.data_ptr() % 16 or not weight.is_contiguous())):
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    target = target.contiguous()
+    ldh, ldw = max(hidden.stride(0), H), H if weight.is_contiguous() else weight.stride(0)
+    with _lib.on(dev):
+        loss = torch.empty(T if reduction == 0 else (), dtype=torch.float32, device=dev)
+        # one buffer for what the backward takes back: the packed rows, lse [T], tokens [3 T + 1]
+        rows = L.ceeg_linear_ce_packed_bytes(T, H, dtype)
+        kept = _lib.workspace(rows + 16 * T + 4, dev)
+        packed = kept.data_ptr()
+        lse, tokens = packed + rows, packed + rows + 4 * T
+        ws = _lib.workspace(L.ceeg_linear_ce_fwd_ws_bytes(T, H, V, dtype), dev)
+        with _lib.timed("linear_ce_fwd"):
+            _lib.check(L.ceeg_linear_ce_fwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, target.data_ptr(), T, H, V, dtype, ignore_index, reduction,
+                                            loss.data_ptr(), lse, tokens, packed, ws.data_ptr(), ws.numel(), _lib.stream()),
+                       "ceeg_linear_ce_fwd")
+    return loss, kept, weight, (T, H, V, ldw, dtype, reduction, rows)
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, ignore_index, reduction):
-        L = _lib.lib()
-        dtype = _dtype(hidden, "hidden")
-        (T, H), V = hidden.shape, weight.shape[0]
-        dev = hidden.device
-        if hidden.stride(1) != 1 or (T > 1 and hidden.stride(0) < H):
-            hidden = hidden.contiguous()
-        if weight.stride(1) != 1 or (V > 1 and not H <= weight.stride(0) <= 1 << 22) or (dtype == _lib.CEEG_BF16 and (weight.data_ptr() % 16 or not weight.is_contiguous())):
-            weight = weight.clone(memory_format=torch.contiguous_format)
-        target = target.contiguous()
-        ldh, ldw = max(hidden.stride(0), H), H if weight.is_contiguous() else weight.stride(0)
-        with _lib.on(dev):
-            loss = torch.empty(T if reduction == 0 else 1, dtype=torch.float32, device=dev)
-            # one buffer for what the backward takes back: the packed rows, lse [T], tokens [3 T + 1]
-            rows = L.ceeg_linear_ce_packed_bytes(T, H, dtype)
-            kept = _lib.workspace(rows + 16 * T + 4, dev)
-            packed = kept.data_ptr()
-            lse, tokens = packed + rows, packed + rows + 4 * T
-            ws = _lib.workspace(L.ceeg_linear_ce_fwd_ws_bytes(T, H, V, dtype), dev)
-            with _lib.timed("linear_ce_fwd"):
-                _lib.check(L.ceeg_linear_ce_fwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, target.data_ptr(), T, H, V, dtype, ignore_index, reduction,
-                                                loss.data_ptr(), lse, tokens, packed, ws.data_ptr(), ws.numel(), _lib.stream()),
-                           "ceeg_linear_ce_fwd")
+        loss, kept, weight, ctx.sizes = _linear_ce(hidden, weight, target, ignore_index, reduction)
         ctx.save_for_backward(kept, weight)
-        ctx.sizes = T, H, V, ldw, dtype, reduction, rows
-        return loss if reduction == 0 else loss[0]
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -96,7 +101,11 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
     if target.numel() == 0:  # no token: nothing to launch, the gradients are zero
         none = hidden.float().sum(-1) + weight[:0].float().sum()
         return none if reduction == "none" else none.sum()
-    loss = _LinearCrossEntropy.apply(hidden.reshape(-1, hidden.shape[-1]), weight, target.reshape(-1), int(ignore_index), _REDUCTIONS[reduction])
+    args = hidden.reshape(-1, hidden.shape[-1]), weight, target.reshape(-1), int(ignore_index), _REDUCTIONS[reduction]
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        loss = _LinearCrossEntropy.apply(*args)
+    else:  # nothing comes back: autograd's part of the call is left out
+        loss = _linear_ce(*args)[0]
     return loss.view(target.shape) if reduction == "none" else loss
 
 

@@ -111,6 +111,41 @@ def test_reductions_and_upstream_gradients(reduction, dtype):
     _check(h, w, y, loss, dh, dw, reduction, g)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("T,H,V", [(1, 129, 65), (2, 64, 4097), (3, 77, 63), (4, 768, 1030), (5, 8, 128), (7, 1538, 100), (8, 192, 5003), (9, 192, 5003), (1, 12352, 70), (6, 2100, 257)])
+def test_few_tokens(T, H, V, reduction, dtype):
+    """Up to eight tokens, where the vocabulary's rows are read as they are, and its edges; the last token is ignored, so that a single one leaves none."""
+    h, w, y = _inputs(T, H, V, dtype, ignored=0.0)
+    y[-1] = -100
+    h[-1] = float("nan")
+    g = torch.linspace(-1.5, 2.0, T, device="cuda") if reduction == "none" else torch.tensor(0.7, device="cuda")
+    loss, dh, dw, g = _run(h, w, y, reduction, g)
+    _check(h, w, y, loss, dh, dw, reduction, g)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_few_tokens_strided_and_out_of_range(dtype):
+    from causal_eeg_vae_amd import linear_cross_entropy
+    h, w, y = _inputs(6, 192, 1000, dtype, ignored=0.0)
+    want = _run(h, w, y)
+    wide = torch.full((6, 201), 9.0, dtype=dtype, device="cuda")
+    wide[:, 3:195] = h
+    base = torch.zeros(1000 * 192 + 1, dtype=dtype, device="cuda")
+    base[1:] = w.reshape(-1)
+    loose = torch.full((1000, 195), float("inf"), dtype=dtype, device="cuda")
+    loose[:, :192] = w
+    for a in (wide[:, 3:195], h):
+        for b in (base[1:].view(1000, 192), loose[:, :192], w):
+            for x, z in zip(_run(a, b, y), want):
+                assert torch.equal(x, z)
+    rows = linear_cross_entropy(h, w, y, reduction="none")
+    y[2], y[4] = 1000, -1
+    bad = linear_cross_entropy(h, w, y, reduction="none")
+    odd = torch.tensor([False, False, True, False, True, False], device="cuda")
+    assert torch.equal(bad.isnan(), odd) and torch.equal(bad[~odd], rows[~odd])
+
+
 def test_no_upstream_gradient_is_zero():
     h, w, y = _inputs(50, 64, 300, torch.bfloat16)
     for reduction, g in (("none", torch.zeros(50, device="cuda")), ("sum", torch.zeros((), device="cuda"))):
