@@ -8,11 +8,10 @@
 //                small ones first - 6/16 of the bf16 rate instead of the 1/16 of the fp32 instruction.
 // Tokens that are ignored are dropped before the first product: their rows are packed away, the grids cover all T tokens and what
 // lies behind the last one that counts leaves at once (its number is read on the device, the host never waits for it).
-// Measured, bf16, 8192 tokens (7373 count) x 1024 x 131072: statistics 1.85 ms (1.07 PFLOP/s), and per half of the vocabulary dl 1.07 ms (0.92), dh 0.88 ms (1.12),
-// dW 0.80 ms (1.24); 1.09 over all.  fp32, 16384 x 256 x 4096: 238, 271, 188 and 190 us (0.87, 0.76, 1.10, 1.08 PFLOP/s of bf16 products, a sixth of that in fp32).
-// One token x 768 x 50257: 18 us, W at 4.2 TB/s.
 // The vocabulary is taken in pieces; of a piece only dl is held (bf16).  A product whose operand runs across the summed axis (W in dh, h and dl in
 // dW) reads it through the transposing LDS read, so nothing is ever stored transposed.  No float atomics: the pieces of a sum are added in a fixed order.
+// Measured, bf16, 8192 tokens (7373 count) x 1024 x 131072: statistics 1.85 ms (1.07 PFLOP/s), and per half of the vocabulary dl 1.07 ms (0.92), dh 0.88 ms (1.12),
+// dW 0.80 ms (1.24); 1.09 over all.  fp32, 16384 x 256 x 4096: 238, 271, 188 and 190 us (0.87, 0.76, 1.10, 1.08 PFLOP/s of bf16 products, a sixth of that in fp32).
 #include <limits.h>
 #include "ceeg_internal.h"
 
@@ -588,7 +587,8 @@ __global__ __launch_bounds__(1024) void ce_loss_kernel(const int32_t* __restrict
 
 // ------------------------------------------------------------------------------------------------ few tokens
 // The statistics of up to R tokens against W read once as it is (no planes, no padding, fp32 multiply-adds): bound by W's bytes.  16 lanes take four rows of W, a wave sixteen, a
-// workgroup FEW of them; the hidden rows are in LDS in fp32, read once for the four rows.  A last workgroup does what ce_prepare_kernel does meanwhile.
+// workgroup FEW of them; the hidden rows are in LDS in fp32, read once for the four rows; two pieces of 16 bytes of each row are on their way.  A last workgroup
+// does what ce_prepare_kernel does meanwhile.  One token x 768 x 50257: bf16 16.4 us (4.7 TB/s); with the join in fp32 30 us, in bf16 20.
 constexpr int CE_FEW = 64;             // classes of a workgroup
 constexpr int CE_FEW_TOKENS = 8;
 constexpr int CE_FEW_LDS = 48 * 1024;  // bytes of hidden rows
