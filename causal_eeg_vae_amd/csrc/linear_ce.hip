@@ -112,6 +112,10 @@ __device__ __forceinline__ int ce_scan(const CeTokens& a, bool write, int32_t* p
 __global__ __launch_bounds__(1024) void ce_tokens_kernel(CeTokens a) { ce_scan<1024>(a, true, nullptr); }
 
 // ------------------------------------------------------------------------------------------------ planes
+// Where element (r, c) of a blocked matrix of C columns is: blocks of 16 rows x 32 columns, each one piece of 1 KB, so that a tile's loads are whole cache lines whichever way the tile
+// lies.  Rows of 32 columns from a row-major matrix are half lines: twice the requests, which bound the products (the L2 took two thirds of the requests it can).
+__host__ __device__ __forceinline__ int64_t ce_place(int64_t r, int c, int64_t C) { return ((r >> 4) * (C >> 5) + (c >> 5)) * 512 + (r & 15) * 32 + (c & 31); }
+
 // eight columns c.. of a row of C at `src` (NULL: zeros) -> the planes at out
 template <bool F32>
 __device__ __forceinline__ void ce_pack8(const void* src, int c, int C, unsigned short* out, int64_t plane) {
@@ -147,7 +151,7 @@ __device__ __forceinline__ void ce_pack8(const void* src, int c, int C, unsigned
         make_uint4(p[0][a] | (uint32_t)p[1][a] << 16, p[2][a] | (uint32_t)p[3][a] << 16, p[4][a] | (uint32_t)p[5][a] << 16, p[6][a] | (uint32_t)p[7][a] << 16);
 }
 
-// Row-major [R, C] -> planes [P][*][Cp], columns C..Cp zero; `zeros`: the rows behind the last, up to the next multiple of PAD, zero too (a sum over the rows runs over them).
+// Row-major [R, C] -> planes [P][*][Cp] (blocked where there are three), columns C..Cp zero; `zeros`: the rows behind the last, up to the next multiple of PAD, zero too (a sum over the rows runs over them).
 template <bool F32>
 __global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ src, int64_t ld, int64_t R, int C, int Cp, int zeros, unsigned short* __restrict__ out, int64_t plane) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -155,10 +159,10 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const void* __restrict__ s
   const int64_t r = id / per;
   const int c = (int)(id % per) * 8;
   if (r >= (zeros ? up(R, PAD) : R)) return;
-  ce_pack8<F32>(r < R ? static_cast<const char*>(src) + r * ld * (F32 ? 4 : 2) : nullptr, c, C, out + r * Cp + c, plane);
+  ce_pack8<F32>(r < R ? static_cast<const char*>(src) + r * ld * (F32 ? 4 : 2) : nullptr, c, C, out + (F32 ? ce_place(r, c, Cp) : r * Cp + c), plane);
 }
 
-// The hidden states of the tokens that count, packed; `each` tokens per workgroup, the last workgroup adds the zero rows.  SCAN: up to CE_SCAN tokens, whose places every
+// The hidden states of the tokens that count, packed and blocked; `each` tokens per workgroup, the last workgroup adds the zero rows.  SCAN: up to CE_SCAN tokens, whose places every
 // workgroup finds for itself (a few KB from L2) - one launch instead of two; otherwise ce_tokens_kernel has found them.  V = H = 256 forward: 64 tokens 16.3 us, 17.4
 // with two launches; 4096 20.4 and 20.3; 16384 44.7 and 37.4.
 template <bool F32, int SCAN>
@@ -177,11 +181,11 @@ __device__ __forceinline__ void ce_prepare(const CeTokens& a, const void* __rest
     const int64_t t = t0 + i / per;
     if (t >= a.T) break;
     const int j = SCAN ? s_pos[t] : a.pos[t], c = i % per * 8;
-    if (j >= 0) ce_pack8<F32>(static_cast<const char*>(h) + t * ld * (F32 ? 4 : 2), c, H, out + (int64_t)j * Kp + c, plane);
+    if (j >= 0) ce_pack8<F32>(static_cast<const char*>(h) + t * ld * (F32 ? 4 : 2), c, H, out + ce_place(j, c, Kp), plane);
   }
   if (block == blocks - 1) {
     const int rows = (int)up(n, PAD) - n;
-    for (int i = threadIdx.x; i < rows * per; i += 256) ce_pack8<F32>(nullptr, i % per * 8, H, out + (int64_t)(n + i / per) * Kp + i % per * 8, plane);
+    for (int i = threadIdx.x; i < rows * per; i += 256) ce_pack8<F32>(nullptr, i % per * 8, H, out + ce_place(n + i / per, i % per * 8, Kp), plane);
   }
 }
 template <bool F32, bool SCAN>
@@ -229,6 +233,8 @@ struct CeTile {
   static constexpr int LDS = ST * STAGE;
   static_assert(LA > 0 && LB > 0 && LA * WAVES * 512 == BM * BK && LB * WAVES * 512 == BN * BK, "whole loads");
   static_assert(LDS * 2 <= 160 * 1024, "LDS");
+  // B is always a matrix made here, and blocked; A is W, which in bf16 lies as the caller has it, or (both across k) the hidden states
+  static constexpr bool BLOCKED_A = PL == 3 || (TA && TB);
   f32x4 acc[MT][NT];
 
   // Load i of a wave fetches 64 pieces of 16 bytes of the tile: rows `row(lane) + hop(i)`; a hop changes no bit of a row that the swizzle looks at, so that
@@ -241,15 +247,17 @@ struct CeTile {
   static __device__ __forceinline__ int row0(int wave) {
     return !T ? wave * 16 : BR == 256 ? (wave & 1) * 2 + (wave >> 1) * 8 : wave * (512 / BR);  // 256: eight waves
   }
-  template <bool T, int BR>
+  template <bool T, int BR, bool BLOCKED>
   static __device__ __forceinline__ uint32_t offset(const CeMat& x, int wave, int lane) {
     if (T) {
       constexpr int CPR = BR / 8;  // pieces per row k
       const int row = row0<T, BR>(wave) + lane / CPR, slot = lane % CPR, g = ((row & 3) | (row >> 3 & 1) << 2) & (BR / 16 - 1);
-      return (uint32_t)(lane / CPR) * (uint32_t)x.ld * 2u + (uint32_t)(((slot >> 1) ^ g) << 1 | (slot & 1)) * 16u;
+      const uint32_t piece = (uint32_t)(((slot >> 1) ^ g) << 1 | (slot & 1));
+      if (BLOCKED) return (uint32_t)(lane / CPR) * 64u + (piece >> 2) * 1024u + (piece & 3u) * 16u;
+      return (uint32_t)(lane / CPR) * (uint32_t)x.ld * 2u + piece * 16u;
     }
     const int row = lane >> 2;
-    return (uint32_t)row * (uint32_t)x.ld * 2u + (uint32_t)((lane & 3) ^ (row >> 1 & 3)) * 16u;
+    return (uint32_t)row * (BLOCKED ? 64u : (uint32_t)x.ld * 2u) + (uint32_t)((lane & 3) ^ (row >> 1 & 3)) * 16u;
   }
   // bytes that may be read from the tile's first element on: to the end of its last row
   template <bool T>
@@ -278,29 +286,37 @@ struct CeTile {
         for (int j = 0; j < NT; ++j) low[0][i][j] = low[1][i][j] = acc[i][j];
     }
     const int total = (k1 - k0) / BK;
-    const uint32_t va = offset<TA, BM>(A, wave, lane), vb = offset<TB, BN>(B, wave, lane);
-    const int64_t na = range<TA>(A, m0), nb = range<TB>(B, n0);
+    const uint32_t va = offset<TA, BM, BLOCKED_A>(A, wave, lane), vb = offset<TB, BN, true>(B, wave, lane);
+    const int64_t na = range<TA>(A, m0);
 
-    auto fetch = [&](auto t, auto br, auto n, const CeMat& x, const unsigned short* p, int64_t bytes, uint32_t v, unsigned short* to) {
+    auto to_lds = [&](const unsigned short* p, int64_t left, uint32_t v, unsigned short* to) {
+      const uint64_t base = reinterpret_cast<uint64_t>(p);
+      const i32x4 rs = {(int)(uint32_t)base, (int)(uint32_t)(base >> 32), left < 0 ? 0 : left > 0x7fffffff ? 0x7fffffff : (int)left, 0x00020000};
+      ce_to_lds(rs, v, to);
+    };
+    auto fetch = [&](auto t, auto br, auto n, auto blocked, const CeMat& x, int r0, int k, int64_t bytes, uint32_t v, unsigned short* to) {
+      constexpr bool T = decltype(t)::value != 0;
+      constexpr int BR = decltype(br)::value;
+      const unsigned short* p = x.p + (T ? (int64_t)k * x.ld + r0 : (int64_t)r0 * x.ld + k);
+      if (!decltype(blocked)::value && T && k >= x.k_tail) p = x.tail + (int64_t)(k - x.k_tail) * x.ld + r0;
 #pragma unroll
       for (int a = 0; a < PL; ++a) {
 #pragma unroll
         for (int i = 0; i < n.value; ++i) {
-          const int r = row0<t.value != 0, br.value>(wave) + hop<t.value != 0, br.value>(i);
-          const uint64_t base = reinterpret_cast<uint64_t>(p + a * x.plane + r * x.ld);
-          const int64_t left = bytes - r * x.ld * 2;
-          const i32x4 rs = {(int)(uint32_t)base, (int)(uint32_t)(base >> 32), left < 0 ? 0 : left > 0x7fffffff ? 0x7fffffff : (int)left, 0x00020000};
-          ce_to_lds(rs, v, to + a * PLANE + r * (t.value ? br.value : BK));
+          const int r = row0<T, BR>(wave) + hop<T, BR>(i);
+          unsigned short* const at = to + a * PLANE + r * (T ? BR : BK);
+          const int64_t strip = x.ld >> 5;  // blocks of a row of blocks
+          if (!decltype(blocked)::value) to_lds(p + a * x.plane + r * x.ld, bytes - r * x.ld * 2, v, at);
+          else if (T) to_lds(x.p + a * x.plane + (((k + r) >> 4) * strip + (r0 >> 5)) * 512 + (r & 15) * 32, (strip - (r0 >> 5)) * 1024 - (r & 15) * 64, v, at);  // to the end of the row of blocks
+          else to_lds(x.p + a * x.plane + (((r0 + r) >> 4) * strip + (k >> 5)) * 512, ((r0 + r) & ~15) < x.r_end ? 1024 : 0, v, at);
         }
       }
     };
     auto stage = [&](int it) {
       const int k = k0 + it * BK;
       unsigned short* const to = lds + it % ST * STAGE;
-      const unsigned short* pa = A.p + (TA ? (int64_t)k * A.ld + m0 : (int64_t)m0 * A.ld + k);
-      if (TA && k >= A.k_tail) pa = A.tail + (int64_t)(k - A.k_tail) * A.ld + m0;
-      fetch(Int<TA>{}, Int<BM>{}, Int<LA>{}, A, pa, na, va, to);
-      fetch(Int<TB>{}, Int<BN>{}, Int<LB>{}, B, B.p + (TB ? (int64_t)k * B.ld + n0 : (int64_t)n0 * B.ld + k), nb, vb, to + BM * BK);
+      fetch(Int<TA>{}, Int<BM>{}, Int<LA>{}, Int<BLOCKED_A>{}, A, m0, k, na, va, to);
+      fetch(Int<TB>{}, Int<BN>{}, Int<LB>{}, Int<1>{}, B, n0, k, 0, vb, to + BM * BK);
     };
     // waits until tile `it` is there for every wave; `ahead`: how many tiles behind it have been asked for.  Every wave has then read all that it read before.
     auto arrive = [&](int it, auto ahead) {
@@ -769,7 +785,7 @@ __global__ __launch_bounds__(1024) void ce_scale_kernel(const int32_t* __restric
   if (threadIdx.x == 0) scale[0] = top;
 }
 
-// dl of one piece of the vocabulary, [P][T][ldv]; columns behind the piece and the rows up to the next multiple of PAD are zero
+// dl of one piece of the vocabulary, [P][T][ldv], blocked; columns behind the piece and the rows up to the next multiple of PAD are zero
 template <class G, int PL, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(G::THREADS, 1) void ce_dlogits_kernel(CeMat W, CeMat h, const int32_t* __restrict__ n, const int32_t* __restrict__ yc, const float* __restrict__ lse,
                                                                 CeScale scale, int v0, int ldv, int64_t plane, int K, unsigned short* __restrict__ dl) {
@@ -808,7 +824,7 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_dlogits_kernel(CeMat W, CeMa
         for (int k = 0; k < 4; ++k)
           if (t >= N || vb + i * 16 + 4 * q + k >= Vc) g.acc[i][j][k] = 0.f;  // whatever was multiplied there
     }
-    // through LDS (the tiles are done with), so that rows leave in whole lines: token by token, its 16-byte pieces at piece ^ (token mod 16)
+    // through LDS (the tiles are done with), so that blocks leave in whole lines: token by token, its 16-byte pieces at piece ^ (token mod 16)
     const int tl = (wn * G::NT + j) * 16 + (lane & 15);
 #pragma unroll
     for (int i = 0; i < G::MT; ++i) {
@@ -834,9 +850,11 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_dlogits_kernel(CeMat W, CeMa
   for (int a = 0; a < PL; ++a) {
 #pragma unroll
     for (int c = 0; c < BN * PER / G::THREADS; ++c) {
-      const int at = c * G::THREADS + threadIdx.x, tl = at / PER, piece = at % PER, t = n0 + tl, v = m0 + piece * 8;
+      // a wave writes one block: 16 tokens x 32 columns
+      const int block = (c * G::THREADS + threadIdx.x) >> 6, l = threadIdx.x & 63, tl = block / (BM / 32) * 16 + (l >> 2), piece = block % (BM / 32) * 4 + (l & 3);
+      const int t = n0 + tl, v = m0 + piece * 8;
       if (t < Nz && v < ldv)
-        *reinterpret_cast<uint4*>(dl + a * plane + (int64_t)t * ldv + v) = *reinterpret_cast<const uint4*>(lds + a * BN * BM + tl * BM + (piece ^ (tl & (PER - 1) & 15)) * 8);
+        *reinterpret_cast<uint4*>(dl + a * plane + ce_place(t, v, ldv)) = *reinterpret_cast<const uint4*>(lds + a * BN * BM + tl * BM + (piece ^ (tl & (PER - 1) & 15)) * 8);
     }
   }
 }
