@@ -10,8 +10,8 @@
 // lies behind the last one that counts leaves at once (its number is read on the device, the host never waits for it).
 // The vocabulary is taken in pieces; of a piece only dl is held (bf16).  A product whose operand runs across the summed axis (W in dh, h and dl in
 // dW) reads it through the transposing LDS read, so nothing is ever stored transposed.  No float atomics: the pieces of a sum are added in a fixed order.
-// Measured, bf16, 8192 tokens (7373 count) x 1024 x 131072: statistics 1.85 ms (1.07 PFLOP/s), and per half of the vocabulary dl 1.07 ms (0.92), dh 0.88 ms (1.12),
-// dW 0.80 ms (1.24); 1.09 over all.  fp32, 16384 x 256 x 4096: 238, 271, 188 and 190 us (0.87, 0.76, 1.10, 1.08 PFLOP/s of bf16 products, a sixth of that in fp32).
+// Measured, bf16, 8192 tokens (7373 count) x 1024 x 131072: statistics 1.73 ms (1.14 PFLOP/s), and per half of the vocabulary dl 1.00 ms (0.99), dh 0.82 ms (1.20),
+// dW 0.80 ms (1.23); 1.13 over all.  fp32, 16384 x 256 x 4096: 212, 247, 179 and 195 us (0.97, 0.83, 1.15, 1.06 PFLOP/s of bf16 products, a sixth of that in fp32).
 #include <limits.h>
 #include "ceeg_internal.h"
 
