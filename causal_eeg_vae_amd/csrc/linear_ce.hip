@@ -235,6 +235,9 @@ struct CeTile {
   static_assert(LDS * 2 <= 160 * 1024, "LDS");
   // B is always a matrix made here, and blocked; A is W, which in bf16 lies as the caller has it, or (both across k) the hidden states
   static constexpr bool BLOCKED_A = PL == 3 || (TA && TB);
+  // A row-major along k, in the largest tile: two k tiles of it at a time, 128 bytes a row, for the same reason as the blocks' (8192 x 1024 x 131072 7.00 -> 6.91 ms,
+  // 5000 x 768 x 50257 forward 279 -> 271 us).
+  static constexpr bool PAIRS = !BLOCKED_A && !TA && BM == 256;
   f32x4 acc[MT][NT];
 
   // Load i of a wave fetches 64 pieces of 16 bytes of the tile: rows `row(lane) + hop(i)`; a hop changes no bit of a row that the swizzle looks at, so that
@@ -312,6 +315,18 @@ struct CeTile {
         }
       }
     };
+    // PAIRS: [2][BM][2 BK] of A, then [4][BN][BK] of B.  A row is 128 bytes, piece p of 16 at p ^ (r / 2 mod 8): 16 rows read together touch all banks once.
+    unsigned short* const lds_b = lds + 2 * BM * 2 * BK;
+    const uint32_t vp = (uint32_t)(lane >> 3) * (uint32_t)A.ld * 2u + (uint32_t)((lane & 7) ^ ((wave & 1) << 2 | lane >> 4)) * 16u;
+    auto stage_a = [&](int pair) {
+      const unsigned short* const p = A.p + (int64_t)m0 * A.ld + k0 + pair * 2 * BK;
+#pragma unroll
+      for (int i = 0; i < 2 * LA; ++i) {
+        const int r = wave * 8 + i * WAVES * 8;
+        to_lds(p + r * A.ld, na + 2 * BK - r * A.ld * 2, vp, lds + (pair & 1) * BM * 2 * BK + r * 2 * BK);
+      }
+    };
+    auto stage_b = [&](int it) { fetch(Int<TB>{}, Int<BN>{}, Int<LB>{}, Int<1>{}, B, n0, k0 + it * BK, 0, vb, lds_b + (it & 3) * BN * BK); };
     auto stage = [&](int it) {
       const int k = k0 + it * BK;
       unsigned short* const to = lds + it % ST * STAGE;
@@ -319,22 +334,40 @@ struct CeTile {
       fetch(Int<TB>{}, Int<BN>{}, Int<LB>{}, Int<1>{}, B, n0, k, 0, vb, to + BM * BK);
     };
     // waits until tile `it` is there for every wave; `ahead`: how many tiles behind it have been asked for.  Every wave has then read all that it read before.
-    auto arrive = [&](int it, auto ahead) {
-      if (it + ahead.value < total) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ahead.value * PL * (LA + LB)) : "memory");
+    auto arrive_when = [&](bool more, auto loads) {
+      if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(loads.value) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last tiles: nothing is asked for behind them
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
     };
+    auto arrive = [&](int it, auto ahead) { arrive_when(it + ahead.value < total, Int<ahead.value * PL * (LA + LB)>{}); };
     const int g = (l15 >> 2) | (q & 1) << 2, at = (q ^ (l15 >> 1 & 3)) * 8, row = 8 * q + (l15 >> 2);
-    auto read_a = [&](int it, int p, int i) { return read<TA, BM>(lds + it % ST * STAGE + p * PLANE, wm * MT + i, l15, at, row, g); };
-    auto read_b = [&](int it, int p, int j) { return read<TB, BN>(lds + it % ST * STAGE + p * PLANE + BM * BK, wn * NT + j, l15, at, row, g); };
+    auto read_a = [&](int it, int p, int i) {
+      if (PAIRS) return *reinterpret_cast<const bf16x8*>(lds + (it >> 1 & 1) * BM * 2 * BK + ((wm * MT + i) * 16 + l15) * 2 * BK + (((it & 1) * 4 + q) ^ l15 >> 1) * 8);
+      return read<TA, BM>(lds + it % ST * STAGE + p * PLANE, wm * MT + i, l15, at, row, g);
+    };
+    auto read_b = [&](int it, int p, int j) {
+      return read<TB, BN>(PAIRS ? lds_b + (it & 3) * BN * BK : lds + it % ST * STAGE + p * PLANE + BM * BK, wn * NT + j, l15, at, row, g);
+    };
 
     if constexpr (AHEAD) {
       // The next tile's fragments are read while this one's are multiplied, so that after a barrier no wave waits for LDS before it can go on.
+      static_assert(!PAIRS || (ST == 4 && PL == 1), "two pairs, four tiles");
+      if (PAIRS) {
+        stage_a(0);
+        stage_b(0);
+        stage_b(1);
+        if (total > 2) {
+          stage_a(1);
+          stage_b(2);
+          stage_b(3);
+        }
+      } else {
 #pragma unroll
-      for (int s = 0; s < ST; ++s)
-        if (s < total) stage(s);
+        for (int s = 0; s < ST; ++s)
+          if (s < total) stage(s);
+      }
       struct Frag {
         bf16x8 a[MT], b[NT];
       };
@@ -351,11 +384,19 @@ struct CeTile {
           for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.a[i], f.b[j], acc[i][j], 0, 0, 0);
       };
       Frag f0, f1;
-      arrive(0, Int<ST - 1>{});
+      // PAIRS: the order is A of tiles 0 and 1, B0, B1, A of 2 and 3, B2, B3, B4, A of 4 and 5, B5, B6, ...
+      if (PAIRS) arrive_when(total > 2, Int<2 * LA + 3 * LB>{});
+      else arrive(0, Int<ST - 1>{});
       load(f0, 0);
-      auto step = [&](int it, const Frag& now, Frag& next) {
-        arrive(it + 1, Int<ST - 2>{});
-        if (it + ST < total) stage(it + ST);
+      auto step = [&](int it, auto odd, const Frag& now, Frag& next) {
+        if (PAIRS) {
+          arrive_when(it + 3 < total, Int<odd.value ? 2 * LB : 2 * LA + 2 * LB>{});
+          if (odd.value && it + 3 < total) stage_a((it + 3) >> 1);
+          if (it + 4 < total) stage_b(it + 4);
+        } else {
+          arrive(it + 1, Int<ST - 2>{});
+          if (it + ST < total) stage(it + ST);
+        }
         load(next, it + 1);
         mul(now);
         constexpr int READS = MT * (TA ? 2 : 1) + NT * (TB ? 2 : 1), EACH = MT * NT / READS;
@@ -366,10 +407,10 @@ struct CeTile {
         }
       };
       for (int it = 0; it + 2 < total; it += 2) {
-        step(it, f0, f1);
-        step(it + 1, f1, f0);
+        step(it, Int<0>{}, f0, f1);
+        step(it + 1, Int<1>{}, f1, f0);
       }
-      step(total - 2, f0, f1);
+      step(total - 2, Int<0>{}, f0, f1);
       mul(f1);
     } else {
 #pragma unroll
