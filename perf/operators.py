@@ -220,23 +220,17 @@ def _random_words(s):
     return torch.stack(c, 1).view(-1)
 
 
-def _held(x, r16, second):
-    """x in 8 bits: e4m3 numbers times one scale a block.  A magnitude is rounded up with the probability that keeps its expectation, for the second
-    moment, which is held as its root, the expectation of the square."""
+def _held(x, r16, keep_positive):
+    """x in 8 bits: e4m3 numbers times one scale a block, each rounded up with the probability of what rounding down leaves out."""
     x = x.view(-1, BLOCK)
     top = x.abs().amax(1)
     none = top < TINY
     scale = torch.where(none, torch.zeros_like(top), top / TOP)
     y = torch.where(none[:, None], torch.zeros_like(x), x.abs() / scale[:, None]).clamp_(max=TOP).view(-1)
-    bits, small = y.view(torch.int32), y < 2.0 ** -6
-    code = torch.where(small, (y * 512).int(), (bits >> 20) - (120 << 3))       # the number below
-    low = torch.where(small, code * 2.0 ** -9, (bits & -(1 << 20)).view(torch.float32))
-    step = torch.where(small, torch.full_like(y, 2.0 ** -9), ((bits & 0x7F800000) - (3 << 23)).view(torch.float32))
-    share = (y - low) / step
-    if second:
-        share = share * (y + low) / (low + low + step)
-    code = code + (share * 65536 + r16 >= 65536).int()
-    if second:
+    normal = ((y.view(torch.int32) + (r16 << 4)) >> 20) - (120 << 3)
+    small = torch.floor(y * 512 + r16.float() / 65536).int()
+    code = torch.where(y >= 2.0 ** -6, normal, small)
+    if keep_positive:
         code = torch.where((y > 0) & (code == 0), torch.ones_like(code), code)
     code = code | (torch.signbit(x).view(-1).int() << 7)
     return code.to(torch.uint8).view(torch.float8_e4m3fn), scale
@@ -251,8 +245,8 @@ def _adamw8(s):
     v = b2 * (u * u) + (1 - b2) * (g * g)
     _moved(s, m, v)
     r = _random_words(s)
-    for x, key, r16, second in ((m, "m", r & 0xFFFF, False), (v.sqrt(), "v", r >> 16, True)):
-        code, scale = _held(x, r16.float(), second)
+    for x, key, r16, positive in ((m, "m", r & 0xFFFF, False), (v.sqrt(), "v", r >> 16, True)):
+        code, scale = _held(x, r16.int(), positive)
         s[key].copy_(code)
         s[key + "_scale"].copy_(scale)
 
@@ -357,8 +351,7 @@ def _exact_adamw(s):
             wide = scale.repeat_interleave(BLOCK)[:n]
             y = torch.where(wide > 0, x.abs() / wide, torch.zeros_like(x)).clamp(max=TOP)
             low = (torch.searchsorted(grid, y, right=True) - 1).clamp(0, 125)
-            at = (lambda z: z * z) if q is vj else (lambda z: z)
-            up = (at(y) - at(grid[low])) / (at(grid[low + 1]) - at(grid[low])) + r.double() / 65536 >= 1
+            up = (y - grid[low]) / (grid[low + 1] - grid[low]) + r.double() / 65536 >= 1
             code = low + up.long()
             if q is vj:
                 code = torch.where((y > 0) & (code == 0), torch.ones_like(code), code)
