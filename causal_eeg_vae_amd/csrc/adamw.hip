@@ -2,8 +2,9 @@
 //   m = b1 m + (1 - b1) g;   v = b2 v + (1 - b2) g^2;   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
 // 8 bits: m and sqrt(v) (the root halves the range of exponents that has to fit) are e4m3 numbers times one fp32 scale per 256 consecutive elements, the
 // block's largest magnitude / 448.  A step changes v by 1 - b2 of itself, far less than half a step of an 8-bit number, so rounding to
-// nearest would hold v where it is for ever; a magnitude is therefore rounded UP with the probability that keeps the expectation - of m, and
-// of v itself: keeping that of the root would add the rounding's variance to v, up to 2^-8 of it a step, which outgrows the decay 1 - b2.
+// nearest would hold v where it is for ever; a magnitude is therefore rounded UP with the probability of what rounding down leaves out, which keeps the
+// expectation of m and of sqrt(v), what the update divides by.  v itself, the root's square, comes out larger by the rounding's variance: 4 % of v once it has
+// settled, and the root 0.8 % (normal gradients, b2 = 0.99 and 0.999 alike).
 // 16 random bits of Philox per value.  sqrt(v) > 0 never becomes 0: a denominator that vanishes while m does not would blow the next step up.
 // Bound: HBM bytes (fp32 28 per element; 8 bits 16 with fp32 parameters, 10 with bf16).  A wave takes one block of 256 elements, 4 per lane - 16-byte loads, the
 // block's maximum by one butterfly, one Philox call per lane for its four elements - so the 8-bit form needs no LDS and no barrier.
@@ -147,21 +148,16 @@ __device__ __forceinline__ float aw_quotient(float a, float b, float r) {
   const float q = a * r;
   return __fmaf_rn(__fmaf_rn(-q, b, a), r, q);
 }
-// x / scale as an e4m3 number, rounded by the 16 random bits `rnd` so that the expectation of its magnitude (SECOND: of its square) is kept.  per_scale: 1 / scale,
-// 0 where the scale is.  Between the numbers L s and (L + 1) s (s: their distance, L < 16) the magnitude is (L + share) s, and
-//   (y^2 - low^2) / (high^2 - low^2) = share (2 L + share) / (2 L + 1).
+// x / scale as an e4m3 number, rounded by the 16 random bits `rnd` so that the expectation of its magnitude is kept.  per_scale: 1 / scale, 0 where the scale is.
+// SECOND: a magnitude > 0 does not become 0.
 template <bool SECOND, bool FINITE>
 __device__ __forceinline__ uint32_t aw_round(float x, float scale, float per_scale, float rnd) {
   const float a = fabsf(x), y = fminf(aw_quotient(a, scale, per_scale), AW_TOP);
   const uint32_t u = __float_as_uint(y);
   const bool small = y < 0x1p-6f;  // there the numbers are 2^-9 apart
   const float t = y * 512.f, below = floorf(t);
-  float share = small ? t - below : (float)(u & 0xfffffu) * 0x1p-20f;
+  const float share = small ? t - below : (float)(u & 0xfffffu) * 0x1p-20f;
   uint32_t c = small ? (uint32_t)below : (u >> 20) - (120u << 3);
-  if (SECOND) {
-    const float l2 = small ? below + below : (float)(16u + 2u * (c & 7u)), d = l2 + 1.f;
-    share = aw_quotient(share * (l2 + share), d, aw_reciprocal(d));
-  }
   c += share * 65536.f + rnd >= 65536.f;
   if (SECOND && c == 0u && y > 0.f) c = 1u;
   if (!FINITE && !aw_finite(x)) c = 0x7fu;  // stays a NaN

@@ -620,7 +620,7 @@ int ceeg_balance_bwd(const void* scores, int64_t ld, int dtype, int64_t T, int E
  * arguments, 56 tensors a launch, so nothing has to outlive the call.  dtype: of p and g.  Empty tensors are skipped (and keep their place).
  * state_bits 32: m, v fp32.  state_bits 8: m and sqrt(v) as e4m3 bytes times one fp32 scale per ceeg_adamw_block() = 256 consecutive elements
  * (scale = largest finite magnitude * fl(1 / 448); below 2^-100 the block is held as zeros); a magnitude is rounded up with the probability that
- * keeps the expectation of m, or of v, by 16 bits of Philox 4x32-10 (key seed; counter {element / 4, 0x41444D57, place of the tensor}; word element % 4,
+ * keeps the expectation of m, or of sqrt(v), by 16 bits of Philox 4x32-10 (key seed; counter {element / 4, 0x41444D57, place of the tensor}; word element % 4,
  * low half for m, high half for v); sqrt(v) > 0 never becomes 0.  A gradient that is not finite makes its element NaN and nothing else.
  * step >= 1: the number of this step.  lr_dev / step_dev (fp32 on the device, or NULL) replace lr / step where a captured graph replays the call;
  * with step_dev the key is seed + step * 0x9E3779B97F4A7C15.

@@ -1,0 +1,114 @@
+"""GPU: the 8-bit moments of adamw_step_ against a restatement of their rounding in numpy: m and sqrt(v) as e4m3 numbers times a scale per block of 256,
+each magnitude rounded up with the probability of what rounding down leaves out.
+
+Codes and scales are compared exactly: every operation of the restatement is one fp32 operation, rounded as the kernel's.  The parameter's bound (u =
+2^-24): m is two products and a sum (3 u of their magnitudes), the update a root, two products and a quotient by a reciprocal (10 u of it), p two u of itself
+and half a step of its type."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+HYPER = dict(step=7, lr=2e-3, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1)
+GRID = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).float().numpy()   # the numbers of e4m3 that are not negative
+
+
+def _random_words(n, seed, tensor):
+    """Philox 4x32-10, key `seed`: element i takes word i % 4 of the counter (i / 4, tag, tensor)."""
+    mask = np.uint64(0xFFFFFFFF)
+    q = np.arange(-(-n // 4), dtype=np.uint64)
+    c = [q & mask, q >> np.uint64(32), np.full_like(q, 0x41444D57), np.full_like(q, tensor)]
+    k = [np.uint64(seed & 0xFFFFFFFF), np.uint64(seed >> 32)]
+    for _ in range(10):
+        a, b = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
+        c = [(b >> np.uint64(32)) ^ c[1] ^ k[0], b & mask, (a >> np.uint64(32)) ^ c[3] ^ k[1], a & mask]
+        k = [(k[0] + np.uint64(0x9E3779B9)) & mask, (k[1] + np.uint64(0xBB67AE85)) & mask]
+    return np.stack(c, 1).reshape(-1)[:n].astype(np.int64)
+
+
+def _held(x, r16, root):
+    """Finite fp32 x in 8 bits: (codes, scales)."""
+    n, pad = x.size, -x.size % 256
+    a = np.pad(np.abs(x), (0, pad)).reshape(-1, 256)
+    top = a.max(1)
+    scale = np.where(top < 2.0 ** -100, np.float32(0), top * (np.float32(1) / np.float32(448))).astype(np.float32)
+    with np.errstate(divide="ignore", invalid="ignore"):
+        y = np.where(scale[:, None] > 0, np.minimum(a / scale[:, None], np.float32(448)), np.float32(0)).reshape(-1)[:n]
+    code = np.clip(np.searchsorted(GRID, y, side="right") - 1, 0, 126)
+    step = np.where(code < 126, GRID[np.minimum(code + 1, 126)] - GRID[code], np.float32(32)).astype(np.float32)
+    code = code + ((y - GRID[code]) / step * np.float32(65536) + r16.astype(np.float32) >= 65536)
+    if root:
+        code = np.where((y > 0) & (code == 0), 1, code)
+    return (code | np.signbit(x).astype(np.int64) << 7).astype(np.uint8), scale
+
+
+def _state(x):
+    """An 8-bit state near given fp32 values."""
+    from causal_eeg_vae_amd.optim import BLOCK, block_state
+    q, s = block_state(x)
+    a = torch.nn.functional.pad(x, (0, -x.numel() % BLOCK)).view(-1, BLOCK)
+    s.copy_(a.abs().amax(1) / 448)
+    q.copy_((a / s.clamp(min=1e-30)[:, None]).view(-1)[:x.numel()].to(torch.float8_e4m3fn))
+    return q, s
+
+
+def _case(sizes, dtype, seed, spread):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rnd = lambda n: torch.randn(n, generator=g, device="cuda")  # noqa: E731
+    p = [rnd(n).to(dtype) for n in sizes]
+    gr = [(rnd(n) * torch.exp(spread * rnd(n))).to(dtype) for n in sizes]
+    return p, gr, [_state(rnd(n) * 0.3) for n in sizes], [_state(rnd(n).abs()) for n in sizes]
+
+
+def _check(sizes, dtype, seed=0x123456789ABCDEF, spread=3.0):
+    from causal_eeg_vae_amd import adamw_step_
+    from causal_eeg_vae_amd.optim import block_values
+    p, g, m, v = _case(sizes, dtype, len(sizes), spread)
+    mf, uf, before = [block_values(x) for x in m], [block_values(x) for x in v], [x.double() for x in p]
+    adamw_step_(p, g, m, v, seed=seed, **HYPER)
+    (b1, b2), (o1, o2) = [np.float32(b) for b in HYPER["betas"]], [np.float32(1 - b) for b in HYPER["betas"]]
+    for j, n in enumerate(sizes):
+        gf, a, u = (x.float().cpu().numpy() for x in (g[j], mf[j], uf[j]))
+        w = _random_words(n, seed, j)
+        m1, v1 = b1 * a + o1 * gf, b2 * (u * u) + o2 * (gf * gf)
+        for (codes, scales), (c, s) in zip((m[j], v[j]), (_held(m1, w & 0xFFFF, False), _held(np.sqrt(v1), w >> 16, True))):
+            np.testing.assert_array_equal(codes.view(torch.uint8).cpu().numpy(), c, err_msg=f"tensor {j}")
+            np.testing.assert_array_equal(scales.cpu().numpy(), s)
+        gd, md, ud = g[j].double(), mf[j].double(), uf[j].double()
+        md, size = HYPER["betas"][0] * md + (1 - HYPER["betas"][0]) * gd, HYPER["betas"][0] * md.abs() + (1 - HYPER["betas"][0]) * gd.abs()
+        den = ((HYPER["betas"][1] * ud * ud + (1 - HYPER["betas"][1]) * gd * gd) / (1 - HYPER["betas"][1] ** HYPER["step"])).sqrt() + HYPER["eps"]
+        up = HYPER["lr"] / (1 - HYPER["betas"][0] ** HYPER["step"]) / den
+        want = before[j] * (1 - HYPER["lr"] * HYPER["weight_decay"]) - up * md
+        tol = 4 * U * before[j].abs() + up * U * (3 * size + 10 * md.abs()) + torch.finfo(dtype).eps / 2 * want.abs() + 1e-42
+        assert bool(((p[j].double() - want).abs() <= tol).all()), f"parameter {j}"
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("sizes", [[1], [3, 0, 255, 256, 257, 1024, 1025], [5000, 2], [40 + i for i in range(70)], [300000]], ids=str)
+def test_codes_scales_and_parameters(sizes, dtype):
+    _check(sizes, dtype)
+
+
+@pytest.mark.parametrize("root", [1.03, 1.0625, 1.18, 1.9])
+def test_the_expectation_of_the_root_is_kept(root):
+    """One step of n = 2^20 elements that all come to the same root, between two numbers of e4m3 (low = 8 steps or more, step = 1/8): every new root is one of the
+    two, and their mean is the root to 6 standard deviations of at most step / 2 / sqrt(n) (0.003 steps), 2^-16 of a step for the 16 random bits and 4 u
+    of the root.  Keeping the expectation of the square instead would put the mean share (1 - share) step / (2 low + step) of a step lower (share 1/2 at
+    8 steps: 0.0147)."""
+    from causal_eeg_vae_amd import adamw_step_
+    from causal_eeg_vae_amd.optim import block_state, block_values
+    n, b2 = 1 << 20, 0.25
+    p = torch.zeros(n, device="cuda")
+    m, v = block_state(p), block_state(p)
+    v[1].fill_(1.0)
+    v[0].copy_(torch.full((n,), 2.0, device="cuda").to(torch.float8_e4m3fn))
+    g = torch.full((n,), ((root * root - b2 * 4) / (1 - b2)) ** 0.5, device="cuda")
+    v[0].view(torch.uint8)[::256] = 0x7E      # 448, and a gradient that keeps it there: it holds the block's scale
+    g[::256] = 448.0
+    adamw_step_([p], [g], [m], [v], step=3, betas=(0.9, b2), seed=11)
+    got = block_values(v).double()[torch.arange(n, device="cuda") % 256 != 0] / float(v[1][0])
+    want = root / float(v[1][0])
+    low = int(want * 8) / 8
+    assert bool(((got == low) | (got == low + 0.125)).all())
+    assert abs(float(got.mean()) - want) <= 0.125 * (0.003 + 2.0 ** -16) + 4 * U * want
