@@ -22,6 +22,14 @@ def _same_device(*tensors):
         raise ValueError(f"all tensors must be on one device, got {[str(t.device) for t in tensors if t is not None]}")
 
 
+def _weight_rows(weight, dtype):
+    """(weight, row stride) as the entries take it: a copy where its strides or its alignment do not allow to read it in place."""
+    V, H = weight.shape
+    if weight.stride(1) != 1 or (V > 1 and not H <= weight.stride(0) <= 1 << 22) or (dtype == _lib.CEEG_BF16 and (weight.data_ptr() % 16 or not weight.is_contiguous())):
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    return weight, H if weight.is_contiguous() else weight.stride(0)
+
+
 def _linear_ce(hidden, weight, target, ignore_index, reduction):
     """The loss, and what the backward takes back."""
     L = _lib.lib()
@@ -30,10 +38,9 @@ def _linear_ce(hidden, weight, target, ignore_index, reduction):
     dev = hidden.device
     if hidden.stride(1) != 1 or (T > 1 and hidden.stride(0) < H):
         hidden = hidden.contiguous()
-    if weight.stride(1) != 1 or (V > 1 and not H <= weight.stride(0) <= 1 << 22) or (dtype == _lib.CEEG_BF16 and (weight.data_ptr() % 16 or not weight.is_contiguous())):
-        weight = weight.clone(memory_format=torch.contiguous_format)
+    weight, ldw = _weight_rows(weight, dtype)
     target = target.contiguous()
-    ldh, ldw = max(hidden.stride(0), H), H if weight.is_contiguous() else weight.stride(0)
+    ldh = max(hidden.stride(0), H)
     with _lib.on(dev):
         loss = torch.empty(T if reduction == 0 else (), dtype=torch.float32, device=dev)
         # one buffer for what the backward takes back: the packed rows, lse [T], tokens [3 T + 1]
@@ -46,7 +53,7 @@ def _linear_ce(hidden, weight, target, ignore_index, reduction):
             _lib.check(L.ceeg_linear_ce_fwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, target.data_ptr(), T, H, V, dtype, ignore_index, reduction,
                                             loss.data_ptr(), lse, tokens, packed, ws.data_ptr(), ws.numel(), _lib.stream()),
                        "ceeg_linear_ce_fwd")
-    return loss, kept, weight, (T, H, V, ldw, dtype, reduction, rows)
+    return loss, kept, weight, (T, H, V, dtype, reduction, rows)
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
@@ -60,8 +67,12 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         kept, weight = ctx.saved_tensors
-        T, H, V, ldw, dtype, reduction, rows = ctx.sizes
+        T, H, V, dtype, reduction, rows = ctx.sizes
         L = _lib.lib()
+        # saved tensors may come back through a hook as other tensors of the same values: strides and alignment are theirs, not those of the forward
+        weight, ldw = _weight_rows(weight, dtype)
+        if kept.data_ptr() % 256 or not kept.is_contiguous():
+            kept = kept.clone(memory_format=torch.contiguous_format)
         dev = weight.device
         need_h, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         with _lib.on(dev):

@@ -1,0 +1,47 @@
+"""GPU: linear_cross_entropy at values that are not finite, in forward mode and where saved tensors come back as other tensors."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BOTH = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+
+
+def _inputs(T, H, V, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed * 7919 + T * 31 + H * 17 + V)
+    h = torch.randn(T, H, generator=g, device="cuda").to(dtype)
+    w = (torch.randn(V, H, generator=g, device="cuda") * (2 / H ** 0.5)).to(dtype)
+    return h, w, torch.randint(0, V, (T,), generator=g, device="cuda")
+
+
+def _run(h, w, y, reduction="mean", g=None):
+    from causal_eeg_vae_amd import linear_cross_entropy
+    a, b = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    loss = linear_cross_entropy(a, b, y, reduction=reduction)
+    return (loss.detach(),) + torch.autograd.grad(loss, (a, b), torch.ones_like(loss) if g is None else g)
+
+
+def _moved(x):
+    """The values of x in a tensor of other strides and alignment."""
+    if x.dim() < 2:
+        return torch.cat((x.new_zeros(3), x))[3:]
+    return torch.cat((x.new_zeros(x.shape[0], 3), x, x.new_zeros(x.shape[0], 2)), 1)[:, 3:3 + x.shape[1]]
+
+
+@BOTH
+@pytest.mark.parametrize("T,H,V", [(5, 64, 300), (60, 64, 333), (60, 70, 333), (1, 64, 1)])
+def test_saved_tensors_that_come_back_as_others(T, H, V, dtype):
+    """What a hook hands back holds the same values, not the same strides or alignment."""
+    h, w, y = _inputs(T, H, V, dtype)
+    wide = torch.full((V, H + 11), 9.0, dtype=dtype, device="cuda")
+    wide[:, :H] = w
+    want = _run(h, w, y)
+    for weight in (w, wide[:, :H]):
+        for unpack in (lambda x: x.clone(memory_format=torch.contiguous_format), _moved, lambda x: x.clone() if x.dim() < 2 else x.t().contiguous().t()):
+            with torch.autograd.graph.saved_tensors_hooks(lambda x: x, unpack):
+                got = _run(h, weight, y)
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+        with torch.autograd.graph.save_on_cpu():
+            got = _run(h, weight, y)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)

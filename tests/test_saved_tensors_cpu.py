@@ -1,0 +1,67 @@
+"""CPU: what the backward of linear_cross_entropy and of balance_loss hands to the library where saved tensors come back with other strides, as
+torch.autograd.graph.save_on_cpu gives them: rows that a stride walks have to lie inside the tensor.  The library is replaced by one that only records."""
+import contextlib
+
+import pytest
+import torch
+
+
+class _Recorder:
+    def __init__(self):
+        self.calls = {}
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls[name] = args
+            return 4096 if name.endswith("bytes") else 0
+        return call
+
+
+@pytest.fixture
+def library(monkeypatch):
+    from causal_eeg_vae_amd import _lib
+    rec = _Recorder()
+    monkeypatch.setattr(_lib, "lib", lambda: rec)
+    monkeypatch.setattr(_lib, "require_cuda", lambda *t: None)
+    monkeypatch.setattr(_lib, "on", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(_lib, "stream", lambda: None)
+    return rec
+
+
+def _hooks(back):
+    """Saved tensors go away as copies and come back as `back` makes them; the last matrix that did."""
+    seen = []
+
+    def unpack(x):
+        y = back(x)
+        if y.dim() == 2:
+            seen.append(y)
+        return y
+
+    return torch.autograd.graph.saved_tensors_hooks(lambda x: x, unpack), seen
+
+
+BACK = {"packed": lambda x: x.clone(memory_format=torch.contiguous_format), "transposed": lambda x: x.t().contiguous().t() if x.dim() == 2 else x.clone(),
+        "wider": lambda x: torch.cat((x, x), 1)[:, :x.shape[1]] if x.dim() == 2 else x.clone()}
+
+
+def _inside(pointer, ld, rows, cols, given):
+    """`rows` rows of `cols`, `ld` apart, from `pointer` on: inside the tensor that was given back, or packed rows of a copy."""
+    if pointer != given.data_ptr():
+        return ld == cols
+    size = given.untyped_storage().nbytes() // given.element_size() - given.storage_offset()
+    return ld >= cols and (rows - 1) * ld + cols <= size and (rows == 1 or ld == given.stride(0)) and given.stride(1) == 1
+
+
+@pytest.mark.parametrize("back", list(BACK))
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_linear_cross_entropy(library, back, dtype):
+    from causal_eeg_vae_amd import linear_cross_entropy
+    V, H, T = 50, 8, 7
+    w = torch.zeros(V, H + 3, dtype=dtype)[:, :H].requires_grad_(True)
+    hooks, seen = _hooks(BACK[back])
+    with hooks:
+        loss = linear_cross_entropy(torch.zeros(T, H, dtype=dtype), w, torch.zeros(T, dtype=torch.int64))
+        torch.autograd.grad(loss, w)
+    packed, weight, ldw = library.calls["ceeg_linear_ce_bwd"][:3]
+    assert _inside(weight, ldw, V, H, seen[-1])
