@@ -120,6 +120,14 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
     return loss.view(target.shape) if reduction == "none" else loss
 
 
+def _score_rows(scores):
+    """(scores, row stride) as the entries take them."""
+    T, E = scores.shape
+    if scores.stride(1) != 1 or (T > 1 and scores.stride(0) < E):
+        scores = scores.contiguous()
+    return scores, max(scores.stride(0), E)
+
+
 class _Balance(torch.autograd.Function):
     @staticmethod
     def forward(ctx, scores, indices, mask):
@@ -127,11 +135,9 @@ class _Balance(torch.autograd.Function):
         dtype = _dtype(scores, "scores")
         (T, E), K = scores.shape, indices.shape[1]
         dev = scores.device
-        if scores.stride(1) != 1 or (T > 1 and scores.stride(0) < E):
-            scores = scores.contiguous()
+        scores, ld = _score_rows(scores)
         indices = indices.contiguous()
         mask = None if mask is None else mask.contiguous()
-        ld = max(scores.stride(0), E)
         with _lib.on(dev):
             loss = torch.empty(1, dtype=torch.float32, device=dev)
             counts = torch.empty(E, dtype=torch.int64, device=dev)
@@ -142,7 +148,7 @@ class _Balance(torch.autograd.Function):
                                               loss.data_ptr(), counts.data_ptr(), stats.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream()),
                            "ceeg_balance_fwd")
         ctx.save_for_backward(scores, mask, stats)
-        ctx.sizes = T, E, ld, dtype
+        ctx.sizes = T, E, dtype
         ctx.mark_non_differentiable(counts)
         return loss[0], counts
 
@@ -150,8 +156,11 @@ class _Balance(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _g_counts):
         scores, mask, stats = ctx.saved_tensors
-        T, E, ld, dtype = ctx.sizes
+        T, E, dtype = ctx.sizes
         dev = scores.device
+        # saved tensors may come back through a hook as other tensors of the same values: strides are theirs, not those of the forward
+        scores, ld = _score_rows(scores)
+        mask, stats = None if mask is None else mask.contiguous(), stats.contiguous()
         with _lib.on(dev):
             g = g.to(torch.float32).contiguous()
             ds = torch.empty(T, E, dtype=scores.dtype, device=dev)

@@ -65,3 +65,17 @@ def test_linear_cross_entropy(library, back, dtype):
         torch.autograd.grad(loss, w)
     packed, weight, ldw = library.calls["ceeg_linear_ce_bwd"][:3]
     assert _inside(weight, ldw, V, H, seen[-1])
+
+
+@pytest.mark.parametrize("back", list(BACK))
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_balance_loss(library, back, dtype):
+    from causal_eeg_vae_amd import balance_loss
+    T, E = 50, 8
+    s = torch.zeros(T, E + 3, dtype=dtype)[:, :E].requires_grad_(True)
+    hooks, seen = _hooks(BACK[back])
+    with hooks:
+        loss, _ = balance_loss(s, torch.zeros(T, dtype=torch.int64))
+        torch.autograd.grad(loss, s)
+    scores, ld = library.calls["ceeg_balance_bwd"][:2]
+    assert _inside(scores, ld, T, E, seen[-1])
