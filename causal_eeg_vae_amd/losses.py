@@ -22,6 +22,10 @@ def _same_device(*tensors):
         raise ValueError(f"all tensors must be on one device, got {[str(t.device) for t in tensors if t is not None]}")
 
 
+def _has_tangent(t):
+    return torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+
+
 def _weight_rows(weight, dtype):
     """(weight, row stride) as the entries take it: a copy where its strides or its alignment do not allow to read it in place."""
     V, H = weight.shape
@@ -94,7 +98,8 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
     hidden [..., H], weight [V, H] (both float32 or both bfloat16), target [...] int64 of hidden's leading shape.  Tokens whose target is
     `ignore_index` (padding) take no part, whatever their hidden row holds.  reduction: "mean" over the tokens that count (0 where none does),
     "sum", or "none" (target's shape, 0 where ignored).  The loss is float32; the gradients have their inputs' types, all sums are float32.
-    A target outside [0, V) makes the loss and the gradients it reaches NaN: an error would need a host read of the targets."""
+    A target outside [0, V) makes the loss and the gradients it reaches NaN: an error would need a host read of the targets.
+    There is no forward mode: a tangent is a NotImplementedError."""
     if not all(isinstance(t, torch.Tensor) for t in (hidden, weight, target)):
         raise TypeError("hidden, weight and target must be tensors")
     if reduction not in _REDUCTIONS:
@@ -113,8 +118,8 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
         none = hidden.float().sum(-1) + weight[:0].float().sum()
         return none if reduction == "none" else none.sum()
     args = hidden.reshape(-1, hidden.shape[-1]), weight, target.reshape(-1), int(ignore_index), _REDUCTIONS[reduction]
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-        loss = _LinearCrossEntropy.apply(*args)
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad) or _has_tangent(hidden) or _has_tangent(weight):
+        loss = _LinearCrossEntropy.apply(*args)   # which refuses forward mode
     else:  # nothing comes back: autograd's part of the call is left out
         loss = _linear_ce(*args)[0]
     return loss.view(target.shape) if reduction == "none" else loss

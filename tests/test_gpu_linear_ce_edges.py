@@ -20,6 +20,20 @@ def _run(h, w, y, reduction="mean", g=None):
     return (loss.detach(),) + torch.autograd.grad(loss, (a, b), torch.ones_like(loss) if g is None else g)
 
 
+def test_forward_mode_is_refused():
+    """A tangent that would be dropped is an error, with and without anything that asks for a gradient."""
+    import torch.autograd.forward_ad as fwd
+    from causal_eeg_vae_amd import linear_cross_entropy
+    h, w, y = _inputs(20, 64, 100, torch.float32)
+    with fwd.dual_level():
+        for a, b in ((fwd.make_dual(h, torch.ones_like(h)), w), (h, fwd.make_dual(w, torch.ones_like(w)))):
+            with pytest.raises(NotImplementedError):
+                linear_cross_entropy(a, b, y)
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                linear_cross_entropy(a, b, y, reduction="none")
+        linear_cross_entropy(h, w, y)       # no tangent: nothing to refuse
+
+
 def _moved(x):
     """The values of x in a tensor of other strides and alignment."""
     if x.dim() < 2:
