@@ -807,7 +807,7 @@ __global__ __launch_bounds__(1024) void ce_few_loss_kernel(const int32_t* __rest
 struct CeScale {
   const float* g;
   int reduction;
-  const float *top, *r;  // no reduction: s = the largest |g|, r_j = g_j / s
+  const float *top, *r;  // no reduction: s = the largest finite |g|, r_j = g_j / s; what is not finite is its token's own r and leaves the others' alone
   __device__ __forceinline__ float s(int N) const { return reduction == 0 ? top[0] : reduction == 1 ? g[0] / (float)(N > 0 ? N : 1) : g[0]; }
   __device__ __forceinline__ float row(int j, int y) const { return y < 0 ? __uint_as_float(0x7fc00000u) : reduction == 0 ? r[j] : 1.f; }
 };
@@ -816,7 +816,10 @@ __global__ __launch_bounds__(1024) void ce_scale_kernel(const int32_t* __restric
   __shared__ float s[16];
   const int N = n[0];
   float top = 0.f;
-  for (int j = threadIdx.x; j < N; j += 1024) top = fmaxf(top, fabsf(g[rows[j]]));
+  for (int j = threadIdx.x; j < N; j += 1024) {
+    const float x = fabsf(g[rows[j]]);
+    if (x <= 3.402823466e38f) top = fmaxf(top, x);
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = top;

@@ -584,7 +584,7 @@ int ceeg_neg_sample_uniform_filtered(const int32_t* rowptr, const int32_t* col, 
  * reduction 0: loss [T]; 1: mean over the tokens that count (0 where none does) -> loss [1]; 2: sum -> loss [1].
  * lse [T] fp32, tokens [3 T + 1] int32 (how many tokens count, which, their place and class) and packed (ceeg_linear_ce_packed_bytes(), 256-byte aligned: their
  * rows of h as the products read them) are written by the forward for the backward.
- * g: what comes back for loss (fp32, [T] or [1]).  dh [T, H] and dW [V, H] contiguous, either may be NULL.
+ * g: what comes back for loss (fp32, [T] or [1]); a value of [T] that is not finite reaches its token's row of dh alone, and all of dW.  dh [T, H] and dW [V, H] contiguous, either may be NULL.
  * Limits: T <= 2^22, H <= 2^15, V <= 2^28, ldw <= 2^22; bf16 with H a multiple of 64 reads W in place: 16-byte aligned, ldw = H.
  * The backward's workspace holds dl for a piece of the vocabulary; pieces are chosen so that they take about 1 GiB at most together.
  * ----------------------------------------------------------------------------------------------*/

@@ -20,6 +20,22 @@ def _run(h, w, y, reduction="mean", g=None):
     return (loss.detach(),) + torch.autograd.grad(loss, (a, b), torch.ones_like(loss) if g is None else g)
 
 
+@BOTH
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("T", [3, 70])
+def test_an_upstream_value_that_is_not_finite_stays_with_its_token(T, bad, dtype):
+    h, w, y = _inputs(T, 72, 300, dtype)
+    g = torch.linspace(-1.5, 2.0, T, device="cuda")
+    g[1] = 0.0
+    _, clean, _ = _run(h, w, y, "none", g)
+    g[1] = bad
+    _, dh, dw = _run(h, w, y, "none", g)
+    others = torch.arange(T, device="cuda") != 1
+    assert torch.equal(dh[others], clean[others]) and not bool(torch.isfinite(dh[1]).any()) and not bool(torch.isfinite(dw).any())
+    g[:] = bad
+    assert not bool(torch.isfinite(_run(h, w, y, "none", g)[1]).any())
+
+
 def test_forward_mode_is_refused():
     """A tangent that would be dropped is an error, with and without anything that asks for a gradient."""
     import torch.autograd.forward_ad as fwd
