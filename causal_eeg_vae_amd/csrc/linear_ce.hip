@@ -444,7 +444,14 @@ struct CeTile {
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] += (low[0][i][j] + low[1][i][j] * 0x1p-8f) * 0x1p-8f;
+        for (int j = 0; j < NT; ++j) {
+          // An infinite factor lies in its first plane alone and meets the other's lower planes, zeros and other signs among them: where the first planes'
+          // sum is not finite, it is the sum.  (Selected by value: elements of a vector written under conditions of their own came out of the
+          // compiler as copies of the first.)
+          const f32x4 x = acc[i][j], y = x + (low[0][i][j] + low[1][i][j] * 0x1p-8f) * 0x1p-8f;
+          const auto pick = [](float a, float b) { return fabsf(a) <= 3.402823466e38f ? b : a; };
+          acc[i][j] = f32x4{pick(x[0], y[0]), pick(x[1], y[1]), pick(x[2], y[2]), pick(x[3], y[3])};
+        }
     }
     __syncthreads();
 #endif

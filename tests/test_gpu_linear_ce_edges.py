@@ -36,6 +36,48 @@ def test_an_upstream_value_that_is_not_finite_stays_with_its_token(T, bad, dtype
     assert not bool(torch.isfinite(_run(h, w, y, "none", g)[1]).any())
 
 
+@BOTH
+@pytest.mark.parametrize("T,H,V", [(3, 40, 200), (8, 40, 200), (9, 40, 200), (70, 40, 200), (700, 64, 6001), (2100, 320, 25701)])
+def test_a_class_of_minus_infinity_is_not_there(T, H, V, dtype):
+    """A weight of -inf where every hidden state is positive gives the class no probability, whatever the number of tokens: loss and gradients are those of the
+    vocabulary without it, its own gradient is zero, and only the column of the -inf is lost in dh (0 * inf).  Against 64 bits: every sum here has the same
+    magnitudes as in the other parity tests of the package, rtol 1e-5 of a tensor's largest in float32; in bf16 dl and the gradient are rounded, 2^-8 each."""
+    h, w, y = _inputs(T, H, V, dtype)
+    h[:, 5] = h[:, 5].abs() + 0.25
+    dead = V // 2
+    y[y == dead] = 0
+    w[dead, 5] = float("-inf")
+    loss, dh, dw = _run(h, w, y)
+    alive = torch.arange(V, device="cuda") != dead
+    columns = torch.arange(H, device="cuda") != 5
+    hd, wd = h.double(), w[alive].double()
+    z = hd @ wd.t()
+    lse = torch.logsumexp(z, 1)
+    at, own = torch.arange(T, device="cuda"), torch.where(y > dead, y - 1, y)
+    want = (lse - z[at, own]).mean()
+    d = torch.exp(z - lse[:, None])
+    d[at, own] -= 1
+    d /= T
+    assert abs(float(loss) - float(want)) <= 1e-5 * float(want)
+    tol = 1e-5 if dtype == torch.float32 else 2.0 ** -7
+    for got, ref in ((dh[:, columns], (d @ wd)[:, columns]), (dw[alive], d.t().contiguous() @ hd)):
+        assert float((got.double() - ref).abs().max()) <= tol * float(ref.abs().max())
+    assert not bool(torch.isfinite(dh[:, 5]).any()) and bool((dw[dead] == 0).all())
+
+
+@BOTH
+@pytest.mark.parametrize("T", [3, 9, 200])
+def test_a_hidden_state_that_is_not_finite_is_one_tokens(T, dtype):
+    from causal_eeg_vae_amd import linear_cross_entropy
+    h, w, y = _inputs(T, 72, 700, dtype)
+    clean, dh, _ = _run(h, w, y, "none")
+    h[1, 3] = float("inf")
+    rows, dh1, _ = _run(h, w, y, "none")
+    others = torch.arange(T, device="cuda") != 1
+    assert torch.equal(rows[others], clean[others]) and torch.equal(dh1[others], dh[others]) and not bool(torch.isfinite(rows[1]))
+    assert torch.equal(linear_cross_entropy(h, w, y, reduction="none")[others], clean[others])
+
+
 def test_forward_mode_is_refused():
     """A tangent that would be dropped is an error, with and without anything that asks for a gradient."""
     import torch.autograd.forward_ad as fwd
