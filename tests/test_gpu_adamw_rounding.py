@@ -90,6 +90,12 @@ def test_codes_scales_and_parameters(sizes, dtype):
     _check(sizes, dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_workgroups_of_four_blocks_a_wave(dtype):
+    """8-bit lists of 2^22 elements or more: 4096 elements a workgroup, here with ends inside a block, inside a wave's four blocks and inside a workgroup's."""
+    _check([(1 << 22) + 1001, 4095, 0, 77, 8192 + 256, 5000], dtype)
+
+
 @pytest.mark.parametrize("root", [1.03, 1.0625, 1.18, 1.9])
 def test_the_expectation_of_the_root_is_kept(root):
     """One step of n = 2^20 elements that all come to the same root, between two numbers of e4m3 (low = 8 steps or more, step = 1/8): every new root is one of the
