@@ -21,7 +21,7 @@ using f32x4 = __attribute__((ext_vector_type(4))) float;
 using i32x4 = __attribute__((ext_vector_type(4))) int;
 
 constexpr int PAD = 64;                                  // rows and columns of the packed operands are padded to this with zeros
-constexpr int64_t CE_CAP = (int64_t)1 << 30;             // bytes that the pieces of the backward pass may take together
+constexpr int64_t CE_CAP = (int64_t)1 << 30;             // bytes that a piece of the vocabulary may take, where 256 columns of it take less
 constexpr int CE_SCAN = 4096;                           // tokens whose places a workgroup finds by itself
 constexpr int64_t CE_MAX_PIECE = (int64_t)1 << 20;       // columns per piece: 32-bit offsets inside a tile
 __host__ __device__ constexpr int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }

@@ -586,7 +586,11 @@ int ceeg_neg_sample_uniform_filtered(const int32_t* rowptr, const int32_t* col, 
  * rows of h as the products read them) are written by the forward for the backward.
  * g: what comes back for loss (fp32, [T] or [1]); a value of [T] that is not finite reaches its token's row of dh alone, and all of dW.  dh [T, H] and dW [V, H] contiguous, either may be NULL.
  * Limits: T <= 2^22, H <= 2^15, V <= 2^28, ldw <= 2^22; bf16 with H a multiple of 64 reads W in place: 16-byte aligned, ldw = H.
- * The backward's workspace holds dl for a piece of the vocabulary; pieces are chosen so that they take about 1 GiB at most together.
+ * The backward's workspace holds dl, and W's planes where W is not read in place, for a piece of the vocabulary: a piece has as many columns as fit 1 GiB, and 256
+ * at least.  A column is 2 T' bytes, and 2 H' where W is packed, per plane (CEEG_F32 3, CEEG_BF16 1; ' : up to a multiple of 64), so that from 0.7 million tokens
+ * (bf16: 2.1 million) on 256 columns are more than 1 GiB (T = 2^22: 6.4 and 2.1 GB).  With 256 columns of rounding, the slots of the sums (dh: the larger of
+ * 4 T H bytes and 64 MiB; dW: 128 MiB) and 4 T bytes besides, that is all.  The forward's holds 8 T ceil(V / edge) bytes of statistics (edge 64 to 256, by the
+ * size) and the same pieces of a packed W, up to 1 GiB.
  * ----------------------------------------------------------------------------------------------*/
 size_t ceeg_linear_ce_fwd_ws_bytes(int64_t T, int64_t H, int64_t V, int dtype);
 size_t ceeg_linear_ce_bwd_ws_bytes(int64_t T, int64_t H, int64_t V, int dtype);
