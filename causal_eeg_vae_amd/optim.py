@@ -43,7 +43,7 @@ def _scalar(x, name, dev):
 def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, seed=0):
     """One AdamW step over lists of tensors, in place.
 
-    params and grads: all float32 or all bfloat16, contiguous, one device.  exp_avgs and exp_avg_sqs: float32 tensors, or pairs
+    params and grads: all float32 or all bfloat16, contiguous, one device, each gradient of its parameter's shape.  exp_avgs and exp_avg_sqs: float32 tensors, or pairs
     (codes, scales) as `block_state` makes them, which hold m and sqrt(v) in 8 bits (all tensors alike).  step: the number of this step, from 1.
     step and lr may be float32 tensors of one element on the device, which a captured graph reads anew at every replay.  seed: of the random
     numbers that round 8-bit moments; take another one for every step (with a step tensor it changes by itself)."""
@@ -75,8 +75,9 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9,
     try:   # a call goes through hundreds of small tensors: mapped methods, no loop of attributes
         sizes = list(map(T.numel, params))
         at = params[0].get_device()
+        shapes = list(map(T.size, params))   # a gradient of as many elements in another shape is not this parameter's
         for what, tensors, want in every:
-            if list(map(T.numel, tensors)) != sizes or not all(map(T.is_contiguous, tensors)) or set(map(_dtype_of, tensors)) != {want} or \
+            if (list(map(T.size, tensors)) != shapes if tensors is grads else list(map(T.numel, tensors)) != sizes) or not all(map(T.is_contiguous, tensors)) or set(map(_dtype_of, tensors)) != {want} or \
                     set(map(T.get_device, tensors)) != {at}:
                 raise ValueError(f"{what}: contiguous {want} tensors of the parameters' sizes on {dev} expected, got " +
                                  ", ".join(f"{t.dtype} {tuple(t.shape)} on {t.device}" for t in tensors[:4]))
