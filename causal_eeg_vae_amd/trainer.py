@@ -59,6 +59,8 @@ class Trainer:
         one byte an element (causal_eeg_vae_amd.AdamW)."""
         if optimizer not in ("adam", "adamw"):
             raise ValueError(f"optimizer must be 'adam' or 'adamw', got {optimizer!r}")
+        if optimizer == "adam" and state_bits != 32:
+            raise ValueError(f"state_bits={state_bits} needs optimizer='adamw': adam's moments have 32 bits")
         self.model = model
         self.world_size = int(world_size)
         self.force_exchange = bool(force_exchange)   # broadcast + all-reduce even with one rank (one-GPU RCCL rehearsal)

@@ -12,3 +12,12 @@ def test_adamw_step_refuses_a_gradient_of_another_shape():
             adamw_step_([t(3), p], [t(3), g], [t(3), t(24)], [t(3), t(24)], step=1)
     with pytest.raises(CeegError):      # the right shape gets as far as the device; moments may lie flat
         adamw_step_([t(3), t(4, 6)], [t(3), t(4, 6)], [t(3), t(24)], [t(3), t(24)], step=1)
+
+
+def test_8_bit_moments_need_adamw():
+    """They were asked for and not taken."""
+    from causal_eeg_vae_amd.trainer import Trainer
+    for bits in (8, 16):
+        with pytest.raises(ValueError, match="adamw"):
+            Trainer(torch.nn.Linear(2, 2), state_bits=bits)
+    Trainer(torch.nn.Linear(2, 2), state_bits=32)
