@@ -206,11 +206,11 @@ __global__ __launch_bounds__(256) void ce_prepare_kernel(CeTokens a, const void*
 // joined at the end, small ones first.
 #if defined(__HIP_DEVICE_COMPILE__)
 // 16 bytes a lane from a buffer's base + v into LDS, lane after lane.  Written out because the compiler, which knows that such a load writes LDS, would
-// wait for all of them before every transposing read; run() waits for exactly those it needs.  It has no output register; m0, which the
-// compiler sets right before its own uses, takes a wait state to be read.
+// wait for all of them before every transposing read; run() waits for exactly those it needs.  It has no output register.  m0, the
+// place in LDS, is an input that the compiler sets (and computes in place); it takes a wait state to be read.
 __device__ __forceinline__ void ce_to_lds(i32x4 rsrc, uint32_t v, unsigned short* to) {
   const uint32_t at = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)to);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(v), "s"(rsrc) : "memory");
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"(at), "v"(v), "s"(rsrc) : "memory");
 }
 #endif
 
