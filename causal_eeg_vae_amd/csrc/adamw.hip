@@ -238,6 +238,7 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_kernel(AwList L, AwHyper h) 
       mo[k] = h.b1 * mo[k] + h.omb1 * gv[k];
       vo[k] = h.b2 * vo[k] + h.omb2 * (gv[k] * gv[k]);
       root[k] = sqrtf(vo[k]);
+      // the reciprocal by the instruction alone, a unit (2^-23) off at most: of an update, which is itself lr of a parameter of ordinary size
       pv[k] = pv[k] * decay - step_size * (mo[k] * __builtin_amdgcn_rcpf(root[k] * inv_sqrt_c2 + h.eps));
     }
     aw_store4<FULL, BF16>(p, i, n, vec, pv);

@@ -8,7 +8,10 @@
 //                small ones first - 6/16 of the bf16 rate instead of the 1/16 of the fp32 instruction.
 // Tokens that are ignored are dropped before the first product: their rows are packed away, the grids cover all T tokens and what
 // lies behind the last one that counts leaves at once (its number is read on the device, the host never waits for it).
-// The vocabulary is taken in pieces; of a piece only dl is held (bf16).  A product whose operand runs across the summed axis (W in dh, h and dl in
+// bf16 inputs: dl is rounded to bf16 before both gradient products (half a step, 2^-8 of a value, at most), because the instruction takes bf16 and three planes of it would be
+// three products; the common factor s stays out of it.  What that adds to a gradient (5e-4 to 7e-4 of its rms at the sizes below) is less than the
+// gradient's own rounding to bf16.  lse is one fp32 number: a probability of the backward is off by 2^-24 |lse| of itself.
+// The vocabulary is taken in pieces; of a piece only dl is held.  A product whose operand runs across the summed axis (W in dh, h and dl in
 // dW) reads it through the transposing LDS read, so nothing is ever stored transposed.  No float atomics: the pieces of a sum are added in a fixed order.
 // Measured, bf16, 8192 tokens (7373 count) x 1024 x 131072: statistics 1.73 ms (1.14 PFLOP/s), and per half of the vocabulary dl 1.00 ms (0.99), dh 0.82 ms (1.20),
 // dW 0.80 ms (1.23); 1.13 over all.  fp32, 16384 x 256 x 4096: 212, 247, 179 and 195 us (0.97, 0.83, 1.15, 1.06 PFLOP/s of bf16 products, a sixth of that in fp32).

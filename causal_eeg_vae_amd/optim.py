@@ -57,7 +57,8 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9,
     dtype, dev = params[0].dtype, params[0].device
     if dtype not in _DTYPES:
         raise TypeError(f"parameters must be float32 or bfloat16, got {dtype}")
-    held = not isinstance(exp_avgs[0], torch.Tensor)
+    T = torch.Tensor
+    held = not isinstance(exp_avgs[0], T)
     scales = None
     if held:
         try:
@@ -65,26 +66,27 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9,
         except (TypeError, ValueError):
             raise TypeError("exp_avgs and exp_avg_sqs must be all tensors or all pairs (codes, scales)") from None
         scales = m_scales + v_scales
-        if not all(isinstance(t, torch.Tensor) for t in scales):
-            raise TypeError("exp_avgs and exp_avg_sqs must be all tensors or all pairs (codes, scales)")
+        try:
+            scale_sizes = list(map(T.numel, scales))
+        except TypeError:
+            raise TypeError("exp_avgs and exp_avg_sqs must be all tensors or all pairs (codes, scales)") from None
     else:
         ms, vs = exp_avgs, exp_avg_sqs
     state = torch.float8_e4m3fn if held else torch.float32
     every = (("params", params, dtype), ("grads", grads, dtype), ("exp_avgs", ms, state), ("exp_avg_sqs", vs, state))
-    T = torch.Tensor
     try:   # a call goes through hundreds of small tensors: mapped methods, no loop of attributes
         sizes = list(map(T.numel, params))
         at = params[0].get_device()
         shapes = list(map(T.size, params))   # a gradient of as many elements in another shape is not this parameter's
         for what, tensors, want in every:
-            if (list(map(T.size, tensors)) != shapes if tensors is grads else list(map(T.numel, tensors)) != sizes) or not all(map(T.is_contiguous, tensors)) or set(map(_dtype_of, tensors)) != {want} or \
-                    set(map(T.get_device, tensors)) != {at}:
+            fits = list(map(T.size, tensors)) == shapes if tensors is grads else tensors is params or list(map(T.numel, tensors)) == sizes
+            if not fits or not all(map(T.is_contiguous, tensors)) or set(map(_dtype_of, tensors)) != {want} or set(map(T.get_device, tensors)) != {at}:
                 raise ValueError(f"{what}: contiguous {want} tensors of the parameters' sizes on {dev} expected, got " +
                                  ", ".join(f"{t.dtype} {tuple(t.shape)} on {t.device}" for t in tensors[:4]))
     except TypeError:
         raise ValueError("params, grads, exp_avgs and exp_avg_sqs: tensors expected") from None
     if held:
-        if list(map(T.numel, scales)) != [-(-k // BLOCK) for k in sizes] * 2 or not all(map(T.is_contiguous, scales)) or \
+        if scale_sizes != [-(-k // BLOCK) for k in sizes] * 2 or not all(map(T.is_contiguous, scales)) or \
                 set(map(_dtype_of, scales)) != {torch.float32} or set(map(T.get_device, scales)) != {at}:
             raise ValueError(f"scales: contiguous float32 tensors of one element per {BLOCK} on {dev} expected, got " +
                              ", ".join(f"{t.dtype} {tuple(t.shape)} on {t.device}" for t in scales[:4]))
@@ -92,7 +94,7 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9,
     pp, mp, vp = _addresses(params), _addresses(ms), _addresses(vs)
     sp = _addresses(scales) if held else []
     where = pp + mp + vp + sp
-    if len(set(where) - {0}) < len(where) - where.count(0):   # an empty tensor has no address
+    if len(set(where)) < len(where) and len(set(where) - {0}) < len(where) - where.count(0):   # an empty tensor has no address
         raise ValueError("a tensor that the step writes is given twice")
     b1, b2 = betas
     step_t, lr_t = _scalar(step, "step", dev), _scalar(lr, "lr", dev)
