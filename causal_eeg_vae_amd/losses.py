@@ -22,6 +22,12 @@ def _same_device(*tensors):
         raise ValueError(f"all tensors must be on one device, got {[str(t.device) for t in tensors if t is not None]}")
 
 
+def _came_back(t, shape, dtype, dev):
+    """A saved tensor comes back through a hook with its values in other strides, perhaps; not as something else, whose memory would be read as the old one's."""
+    if t.shape != shape or t.dtype != dtype or t.device != dev:
+        raise ValueError(f"a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}, not as {dtype} {tuple(shape)} on {dev}")
+
+
 def _has_tangent(t):
     return torch.autograd.forward_ad.unpack_dual(t).tangent is not None
 
@@ -57,7 +63,7 @@ def _linear_ce(hidden, weight, target, ignore_index, reduction):
             _lib.check(L.ceeg_linear_ce_fwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, target.data_ptr(), T, H, V, dtype, ignore_index, reduction,
                                             loss.data_ptr(), lse, tokens, packed, ws.data_ptr(), ws.numel(), _lib.stream()),
                        "ceeg_linear_ce_fwd")
-    return loss, kept, weight, (T, H, V, dtype, reduction, rows)
+    return loss, kept, weight, (T, H, V, dtype, reduction, rows, kept.numel())
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
@@ -71,9 +77,11 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         kept, weight = ctx.saved_tensors
-        T, H, V, dtype, reduction, rows = ctx.sizes
+        T, H, V, dtype, reduction, rows, kept_bytes = ctx.sizes
         L = _lib.lib()
         # saved tensors may come back through a hook as other tensors of the same values: strides and alignment are theirs, not those of the forward
+        _came_back(weight, (V, H), torch.float32 if dtype == _lib.CEEG_F32 else torch.bfloat16, g.device)
+        _came_back(kept, (kept_bytes,), torch.uint8, g.device)
         weight, ldw = _weight_rows(weight, dtype)
         if kept.data_ptr() % 256 or not kept.is_contiguous():
             kept = kept.clone(memory_format=torch.contiguous_format)
@@ -166,6 +174,10 @@ class _Balance(torch.autograd.Function):
         T, E, dtype = ctx.sizes
         dev = scores.device
         # saved tensors may come back through a hook as other tensors of the same values: strides are theirs, not those of the forward
+        _came_back(scores, (T, E), torch.float32 if dtype == _lib.CEEG_F32 else torch.bfloat16, g.device)
+        _came_back(stats, (E + 1,), torch.float32, g.device)
+        if mask is not None:
+            _came_back(mask, (T,), torch.bool, g.device)
         scores, ld = _score_rows(scores)
         mask, stats = None if mask is None else mask.contiguous(), stats.contiguous()
         with _lib.on(dev):

@@ -79,3 +79,26 @@ def test_balance_loss(library, back, dtype):
         torch.autograd.grad(loss, s)
     scores, ld = library.calls["ceeg_balance_bwd"][:2]
     assert _inside(scores, ld, T, E, seen[-1])
+
+
+@pytest.mark.parametrize("back", [lambda x: x.half(), lambda x: x[:-1].clone(), lambda x: x.reshape(-1, 1).clone()], ids=["type", "short", "shape"])
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_another_tensor_is_refused(library, back, which):
+    """`which`: of the saved tensors, in their order.  Nothing is launched on what is not the saved tensor."""
+    from causal_eeg_vae_amd import balance_loss, linear_cross_entropy
+    x = torch.zeros(50, 8, requires_grad=True)
+    for entry, loss in (("ceeg_linear_ce_bwd", lambda: linear_cross_entropy(torch.zeros(7, 8), x, torch.zeros(7, dtype=torch.int64))),
+                        ("ceeg_balance_bwd", lambda: balance_loss(x, torch.zeros(50, dtype=torch.int64), torch.ones(50, dtype=torch.bool))[0])):
+        if which == 2 and entry == "ceeg_linear_ce_bwd":
+            continue
+        seen = []
+
+        def pack(t):
+            seen.append(t)
+            return len(seen) - 1
+
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda k: back(seen[k]) if k == which else seen[k]):
+            out = loss()
+        with pytest.raises(ValueError, match="came back"):
+            torch.autograd.grad(out, x)
+        assert entry not in library.calls
