@@ -8,8 +8,8 @@
 // 16 random bits of Philox per value.  sqrt(v) > 0 never becomes 0: a denominator that vanishes while m does not would blow the next step up.
 // Bound: HBM bytes (fp32 28 per element; 8 bits 16 with fp32 parameters, 10 with bf16).  A wave takes one block of 256 elements, 4 per lane - 16-byte loads, the
 // block's maximum by one butterfly, one Philox call per lane for its four elements - so the 8-bit form needs no LDS and no barrier.
-// Measured, 66 M elements in 148 tensors: 32 bits 347 us (5.3 TB/s); 8 bits 244 us (4.3 TB/s: vector instructions, about 140 an element, are as long as the bytes), with 50 M
-// bf16 parameters 156 us (3.2 TB/s).
+// Measured, 66 M elements in 148 tensors: 32 bits 347 us (5.3 TB/s); 8 bits 238 us (4.4 TB/s: vector instructions, about 120 an element, are as long as the bytes), with 50 M
+// bf16 parameters 145 us (3.5 TB/s; 130 instructions).
 // The tensors' pointers travel in the kernel arguments: no table in device memory, nothing to copy or to keep alive.
 #include <math.h>
 #include "ceeg_internal.h"
@@ -327,8 +327,9 @@ extern "C" int ceeg_adamw_step(int tensors, const int64_t* numel, void* const* p
   h.b1d = step_dev ? beta1 : 1.0 / c1; h.b2d = beta2; h.lrd = lr; h.wdd = weight_decay;
   h.step_dev = step_dev; h.lr_dev = lr_dev;
   h.seed = seed;
-  // Elements per workgroup.  One block per wave fills the compute units soonest and balances them best (32 bits, 148 tensors of 66 M together: 354 us, 377 with 4096; 8 bits,
-  // 1 M: 8.0 us instead of 9.8).  The longer start of 8 bits is worth four blocks a wave from 4 M on (148 tensors of 66 M: 244 us instead of 267, 250 with 8192).
+  // Elements per workgroup.  One block per wave fills the compute units soonest and balances them best (32 bits, 148 tensors of 66 M together: 352 us, 379 with 4096; 8 bits,
+  // 1 M: 7.9 us instead of 9.2, 2 M 12.4 and 12.7).  The longer start of 8 bits is worth four blocks a wave from 4 M on (one tensor of 4 M: 19.6 us instead of 20.9, 8192 21.3;
+  // 148 tensors of 66 M: 235 us instead of 266, 238 with 8192).
   h.per_wg = state_bits == 8 && total >= (int64_t)1 << 22 ? 4096 : 1024;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   for (int t = 0; t < tensors;) {

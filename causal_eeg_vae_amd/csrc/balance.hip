@@ -5,7 +5,7 @@
 // lanes, 16-byte loads where the rows allow them), its softmax is two butterflies; the column sums of p stay in registers over all rows
 // of a wave, because a lane keeps its columns, and are joined over waves and workgroups in a fixed order: no float atomics.  The counts are
 // integer LDS atomics, whose order does not matter.
-// Measured, fp32, 262144 x 512, one code a row: row pass 141 us (3.8 TB/s, what a pass that only reads reaches), joins 10 + 5, gradient 192 us (5.6 TB/s).
+// Measured, fp32, 262144 x 512, one code a row: row pass 134 us (4.0 TB/s, what a pass that only reads reaches), joins 9 + 5, gradient 189 us (5.7 TB/s).
 #include "ceeg_internal.h"
 
 namespace {

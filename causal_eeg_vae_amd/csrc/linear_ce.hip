@@ -9,12 +9,13 @@
 // Tokens that are ignored are dropped before the first product: their rows are packed away, the grids cover all T tokens and what
 // lies behind the last one that counts leaves at once (its number is read on the device, the host never waits for it).
 // bf16 inputs: dl is rounded to bf16 before both gradient products (half a step, 2^-8 of a value, at most), because the instruction takes bf16 and three planes of it would be
-// three products; the common factor s stays out of it.  What that adds to a gradient (5e-4 to 7e-4 of its rms at the sizes below) is less than the
-// gradient's own rounding to bf16.  lse is one fp32 number: a probability of the backward is off by 2^-24 |lse| of itself.
+// three products; the common factor s stays out of it.  A gradient is 5e-4 to 7e-4 of its rms off one from an fp32 dl at
+// the sizes below, 2e-3 at small ones; its own rounding to bf16 is 1.1e-3 to 2.3e-3.  lse is one fp32 number: a probability of the backward is off by 2^-24 |lse| of itself.
 // The vocabulary is taken in pieces; of a piece only dl is held.  A product whose operand runs across the summed axis (W in dh, h and dl in
 // dW) reads it through the transposing LDS read, so nothing is ever stored transposed.  No float atomics: the pieces of a sum are added in a fixed order.
-// Measured, bf16, 8192 tokens (7373 count) x 1024 x 131072: statistics 1.73 ms (1.14 PFLOP/s), and per half of the vocabulary dl 1.00 ms (0.99), dh 0.82 ms (1.20),
-// dW 0.80 ms (1.23); 1.13 over all.  fp32, 16384 x 256 x 4096: 212, 247, 179 and 195 us (0.97, 0.83, 1.15, 1.06 PFLOP/s of bf16 products, a sixth of that in fp32).
+// Measured, bf16, 8192 tokens (7373 count) x 1024 x 131072: statistics 1.73 ms (1.14 PFLOP/s), and per half of the vocabulary dl 0.96 ms (1.03), dh 0.81 ms (1.21),
+// dW 0.81 ms (1.23); 1.13 over all, the recomputed logits counted, 0.85 without.  fp32, 16384 x 256 x 4096: 197, 226, 188 and 166 us (1.05, 0.91, 1.10, 1.24 PFLOP/s of bf16
+// products, a sixth of that in fp32).
 #include <limits.h>
 #include "ceeg_internal.h"
 
@@ -116,7 +117,7 @@ __global__ __launch_bounds__(1024) void ce_tokens_kernel(CeTokens a) { ce_scan<1
 
 // ------------------------------------------------------------------------------------------------ planes
 // Where element (r, c) of a blocked matrix of C columns is: blocks of 16 rows x 32 columns, each one piece of 1 KB, so that a tile's loads are whole cache lines whichever way the tile
-// lies.  Rows of 32 columns from a row-major matrix are half lines: twice the requests, which bound the products (the L2 took two thirds of the requests it can).
+// lies.  Rows of 32 columns from a row-major matrix are half lines, twice the requests: 3 to 5 % of the products' time.
 __host__ __device__ __forceinline__ int64_t ce_place(int64_t r, int c, int64_t C) { return ((r >> 4) * (C >> 5) + (c >> 5)) * 512 + (r & 15) * 32 + (c & 31); }
 
 // eight columns c.. of a row of C at `src` (NULL: zeros) -> the planes at out
@@ -655,7 +656,8 @@ __global__ __launch_bounds__(1024) void ce_loss_kernel(const int32_t* __restrict
 // ------------------------------------------------------------------------------------------------ few tokens
 // The statistics of up to R tokens against W read once as it is (no planes, no padding, fp32 multiply-adds): bound by W's bytes.  16 lanes take four rows of W, a wave sixteen, a
 // workgroup FEW of them; the hidden rows are in LDS in fp32, read once for the four rows; two pieces of 16 bytes of each row are on their way.  A last workgroup
-// does what ce_prepare_kernel does meanwhile.  One token x 768 x 50257: bf16 16.4 us (4.7 TB/s); with the join in fp32 30 us, in bf16 20.
+// does what ce_prepare_kernel does meanwhile.  One token x 768 x 50257: bf16 15.6 us (4.9 TB/s, W
+// in the 256 MB cache from the call before); with the join in fp32 30 us, in bf16 19.0, and 21.6 where the weights of twelve calls take turns and W comes from memory.
 constexpr int CE_FEW = 64;             // classes of a workgroup
 constexpr int CE_FEW_TOKENS = 8;
 constexpr int CE_FEW_LDS = 48 * 1024;  // bytes of hidden rows
@@ -1075,7 +1077,7 @@ struct CePlan {
 };
 
 // Up to eight tokens in fp32, two in bf16: the tiles' time hardly depends on how few there are, as they first make planes of W (fp32) or pad it (bf16 of an H that is no multiple
-// of 64).  768 x 50257: fp32 1 token 30 us, tiles 134; 8 tokens 48 and 139; bf16 1 token 19.2 and 28.5, 4 tokens 28.6 and 29.2, 8 tokens 41 and 30.
+// of 64).  768 x 50257: fp32 1 token 30 us, tiles 134; 8 tokens 48 and 139; bf16 1 token 19.0 and 28.5, 4 tokens 28.6 and 29.2, 8 tokens 41 and 30.
 size_t ce_few_lds(int few, int64_t H, int dtype) { return (size_t)few * up(H, dtype == CEEG_F32 ? 128 : 256) * 4; }
 int ce_few(int64_t T, int64_t H, int dtype) {
   if (T > (dtype == CEEG_F32 ? CE_FEW_TOKENS : 2)) return 0;

@@ -2,6 +2,7 @@
 scripts/gpt2.py:1080-1084 and scripts/models.py:34, over the hidden states of the caller's language decoder) and the balance loss over an
 assignment to codes or experts.  The kernels are ceeg_linear_ce_fwd / _bwd and ceeg_balance_fwd / _bwd (include/ceeg.h)."""
 import torch
+import torch.autograd.forward_ad as _forward
 
 from . import _lib
 
@@ -22,14 +23,20 @@ def _same_device(*tensors):
         raise ValueError(f"all tensors must be on one device, got {[str(t.device) for t in tensors if t is not None]}")
 
 
-def _came_back(t, shape, dtype, dev):
-    """A saved tensor comes back through a hook with its values in other strides, perhaps; not as something else, whose memory would be read as the old one's."""
-    if t.shape != shape or t.dtype != dtype or t.device != dev:
-        raise ValueError(f"a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}, not as {dtype} {tuple(shape)} on {dev}")
+def _like(*tensors):
+    """Type, shape and device of saved tensors.  Through a hook they come back with their values in other strides, perhaps; as something else they are refused, as its
+    memory would be read as the old one's."""
+    return [None if t is None else (t.dtype, t.shape, t.get_device()) for t in tensors]
 
 
-def _has_tangent(t):
-    return torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+def _came_back(tensors, like):
+    if _like(*tensors) != like:
+        raise ValueError(f"saved tensors came back as {_like(*tensors)}, not as {like}")
+
+
+def _has_tangent(*tensors):
+    """Inside a level of forward mode (where there is none, nothing has one): whether one of them carries a tangent."""
+    return _forward._current_level >= 0 and any(_forward.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _weight_rows(weight, dtype):
@@ -63,7 +70,7 @@ def _linear_ce(hidden, weight, target, ignore_index, reduction):
             _lib.check(L.ceeg_linear_ce_fwd(hidden.data_ptr(), ldh, weight.data_ptr(), ldw, target.data_ptr(), T, H, V, dtype, ignore_index, reduction,
                                             loss.data_ptr(), lse, tokens, packed, ws.data_ptr(), ws.numel(), _lib.stream()),
                        "ceeg_linear_ce_fwd")
-    return loss, kept, weight, (T, H, V, dtype, reduction, rows, kept.numel())
+    return loss, kept, weight, (T, H, V, dtype, reduction, rows)
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
@@ -71,17 +78,17 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, hidden, weight, target, ignore_index, reduction):
         loss, kept, weight, ctx.sizes = _linear_ce(hidden, weight, target, ignore_index, reduction)
         ctx.save_for_backward(kept, weight)
+        ctx.like = _like(kept, weight)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        kept, weight = ctx.saved_tensors
-        T, H, V, dtype, reduction, rows, kept_bytes = ctx.sizes
+        saved = kept, weight = ctx.saved_tensors
+        T, H, V, dtype, reduction, rows = ctx.sizes
         L = _lib.lib()
         # saved tensors may come back through a hook as other tensors of the same values: strides and alignment are theirs, not those of the forward
-        _came_back(weight, (V, H), torch.float32 if dtype == _lib.CEEG_F32 else torch.bfloat16, g.device)
-        _came_back(kept, (kept_bytes,), torch.uint8, g.device)
+        _came_back(saved, ctx.like)
         weight, ldw = _weight_rows(weight, dtype)
         if kept.data_ptr() % 256 or not kept.is_contiguous():
             kept = kept.clone(memory_format=torch.contiguous_format)
@@ -127,8 +134,10 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
     if target.numel() == 0:  # no token: nothing to launch, the gradients are zero
         none = hidden.float().sum(-1) + weight[:0].float().sum()
         return none if reduction == "none" else none.sum()
-    args = hidden.reshape(-1, hidden.shape[-1]), weight, target.reshape(-1), int(ignore_index), _REDUCTIONS[reduction]
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad) or _has_tangent(hidden) or _has_tangent(weight):
+    if hidden.dim() != 2:   # rows of a matrix go in as they are: a view would be another node of the graph
+        hidden = hidden.reshape(-1, hidden.shape[-1])
+    args = hidden, weight, target.reshape(-1), int(ignore_index), _REDUCTIONS[reduction]
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad) or _has_tangent(hidden, weight):
         loss = _LinearCrossEntropy.apply(*args)   # which refuses forward mode
     else:  # nothing comes back: autograd's part of the call is left out
         loss = _linear_ce(*args)[0]
@@ -138,9 +147,11 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
 def _score_rows(scores):
     """(scores, row stride) as the entries take them."""
     T, E = scores.shape
-    if scores.stride(1) != 1 or (T > 1 and scores.stride(0) < E):
+    row, column = scores.stride()
+    if column != 1 or (T > 1 and row < E):
         scores = scores.contiguous()
-    return scores, max(scores.stride(0), E)
+        row = scores.stride(0)
+    return scores, max(row, E)
 
 
 class _Balance(torch.autograd.Function):
@@ -154,7 +165,7 @@ class _Balance(torch.autograd.Function):
         indices = indices.contiguous()
         mask = None if mask is None else mask.contiguous()
         with _lib.on(dev):
-            loss = torch.empty(1, dtype=torch.float32, device=dev)
+            loss = torch.empty((), dtype=torch.float32, device=dev)
             counts = torch.empty(E, dtype=torch.int64, device=dev)
             stats = torch.empty(E + 1, dtype=torch.float32, device=dev)
             ws = _lib.workspace(L.ceeg_balance_ws_bytes(T, E), dev)
@@ -163,26 +174,24 @@ class _Balance(torch.autograd.Function):
                                               loss.data_ptr(), counts.data_ptr(), stats.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream()),
                            "ceeg_balance_fwd")
         ctx.save_for_backward(scores, mask, stats)
+        ctx.like = _like(scores, mask, stats)
         ctx.sizes = T, E, dtype
         ctx.mark_non_differentiable(counts)
-        return loss[0], counts
+        return loss, counts
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _g_counts):
-        scores, mask, stats = ctx.saved_tensors
+        saved = scores, mask, stats = ctx.saved_tensors
         T, E, dtype = ctx.sizes
         dev = scores.device
         # saved tensors may come back through a hook as other tensors of the same values: strides are theirs, not those of the forward
-        _came_back(scores, (T, E), torch.float32 if dtype == _lib.CEEG_F32 else torch.bfloat16, g.device)
-        _came_back(stats, (E + 1,), torch.float32, g.device)
-        if mask is not None:
-            _came_back(mask, (T,), torch.bool, g.device)
+        _came_back(saved, ctx.like)
         scores, ld = _score_rows(scores)
         mask, stats = None if mask is None else mask.contiguous(), stats.contiguous()
         with _lib.on(dev):
             g = g.to(torch.float32).contiguous()
-            ds = torch.empty(T, E, dtype=scores.dtype, device=dev)
+            ds = scores.new_empty((T, E))
             with _lib.timed("balance_bwd"):
                 _lib.check(_lib.lib().ceeg_balance_bwd(scores.data_ptr(), ld, dtype, T, E, _lib.ptr(mask), stats.data_ptr(), g.data_ptr(), ds.data_ptr(),
                                                        _lib.stream()), "ceeg_balance_bwd")
