@@ -23,15 +23,10 @@ def _same_device(*tensors):
         raise ValueError(f"all tensors must be on one device, got {[str(t.device) for t in tensors if t is not None]}")
 
 
-def _like(*tensors):
-    """Type, shape and device of saved tensors.  Through a hook they come back with their values in other strides, perhaps; as something else they are refused, as its
-    memory would be read as the old one's."""
-    return [None if t is None else (t.dtype, t.shape, t.get_device()) for t in tensors]
-
-
-def _came_back(tensors, like):
-    if _like(*tensors) != like:
-        raise ValueError(f"saved tensors came back as {_like(*tensors)}, not as {like}")
+def _came_back(t, shape, dtype, dev):
+    """A saved tensor comes back through a hook with its values in other strides, perhaps; as something else it is refused: its memory would be read as the old one's."""
+    if t.shape != shape or t.dtype != dtype or t.device != dev:
+        raise ValueError(f"a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}, not as {dtype} {tuple(shape)} on {dev}")
 
 
 def _has_tangent(*tensors):
@@ -78,21 +73,22 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, hidden, weight, target, ignore_index, reduction):
         loss, kept, weight, ctx.sizes = _linear_ce(hidden, weight, target, ignore_index, reduction)
         ctx.save_for_backward(kept, weight)
-        ctx.like = _like(kept, weight)
+        ctx.saved_as = kept.shape, weight.shape, weight.dtype, weight.device
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        saved = kept, weight = ctx.saved_tensors
+        kept, weight = ctx.saved_tensors
         T, H, V, dtype, reduction, rows = ctx.sizes
         L = _lib.lib()
         # saved tensors may come back through a hook as other tensors of the same values: strides and alignment are theirs, not those of the forward
-        _came_back(saved, ctx.like)
+        kept_shape, shape, saved_type, dev = ctx.saved_as
+        _came_back(kept, kept_shape, torch.uint8, dev)
+        _came_back(weight, shape, saved_type, dev)
         weight, ldw = _weight_rows(weight, dtype)
         if kept.data_ptr() % 256 or not kept.is_contiguous():
             kept = kept.clone(memory_format=torch.contiguous_format)
-        dev = weight.device
         need_h, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         with _lib.on(dev):
             g = g.to(torch.float32).contiguous()
@@ -173,25 +169,27 @@ class _Balance(torch.autograd.Function):
                 _lib.check(L.ceeg_balance_fwd(scores.data_ptr(), ld, dtype, indices.data_ptr(), indices.element_size(), T, E, K, _lib.ptr(mask),
                                               loss.data_ptr(), counts.data_ptr(), stats.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream()),
                            "ceeg_balance_fwd")
-        ctx.save_for_backward(scores, mask, stats)
-        ctx.like = _like(scores, mask, stats)
-        ctx.sizes = T, E, dtype
+        ctx.save_for_backward(scores, mask)
+        ctx.sizes, ctx.stats = (T, E, dtype), stats
+        ctx.saved_as = scores.shape, scores.dtype, dev
         ctx.mark_non_differentiable(counts)
         return loss, counts
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _g_counts):
-        saved = scores, mask, stats = ctx.saved_tensors
-        T, E, dtype = ctx.sizes
-        dev = scores.device
+        scores, mask = ctx.saved_tensors
+        (T, E, dtype), stats = ctx.sizes, ctx.stats
         # saved tensors may come back through a hook as other tensors of the same values: strides are theirs, not those of the forward
-        _came_back(saved, ctx.like)
+        shape, saved_type, dev = ctx.saved_as
+        _came_back(scores, shape, saved_type, dev)
         scores, ld = _score_rows(scores)
-        mask, stats = None if mask is None else mask.contiguous(), stats.contiguous()
+        if mask is not None:
+            _came_back(mask, (T,), torch.bool, dev)
+            mask = mask.contiguous()
         with _lib.on(dev):
             g = g.to(torch.float32).contiguous()
-            ds = scores.new_empty((T, E))
+            ds = torch.empty(T, E, dtype=scores.dtype, device=dev)
             with _lib.timed("balance_bwd"):
                 _lib.check(_lib.lib().ceeg_balance_bwd(scores.data_ptr(), ld, dtype, T, E, _lib.ptr(mask), stats.data_ptr(), g.data_ptr(), ds.data_ptr(),
                                                        _lib.stream()), "ceeg_balance_bwd")

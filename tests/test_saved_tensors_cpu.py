@@ -82,15 +82,13 @@ def test_balance_loss(library, back, dtype):
 
 
 @pytest.mark.parametrize("back", [lambda x: x.half(), lambda x: x[:-1].clone(), lambda x: x.reshape(-1, 1).clone()], ids=["type", "short", "shape"])
-@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("which", [0, 1])
 def test_another_tensor_is_refused(library, back, which):
     """`which`: of the saved tensors, in their order.  Nothing is launched on what is not the saved tensor."""
     from causal_eeg_vae_amd import balance_loss, linear_cross_entropy
     x = torch.zeros(50, 8, requires_grad=True)
     for entry, loss in (("ceeg_linear_ce_bwd", lambda: linear_cross_entropy(torch.zeros(7, 8), x, torch.zeros(7, dtype=torch.int64))),
                         ("ceeg_balance_bwd", lambda: balance_loss(x, torch.zeros(50, dtype=torch.int64), torch.ones(50, dtype=torch.bool))[0])):
-        if which == 2 and entry == "ceeg_linear_ce_bwd":
-            continue
         seen = []
 
         def pack(t):
