@@ -489,6 +489,10 @@ __device__ __forceinline__ float ce_exp(float x, float base) {
   constexpr float LOG2E = 1.44269504088896341f;
   return __builtin_amdgcn_exp2f(PL == 1 ? __fmaf_rn(x, LOG2E, -base * LOG2E) : (x - base) * LOG2E);
 }
+// bf16: a base whose product with log2(e) may overflow takes fp32's form, in its own lane: the other tokens' numbers do not depend on it
+__device__ __forceinline__ bool ce_far(float base) { return fabsf(base) > 0x1p126f; }
+template <int PL, bool FAR>
+__device__ __forceinline__ float ce_exp_of(float x, float base) { return FAR && ce_far(base) ? ce_exp<3>(x, base) : ce_exp<PL>(x, base); }
 
 // four consecutive values of a row of H (left: how many of them there are), in the output's type
 template <bool F32>
@@ -573,10 +577,14 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_stats_kernel(CeMat W, CeMat 
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float base = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
+    const auto add = [&](auto far) {
 #pragma unroll
-    for (int i = 0; i < G::MT; ++i)
+      for (int i = 0; i < G::MT; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum += ce_exp<PL>(g.acc[i][j][k], base);
+        for (int k = 0; k < 4; ++k) sum += ce_exp_of<PL, far.value>(g.acc[i][j][k], base);
+    };
+    if (PL == 1 && __any(ce_far(base))) add(Int<1>{});
+    else add(Int<0>{});
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
     if (q == 0) s[wm * BN + cl] = make_float2(top, sum);
@@ -768,7 +776,7 @@ __global__ __launch_bounds__(256, R == 1 ? 4 : R == 2 ? 3 : 2) void ce_few_kerne
       const float base = top == -INFINITY ? 0.f : top;
       float sum = 0.f;
 #pragma unroll
-      for (int u = 0; u < U; ++u) sum += ce_exp<F32 ? 3 : 1>(acc[u][r], base);
+      for (int u = 0; u < U; ++u) sum += ce_exp_of<F32 ? 3 : 1, !F32>(acc[u][r], base);
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
       if (lane == 0) s_wave[wave][r] = make_float2(top, sum);
@@ -862,10 +870,14 @@ __global__ __launch_bounds__(G::THREADS, 1) void ce_dlogits_kernel(CeMat W, CeMa
     const int t = n0 + (wn * G::NT + j) * 16 + (lane & 15);
     const int class_t = t < N ? yc[t] : -1, y = class_t - v0 - vb;
     const float l = t < N ? lse[t] : 0.f, rt = t < N ? scale.row(t, class_t) : 0.f;
+    const auto set = [&](auto far) {
 #pragma unroll
-    for (int i = 0; i < G::MT; ++i)
+      for (int i = 0; i < G::MT; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) g.acc[i][j][k] = rt * ce_exp<PL>(g.acc[i][j][k], l);
+        for (int k = 0; k < 4; ++k) g.acc[i][j][k] = rt * ce_exp_of<PL, far.value>(g.acc[i][j][k], l);
+    };
+    if (PL == 1 && __any(ce_far(l))) set(Int<1>{});
+    else set(Int<0>{});
     if (__any(y >= 0 && y < G::MT * 16)) {
 #pragma unroll
       for (int i = 0; i < G::MT; ++i)

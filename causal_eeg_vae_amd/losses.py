@@ -110,7 +110,7 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
     `ignore_index` (padding) take no part, whatever their hidden row holds.  reduction: "mean" over the tokens that count (0 where none does),
     "sum", or "none" (target's shape, 0 where ignored).  The loss is float32; the gradients have their inputs' types, all sums are float32.
     bfloat16: the gradient of the logits is rounded to bfloat16 before the two products that it enters (2^-8 of a value at most), and the gradients are
-    rounded again.  A probability in the backward is off by about 2^-24 |log sum exp| of itself, logits beyond 1e38 are not provided for.
+    rounded again.  A probability in the backward is off by about 2^-24 |log sum exp| of itself.
     A target outside [0, V) makes the loss and the gradients it reaches NaN: an error would need a host read of the targets.
     There is no forward mode: a tangent is a NotImplementedError."""
     if not all(isinstance(t, torch.Tensor) for t in (hidden, weight, target)):

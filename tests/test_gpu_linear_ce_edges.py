@@ -78,6 +78,35 @@ def test_a_hidden_state_that_is_not_finite_is_one_tokens(T, dtype):
     assert torch.equal(linear_cross_entropy(h, w, y, reduction="none")[others], clean[others])
 
 
+@BOTH
+@pytest.mark.parametrize("T,H,V", [(1, 64, 200), (2, 64, 200), (9, 40, 200), (70, 64, 3000), (700, 64, 6001), (2100, 320, 25701)])
+def test_the_largest_logits_there_are(T, H, V, dtype):
+    """One class with a logit near the largest float32 takes all the probability: a token's loss is that logit (its own is gone in the rounding: 2^-24 of it, four of them), 0 where it is
+    the target, and the gradient of the logits the difference of two ones.  Every product is a bf16 or float32 number times 1, but for the store (eps / 2) and 2^-22 of fp32 sums
+    of up to T terms.  Logits that are all near the least one give losses from 0 to log V."""
+    h, w, y = _inputs(T, H, V, dtype)
+    h[:, 0] = 1.0
+    top = V - 2
+    w[top, 0] = 3e38
+    y[T // 2:] = 1
+    y[0] = top
+    rows, _, _ = _run(h, w, y, "none")
+    big = w[top, 0].double()
+    want = torch.where(y == top, torch.zeros_like(big), big)
+    assert bool(((rows.double() - want).abs() <= 2.0 ** -22 * big * (y != top)).all())
+    loss, dh, dw = _run(h, w, y)
+    assert abs(float(loss) - float(want.mean())) <= 2.0 ** -21 * float(big)
+    d = torch.zeros(T, V, dtype=torch.float64, device="cuda")
+    d[:, top] = 1
+    d[torch.arange(T, device="cuda"), y] -= 1
+    d /= T
+    for got, ref, size in ((dh, d @ w.double(), d.abs() @ w.double().abs()), (dw, d.t().contiguous() @ h.double(), d.abs().t().contiguous() @ h.double().abs())):
+        assert bool(((got.double() - ref).abs() <= (2.0 ** -22 + T * 2.0 ** -24) * size + torch.finfo(dtype).eps / 2 * ref.abs()).all())
+    w[:, 0] = -3e38
+    rows = _run(h, w, y, "none")[0]
+    assert bool(((rows >= 0) & (rows <= torch.log(torch.tensor(float(V))) * 1.001)).all())
+
+
 def test_forward_mode_is_refused():
     """A tangent that would be dropped is an error, with and without anything that asks for a gradient."""
     import torch.autograd.forward_ad as fwd
